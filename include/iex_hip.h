@@ -443,6 +443,61 @@ int iex_sparse_attention_fits(int dtype, int head_dim, int tokens);
 int iex_sparse_attention(int dtype, int heads, int tokens, int head_dim, int nonzeros, const int* row_offsets, const void* q,
                          const void* k, const void* v, float scale, void* out, const void* tables, size_t bytes, void* stream);
 
+/* ---- a paged cache of keys and values, and single new tokens attending to it (no counterpart in the reference) ----
+ * keys, values: (pages, kv_heads, page_size, head_dim), a page's elements contiguous, pages `*_page_stride` elements apart; of
+ * type `dtype`, or (eight_bits) e4m3 codes whose rows have an exponent each: (pages, kv_heads, page_size), value = code *
+ * 2^(exponent - 127).  table: the pages of every sequence, (seqs, table_width) with rows table_stride apart; lengths: tokens of
+ * every sequence (int32).  bounds (may be null): smallest and largest stored key per page, head and feature, (pages, kv_heads, 2,
+ * head_dim) of type `dtype`.  Tables and lengths are read on the device at every call (a replayed graph follows them); a length
+ * is cut to what the table holds, a page outside the cache counts as given back: nothing is written to it and nothing of it is
+ * attended to.  Heads of 64, 128 or 256; pages of 16, 32, 64, 128 or 256 tokens; fp16 and bf16. */
+typedef struct iex_paged_cache {
+  int dtype, eight_bits;
+  int pages, page_size, kv_heads, head_dim;
+  long long key_page_stride, value_page_stride;
+  void* keys;
+  void* values;
+  unsigned char* key_exponents;
+  unsigned char* value_exponents;
+  void* bounds;
+  const int* table;
+  int seqs, table_width;
+  long long table_stride;
+  const int* lengths;
+} iex_paged_cache;
+
+/* New tokens' keys and values into the cache; keys and queries are rotated by position on the way.  Tokens offsets[s] ..
+ * offsets[s + 1] (offsets[0] = 0; null: token s) are the newest of the lengths[s] tokens that sequence s then has.  k, v: (tokens,
+ * kv_heads, head_dim), q and q_out: (tokens, heads, head_dim), any strides (token, head, feature; elements), heads == 0: no queries.
+ * rotation: (positions, rotary) fp32, rotary / 2 cosines and as many sines of a position, a row for every position that the table
+ * can hold; the first `rotary` features (a multiple of 16, 0: none) turn in pairs (j, j + rotary / 2), or (2j, 2j + 1) where
+ * interleaved.  A sequence longer than its table or shorter than its new tokens is passed over, tokens behind the last
+ * sequence's too: nothing is written to the cache, their rows of q_out are zeros.  Two sequences that append to the same page
+ * in one call leave one of the two in it.  In an 8-bit cache infinities become NaN. */
+int iex_kv_append(const iex_paged_cache* cache, int tokens, const int* offsets, int heads, const void* k, const long long* k_strides,
+                  const void* v, const long long* v_strides, const void* q, const long long* q_strides, void* q_out,
+                  const long long* q_out_strides, const float* rotation, int positions, int rotary, int interleaved, void* stream);
+
+/* out[s, h] = softmax over the tokens of sequence s (scale * q[s, h] . key) value; heads / kv_heads query heads share a key
+ * head.  q, out: (seqs, heads, head_dim), any strides (sequence, head, feature).  listed (null: every page): (seqs, kv_heads,
+ * count), the pages of the sequence's table to attend to; entries outside the table (-1) are passed over, one that comes twice
+ * counts twice.  No token to attend to: zeros.  The sequences are split over their lengths; the parts meet in `workspace`
+ * (iex_paged_attention_workspace_bytes, 0: none; 256-byte aligned), which the call uses until its work on the stream has run.
+ * What is not attended to leaves no trace, infinities and NaN included.  scale > 0. */
+size_t iex_paged_attention_workspace_bytes(const iex_paged_cache* cache, int heads, int count);
+int iex_paged_attention(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, float scale,
+                        const int* listed, int count, void* out, const long long* out_strides, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* out: (seqs, kv_heads, count), the `count` pages of every sequence's table whose keys can score highest with the query heads of
+ * a key head, in ascending order, -1 behind them where there are fewer: the first `first` and last `last` pages that the
+ * sequence uses, then by score = sum over the group's heads and the features of max(q lo, q hi), summed in 64 bits and rounded
+ * once to 32; ties go to the lower page, a NaN score comes first, pages outside the cache are not selected.  Reads cache->bounds, not
+ * keys and values (may be null).  workspace: iex_select_pages_workspace_bytes, 256-byte aligned. */
+size_t iex_select_pages_workspace_bytes(const iex_paged_cache* cache);
+int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, int count, int first,
+                     int last, int* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* In-place row-wise softmax over the stored entries of a CSR matrix:
  * values[z, j] = exp(scale*values[z, j] - max_row) / sum_row.  values is (batch, nnz).
  * The middle step of sparse attention between SDDMM and SpMM (no reference

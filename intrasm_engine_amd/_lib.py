@@ -33,6 +33,16 @@ CSR_BAD_OFFSETS, CSR_COLUMN_OUT_OF_RANGE, CSR_NOT_ASCENDING = 0x1, 0x2, 0x4
 _c = ctypes
 _vp, _i, _ll, _f = _c.c_void_p, _c.c_int, _c.c_longlong, _c.c_float
 
+
+class PagedCache(_c.Structure):
+    """``iex_paged_cache``: pages of keys and values, and whose they are."""
+    _fields_ = [("dtype", _i), ("eight_bits", _i), ("pages", _i), ("page_size", _i), ("kv_heads", _i), ("head_dim", _i),
+                ("key_page_stride", _ll), ("value_page_stride", _ll), ("keys", _vp), ("values", _vp), ("key_exponents", _vp),
+                ("value_exponents", _vp), ("bounds", _vp), ("table", _vp), ("seqs", _i), ("table_width", _i), ("table_stride", _ll), ("lengths", _vp)]
+
+
+_cache, _strides = _c.POINTER(PagedCache), _c.POINTER(_ll)
+
 # name -> (restype, argtypes).  Kept in one table so that the symbol-export test can
 # walk it against the header.
 SIGNATURES = {
@@ -79,6 +89,11 @@ SIGNATURES = {
     "iex_mask_tables": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _c.c_size_t, _vp]),
     "iex_sparse_attention_fits": (_i, [_i, _i, _i]),
     "iex_sparse_attention": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f, _vp, _vp, _c.c_size_t, _vp]),
+    "iex_kv_append": (_i, [_cache, _i, _vp, _i, _vp, _strides, _vp, _strides, _vp, _strides, _vp, _strides, _vp, _i, _i, _i, _vp]),
+    "iex_paged_attention_workspace_bytes": (_c.c_size_t, [_cache, _i, _i]),
+    "iex_paged_attention": (_i, [_cache, _i, _vp, _strides, _f, _vp, _i, _vp, _strides, _vp, _c.c_size_t, _vp]),
+    "iex_select_pages_workspace_bytes": (_c.c_size_t, [_cache]),
+    "iex_select_pages": (_i, [_cache, _i, _vp, _strides, _i, _i, _i, _vp, _vp, _c.c_size_t, _vp]),
     "iex_csr_softmax": (_i, [_i, _i, _i, _vp, _vp, _vp, _f, _vp, _i]),
     "iex_gemm": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _ll, _ll, _ll, _vp]),
     "iex_gemm_ws": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _ll, _ll, _ll, _vp, _vp, _c.c_size_t]),

@@ -22,6 +22,8 @@
 #include <torch/library.h>
 
 #include <array>
+#include <cmath>
+#include <limits>
 #include <mutex>
 #include <optional>
 #include <shared_mutex>
@@ -609,6 +611,9 @@ py::object sparse_attention(const Tensor& q, const Tensor& k, const Tensor& v, c
   return py::cast(out);
 }
 
+// ---- a paged cache -----------------------------------------------------------------------------------------------
+#include "paged_ops.h"
+
 // ---- autograd: the plain calls of MySpMM and MyLinear (no recording, no forced kernels) -----------------------------
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -724,6 +729,14 @@ TORCH_LIBRARY(iex_ops, lib) {
   define("sddmm_sputnik_half", sddmm_schema, TORCH_FN(sddmm<false>));
   define("csr_softmax_", "(Tensor(a!) values, Tensor row_indices, Tensor row_offsets, float scale) -> Tensor(a!)", TORCH_FN(csr_softmax));
   define("gemm_mfma", "(Tensor a, Tensor b, bool trans_b=False) -> Tensor", TORCH_FN(gemm));
+  define("kv_append_", "(Tensor k, Tensor v, Tensor(a!) keys, Tensor(b!) values, Tensor page_table, Tensor lengths, Tensor? offsets=None, Tensor? q=None, "
+         "Tensor? rotation=None, bool interleaved=False, Tensor(c!)? bounds=None, Tensor(d!)? key_exponents=None, Tensor(e!)? value_exponents=None) -> Tensor",
+         TORCH_FN(kv_append));
+  define("paged_attention", "(Tensor q, Tensor keys, Tensor values, Tensor page_table, Tensor lengths, float? scale=None, Tensor? pages=None, "
+         "Tensor? key_exponents=None, Tensor? value_exponents=None) -> Tensor",
+         TORCH_FN(paged_attention));
+  define("select_pages", "(Tensor q, Tensor bounds, Tensor page_table, Tensor lengths, int page_size, int count, int first=1, int last=1) -> Tensor",
+         TORCH_FN(select_pages));
 }
 
 PYBIND11_MODULE(_iex_host, module) {
