@@ -19,9 +19,6 @@ int launch_forms(const AppendParams& p, bool e8, bool staged, bool interleaved, 
   return staged ? launch<BF16, D, false, true>(p, interleaved, grid, s) : launch<BF16, D, false, false>(p, interleaved, grid, s);
 }
 
-// Rows of whole aligned 16-byte chunks.
-bool rows_of_chunks(const void* x, const long long* strides) { return aligned(x, 16) && strides[2] == 1 && strides[0] % 8 == 0 && strides[1] % 8 == 0; }
-
 }  // namespace
 }  // namespace iex
 

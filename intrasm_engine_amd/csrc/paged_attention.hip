@@ -5,53 +5,63 @@
 namespace iex {
 namespace {
 
-// Workgroups that a launch aims at: what fills the chip's 256 CUs several times over, so that parts of unequal length even out.
-constexpr int kPagedWorkgroups = 2048;
+// Workgroups that are resident at once: three, four or five of four wavefronts on each of the 256 CUs, by their registers.
+int resident(int head_dim, bool e8) { return 256 * paged_simd_waves(head_dim, e8); }
+
+// Rows up to this many tiles of keys stay whole: a workgroup each, of eight wavefronts, and no second launch.
+constexpr int kWholeTiles = 8;
 
 struct Split {
-  long long slots, items, blocks;   // parts beyond one per sequence and block of heads, workgroups per block of heads, such blocks
+  long long blocks, workgroups;   // blocks of up to 16 heads of a key head; workgroups of the launch
   int pitch;
+  bool whole_rows;
 };
 Split split_of(const iex_paged_cache& c, int heads, int count) {
-  const int group = heads / c.kv_heads;
+  const int group = heads / c.kv_heads, most = paged_tiles((count ? count : c.table_width) * c.page_size);
   Split s;
   s.blocks = (long long)c.kv_heads * ceil_div(group, 16);
   s.pitch = group < 16 ? group : 16;
-  const long long wanted = kPagedWorkgroups / s.blocks;
-  s.slots = paged_slots(wanted < 1 ? 1 : wanted, c.seqs, (long long)(count ? count : c.table_width) * c.page_size, kPagedLeast);
-  s.items = c.seqs + s.slots;
+  s.whole_rows = most <= kWholeTiles;
+  const long long rows = s.blocks * c.seqs, stretches = rows * ((most + kPagedLeast - 1) / kPagedLeast);
+  s.workgroups = s.whole_rows ? rows : stretches < resident(c.head_dim, c.eight_bits) ? stretches : resident(c.head_dim, c.eight_bits);
   return s;
 }
-// (per part: rows x head_dim sums, then rows pairs)
-size_t partial_floats(const iex_paged_cache& c, const Split& s) { return (size_t)s.items * s.blocks * s.pitch * c.head_dim; }
+// (two parts a workgroup, each rows x head_dim sums and rows pairs)
+size_t partial_floats(const iex_paged_cache& c, const Split& s) { return (size_t)s.workgroups * 2 * s.pitch * c.head_dim; }
 
-template <bool BF16, int D, bool E8>
+template <bool BF16, int D, bool E8, int WAVES>
 int launch(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
-  const int lds = kPagedWaves * s.pitch * (D + 2) * 4;
-  auto kern = paged_attention_kernel<BF16, D, E8>;
+  const int lds = WAVES * s.pitch * (D + 2) * 4;
+  auto kern = paged_attention_kernel<BF16, D, E8, WAVES>;
   if (lds > 64 * 1024) {
     static thread_local bool raised = false;   // per instantiation
     if (!raised) {
-      if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kPagedWaves * 16 * (D + 2) * 4),
+      if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, WAVES * 16 * (D + 2) * 4),
                              "hipFuncSetAttribute(LDS size)"))
         return rc;
       raised = true;
     }
   }
-  note_kernel("paged_attention_kernel<%s, %d, %s>", BF16 ? "bf16" : "f16", D, E8 ? "e4m3" : "16");
-  hipLaunchKernelGGL(kern, dim3((unsigned)s.items, (unsigned)s.blocks), dim3(kPagedWaves * kWave), lds, stream, p);
+  note_kernel("paged_attention_kernel<%s, %d, %s, %d>", BF16 ? "bf16" : "f16", D, E8 ? "e4m3" : "16", WAVES);
+  hipLaunchKernelGGL(kern, dim3((unsigned)s.workgroups), dim3(WAVES * kWave), lds, stream, p);
   if (int rc = check_hip(hipGetLastError(), "paged attention launch")) return rc;
-  if (s.slots == 0) return 0;
+  if (s.whole_rows) return 0;
   note_kernel("paged_join_kernel<%s, %d>", BF16 ? "bf16" : "f16", D);
-  hipLaunchKernelGGL((paged_join_kernel<BF16, D>), dim3((unsigned)p.cache.seqs, (unsigned)p.heads), dim3(256), 0, stream, p, (int)s.items);
+  hipLaunchKernelGGL((paged_join_kernel<BF16, D>), dim3((unsigned)p.cache.seqs, (unsigned)p.heads), dim3(256), 0, stream, p, (int)s.workgroups);
   return check_hip(hipGetLastError(), "paged attention join launch");
+}
+
+template <bool BF16, int D, bool E8>
+int launch_waves(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
+  constexpr int wide = paged_simd_waves(D, E8) > 1 ? 8 : 4;
+  return s.whole_rows ? launch<BF16, D, E8, wide>(p, s, stream) : launch<BF16, D, E8, 4>(p, s, stream);
 }
 
 template <bool BF16>
 int launch_type(const PagedAttentionParams& p, const Split& s, int head_dim, bool e8, hipStream_t stream) {
-  if (head_dim == 64) return e8 ? launch<BF16, 64, true>(p, s, stream) : launch<BF16, 64, false>(p, s, stream);
-  if (head_dim == 128) return e8 ? launch<BF16, 128, true>(p, s, stream) : launch<BF16, 128, false>(p, s, stream);
-  return e8 ? launch<BF16, 256, true>(p, s, stream) : launch<BF16, 256, false>(p, s, stream);
+  if (head_dim == 64) return e8 ? launch_waves<BF16, 64, true>(p, s, stream) : launch_waves<BF16, 64, false>(p, s, stream);
+  if (head_dim == 128) return e8 ? launch_waves<BF16, 128, true>(p, s, stream) : launch_waves<BF16, 128, false>(p, s, stream);
+  return e8 ? launch_waves<BF16, 256, true>(p, s, stream) : launch_waves<BF16, 256, false>(p, s, stream);
 }
 
 int check_heads(const iex_paged_cache* c, int heads, const char* what) {
@@ -68,8 +78,8 @@ extern "C" size_t iex_paged_attention_workspace_bytes(const iex_paged_cache* cac
   using namespace iex;
   if (check_paged_cache(cache, "paged_attention", false) || check_heads(cache, heads, "paged_attention") || heads == 0 || cache->seqs == 0 || count < 0) return 0;
   const Split s = split_of(*cache, heads, count);
-  if (s.slots == 0) return 0;
-  return partial_floats(*cache, s) * 4 + (size_t)s.items * s.blocks * s.pitch * 8;
+  if (s.whole_rows) return 0;
+  return partial_floats(*cache, s) * 4 + (size_t)s.workgroups * 2 * s.pitch * 8;
 }
 
 extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, float scale, const int* listed, int count,
@@ -87,16 +97,17 @@ extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, cons
   IEX_REQUIRE(scale > 0.f && scale < 1e30f, IEX_ERR_UNSUPPORTED, "paged_attention: the scale must be positive and finite");
   const Split s = split_of(*cache, heads, count);
   const long long tiles = (long long)cache->seqs * paged_tiles((count ? count : cache->table_width) * cache->page_size);
-  IEX_REQUIRE(tiles < (1ll << 31) && s.items < (1ll << 31) && s.blocks < 65536 && heads < 65536, IEX_ERR_TOO_LARGE, "paged_attention: too many sequences or heads");
+  IEX_REQUIRE(tiles < (1ll << 31) && s.workgroups < (1ll << 30) && heads < 65536, IEX_ERR_TOO_LARGE, "paged_attention: too many sequences or heads");
   const size_t need = iex_paged_attention_workspace_bytes(cache, heads, count);
   IEX_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), IEX_ERR_BAD_ARGUMENT,
               "paged_attention: needs a 256-byte aligned workspace of %zu bytes", need);
   PagedAttentionParams p{};
   p.cache = paged_params(*cache);
   p.heads = heads, p.group = heads / cache->kv_heads, p.group_tiles = ceil_div(p.group, 16), p.pitch = s.pitch;
-  p.slots = (int)s.slots, p.count = count, p.listed = listed;
+  p.count = count, p.listed = listed, p.whole_rows = s.whole_rows;
   p.q = static_cast<const unsigned short*>(q), p.out = static_cast<unsigned short*>(out);
   for (int i = 0; i < 3; ++i) p.q_strides[i] = q_strides[i], p.out_strides[i] = out_strides[i];
+  p.q_rows = rows_of_chunks(q, q_strides);
   p.scale_log2 = scale * 1.44269504088896340736f;
   p.partial = static_cast<float*>(workspace);
   p.stats = p.partial + (need ? partial_floats(*cache, s) : 0);

@@ -24,58 +24,50 @@ namespace iex {
 struct PagedAttentionParams {
   PagedParams cache;
   int heads, group, group_tiles;   // query heads, those of a key head, blocks of 16 of them
-  int pitch, slots, count;         // query rows of a part's result; parts beyond one per sequence (paged_slots); pages listed per sequence and key head, 0: all of the table
+  int pitch, count;                // query rows of a part's result; pages listed per sequence and key head, 0: all of the table
+  bool whole_rows;                 // a workgroup per row, else equal stretches of all tiles
   const int* listed;
   const unsigned short* q;
   unsigned short* out;
   long long q_strides[3], out_strides[3];   // sequence, head, feature
+  bool q_rows;
   float scale_log2;
   float* partial;   // per part: group_rows x D sums, then per part group_rows maxima and sums
   float* stats;
 };
 
-constexpr int kPagedWaves = 4, kPagedLeast = 2;   // wavefronts of a workgroup; tiles of kPagedTile tokens that are worth a part
+constexpr int kPagedLeast = 2;   // tiles that are worth a workgroup
 
-// The sequence and part of a workgroup, from the lengths (every wavefront for itself).
-struct PagedItem {
-  int seq, part, parts, part_tiles, first_item;
-};
-__device__ __forceinline__ int paged_tokens(const PagedAttentionParams& p, int seq) {
-  const int length = seq < p.cache.seqs ? cached_length(p.cache.lengths[seq], p.cache.table_width, 1 << p.cache.page_shift) : 0;
+__device__ __forceinline__ int row_tokens(const PagedAttentionParams& p, int seq) {
+  const int length = cached_length(p.cache.lengths[seq], p.cache.table_width, 1 << p.cache.page_shift);
   return p.count && length ? p.count << p.cache.page_shift : length;
 }
-template <typename MATCH>
-__device__ __forceinline__ bool paged_find(const PagedAttentionParams& p, MATCH match, PagedItem& item) {
-  const int lane = lane_id(), seqs = p.cache.seqs;
-  int total = 0, tiles = 0;
-  for (int s0 = 0; s0 < seqs; s0 += kWave) {
-    tiles = paged_tiles(paged_tokens(p, s0 + lane));
-    total += tiles;
-  }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) total += __shfl_xor(total, d);
-  item.part_tiles = paged_part_tiles(uniform(total), p.slots, kPagedLeast);
+__device__ __forceinline__ int lane_tiles(const PagedAttentionParams& p, int seq) { return seq < p.cache.seqs ? paged_tiles(row_tokens(p, seq)) : 0; }
+// Tiles of all sequences (of one block of heads).
+__device__ __forceinline__ int all_tiles(const PagedAttentionParams& p) {
+  int total = 0;
+  for (int s0 = 0; s0 < p.cache.seqs; s0 += kWave) total += lane_tiles(p, s0 + lane_id());
+  return bcast_i(wave_scan(total), kWave - 1);
+}
+// The sequence that has tile `at` of them, and the first of its tiles.
+__device__ __forceinline__ int sequence_at(const PagedAttentionParams& p, int at, int& first) {
   int before = 0;
-  for (int s0 = 0; s0 < seqs; s0 += kWave) {
-    if (seqs > kWave) tiles = paged_tiles(paged_tokens(p, s0 + lane));
-    const int parts = s0 + lane < seqs ? paged_parts(tiles, item.part_tiles) : 0;
-    int upto = parts;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int other = __shfl_up(upto, d);
-      if (lane >= d) upto += other;
+  for (int s0 = 0;; s0 += kWave) {
+    const int tiles = lane_tiles(p, s0 + lane_id()), upto = before + wave_scan(tiles);
+    const unsigned long long past = __ballot(upto > at);
+    if (past || s0 + kWave >= p.cache.seqs) {   // (the latter: never, at < all_tiles())
+      const int lane = past ? __ffsll(past) - 1 : 0;
+      first = bcast_i(upto - tiles, lane);
+      return min(s0 + lane, p.cache.seqs - 1);
     }
-    const unsigned long long hit = __ballot(match(s0 + lane, before + upto - parts, parts));
-    if (hit) {
-      const int at = __ffsll(hit) - 1;
-      item.seq = s0 + at;
-      item.parts = uniform(__shfl(parts, at));
-      item.first_item = uniform(__shfl(before + upto - parts, at));
-      return true;
-    }
-    before += uniform(__shfl(upto, kWave - 1));
+    before = bcast_i(upto, kWave - 1);
   }
-  return false;
+}
+// ... and the first tile of a sequence.
+__device__ __forceinline__ int tiles_before(const PagedAttentionParams& p, int seq) {
+  int total = 0;
+  for (int s0 = 0; s0 < seq; s0 += kWave) total += s0 + lane_id() < seq ? lane_tiles(p, s0 + lane_id()) : 0;
+  return bcast_i(wave_scan(total), kWave - 1);
 }
 
 // Two e4m3 codes of a dword to a pair of 16-bit values (exact).
@@ -85,31 +77,51 @@ __device__ __forceinline__ unsigned widen_pair(unsigned codes) {
   else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, HIGH));
 }
 
-template <bool BF16, int D, bool E8>
-__global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void paged_attention_kernel(PagedAttentionParams p) {
+// Wavefronts of a SIMD that the registers are cut for.
+constexpr int paged_simd_waves(int head_dim, bool eight_bits) { return head_dim == 256 ? (eight_bits ? 2 : 1) : head_dim == 128 ? 3 : 4; }
+
+template <bool BF16, int D, bool E8, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_attention_kernel(PagedAttentionParams p) {
   typedef unsigned short u16;
   constexpr int ES = E8 ? 1 : 2;               // bytes of an element
   constexpr int KS = D / 32;                   // steps of the sum over features
   constexpr int KW = D * ES / 64;              // 16-byte loads of a lane for the keys of 16 tokens (E8: each is two steps)
   constexpr int F = D / 16;                    // features of a value row that a lane has: operands of the second product
-  constexpr int VD = F * ES / 4;               // ... in dwords: 1 .. 8
+  constexpr int VD = F * ES / 4, VWORDS = VD == 8 ? 2 : 1;   // ... in dwords: 1, 2, 4 or 8
+  typedef std::conditional_t<VD == 1, unsigned, std::conditional_t<VD == 2, u32x2, u32x4>> VWord;
   constexpr bool PV_BF16 = BF16 || E8;         // (an e4m3 value's power of two goes to the probability, which fp16 has not the range for)
   extern __shared__ __align__(16) float smem[];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int col = lane & 15, g = lane >> 4;
-  const int kv_head = blockIdx.y / p.group_tiles, group_tile = blockIdx.y % p.group_tiles;
-  const int rows = min(16, p.group - group_tile * 16);   // queries
+  const int wave = uniform(threadIdx.x >> 6);
   const PagedParams& cache = p.cache;
 
-  PagedItem item;
-  const int id = blockIdx.x;
-  if (!paged_find(p, [&](int, int first, int parts) { return first + parts > id; }, item)) return;
-  item.part = id - item.first_item;
-  const int seq = item.seq;
+  // ---- this workgroup's stretch of the line of tiles ----
+  int seq, block, total = 0;
+  long long at = 0, stretch_begin = 0, stretch_end = 0, row0 = 0;
+  if (p.whole_rows) {
+    seq = blockIdx.x % cache.seqs, block = blockIdx.x / cache.seqs;
+  } else {
+    total = all_tiles(p);
+    const long long line = (long long)total * (cache.kv_heads * p.group_tiles), stretch = paged_stretch(line, gridDim.x, kPagedLeast);
+    at = stretch_begin = stretch * blockIdx.x;
+    stretch_end = min(line, stretch_begin + stretch);
+    if (at >= line) return;
+    block = (int)(at / total);
+    int first;
+    seq = sequence_at(p, (int)(at - (long long)block * total), first);
+    row0 = (long long)block * total + first;
+  }
+
+  for (;;) {   // the rows of the stretch
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));   // (what follows from the lane is worked out again for each row: kept for all of them it is spilled)
+  const int col = lane & 15, g = lane >> 4;
+  const int kv_head = block / p.group_tiles, group_tile = block % p.group_tiles;
+  const int rows = min(16, p.group - group_tile * 16);   // queries
   const int length = cached_length(cache.lengths[seq], cache.table_width, 1 << cache.page_shift);
-  const int tokens = p.count && length ? p.count << cache.page_shift : length;
-  const long long part_tokens = (long long)item.part_tiles * kPagedTile;
-  const int begin = (int)min((long long)tokens, item.part * part_tokens), end = (int)min((long long)tokens, (item.part + 1) * part_tokens);
+  const int tokens = p.count && length ? p.count << cache.page_shift : length, tiles = paged_tiles(tokens);
+  PagedPart part{0, tiles, 0, true};
+  if (!p.whole_rows) part = paged_part(row0, tiles, at, stretch_begin, stretch_end, blockIdx.x);
+  const int begin = part.from * kPagedTile, end = min(tokens, part.to * kPagedTile);
 
   // ---- queries: columns of the first product ----
   u32x4 fq[KS];
@@ -120,10 +132,14 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = E8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8;
-      unsigned w[4];
+      if (p.q_rows) {   // rows of aligned 16-byte chunks
+        fq[s] = *reinterpret_cast<const u32x4*>(q + d);
+      } else {
+        unsigned w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = q[(d + 2 * j) * p.q_strides[2]] | (unsigned)q[(d + 2 * j + 1) * p.q_strides[2]] << 16;
-      fq[s] = u32x4{w[0], w[1], w[2], w[3]};
+        for (int j = 0; j < 4; ++j) w[j] = q[(d + 2 * j) * p.q_strides[2]] | (unsigned)q[(d + 2 * j + 1) * p.q_strides[2]] << 16;
+        fq[s] = u32x4{w[0], w[1], w[2], w[3]};
+      }
     }
   }
 
@@ -143,56 +159,53 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
     }
   };
 
-  struct Tile {
-    u32x4 k[2][KW];
-    unsigned v[2][4][VD];
-    unsigned ke[2], ve[2];   // exponents of this lane's four tokens
-    int valid[2];
+  // Where 32 tokens lie: two places of 16.  Loads take no branch: what is not attended to is read from a place that exists and
+  // masked where it is used.
+  struct Where {
+    int page[2], row[2], valid[2];
   };
-  auto load = [&](int t, Tile& tile) {
+  auto find = [&](int t) {
+    Where w;
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const PagedPlace place = paged_place(t + a * 16, cache.page_shift);
-      if (place.entry >= window + kWave || place.entry < window) look_up(place.entry);
-      const int page = __builtin_amdgcn_readlane(entry_page, place.entry - window), logical = __builtin_amdgcn_readlane(entry_logical, place.entry - window);
-      const int valid = place.entry < entries ? paged_valid(logical, place.slot, cache.page_shift, page, cache.pages, length) : 0;
-      tile.valid[a] = valid;
-      if (valid == 0) {
-#pragma unroll
-        for (int s = 0; s < KW; ++s) tile.k[a][s] = u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int d = 0; d < VD; ++d) tile.v[a][i][d] = 0u;
-        tile.ke[a] = tile.ve[a] = 0x7F7F7F7Fu;
-        continue;
-      }
-      const size_t row0 = ((size_t)kv_head << cache.page_shift) + place.slot;
-      const unsigned char* k = static_cast<const unsigned char*>(cache.keys) + ((long long)page * cache.key_page + (long long)row0 * D) * ES;
-      const unsigned char* v = static_cast<const unsigned char*>(cache.values) + ((long long)page * cache.value_page + (long long)row0 * D) * ES;
-#pragma unroll
-      for (int s = 0; s < KW; ++s) tile.k[a][s] = *reinterpret_cast<const u32x4*>(k + col * (D * ES) + s * 64 + g * 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned char* at = v + (g * 4 + i) * (D * ES);
-        // (heads of 256 in 16 bits: two halves of 128, so that a load of 16 lanes is 256 consecutive bytes)
-        if constexpr (VD == 8) {
-          *reinterpret_cast<u32x4*>(&tile.v[a][i][0]) = *reinterpret_cast<const u32x4*>(at + col * 16);
-          *reinterpret_cast<u32x4*>(&tile.v[a][i][4]) = *reinterpret_cast<const u32x4*>(at + 256 + col * 16);
-        } else if constexpr (VD == 4) {
-          *reinterpret_cast<u32x4*>(&tile.v[a][i][0]) = *reinterpret_cast<const u32x4*>(at + col * 16);
-        } else if constexpr (VD == 2) {
-          *reinterpret_cast<u32x2*>(&tile.v[a][i][0]) = *reinterpret_cast<const u32x2*>(at + col * 8);
-        } else {
-          tile.v[a][i][0] = *reinterpret_cast<const unsigned*>(at + col * 4);
-        }
-      }
-      if constexpr (E8) {
-        const size_t at = (((size_t)page * cache.kv_heads) << cache.page_shift) + row0 + g * 4;
-        tile.ke[a] = *reinterpret_cast<const unsigned*>(cache.key_exponents + at);
-        tile.ve[a] = *reinterpret_cast<const unsigned*>(cache.value_exponents + at);
-      }
+      if (place.entry >= window + kWave) look_up(place.entry);
+      const int page = bcast_i(entry_page, place.entry - window), logical = bcast_i(entry_logical, place.entry - window);
+      w.valid[a] = place.entry < entries ? paged_valid(logical, place.slot, cache.page_shift, page, cache.pages, length) : 0;
+      w.page[a] = w.valid[a] ? page : 0;
+      w.row[a] = (kv_head << cache.page_shift) + place.slot;
     }
+    return w;
+  };
+  u32x4 key[2][KW];
+  VWord value[2][4][VWORDS];
+  unsigned ke[2], ve[2];   // exponents of this lane's four tokens
+  auto load_keys = [&](const Where& w) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const unsigned char* k = static_cast<const unsigned char*>(cache.keys) + (w.page[a] * cache.key_page + (long long)w.row[a] * D) * ES;
+#pragma unroll
+      for (int s = 0; s < KW; ++s) key[a][s] = *reinterpret_cast<const u32x4*>(k + (col * (D * ES) + s * 64 + g * 16));
+      if constexpr (E8)
+        ke[a] = *reinterpret_cast<const unsigned*>(cache.key_exponents + (((long long)w.page[a] * cache.kv_heads) << cache.page_shift) + w.row[a] + g * 4);
+    }
+  };
+  auto load_values = [&](const Where& w) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const unsigned char* v = static_cast<const unsigned char*>(cache.values) + (w.page[a] * cache.value_page + (long long)w.row[a] * D) * ES;
+      // (heads of 256 in 16 bits: two halves of 128, so that a load of 16 lanes is 256 consecutive bytes)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < VWORDS; ++h) value[a][i][h] = *reinterpret_cast<const VWord*>(v + ((g * 4 + i) * (D * ES) + h * 256 + col * (int)sizeof(VWord)));
+      if constexpr (E8)
+        ve[a] = *reinterpret_cast<const unsigned*>(cache.value_exponents + (((long long)w.page[a] * cache.kv_heads) << cache.page_shift) + w.row[a] + g * 4);
+    }
+  };
+  auto value_dword = [&](int a, int r, int d) -> unsigned {
+    if constexpr (VD == 1) return value[a][r][0];
+    else return value[a][r][d / 4][d % 4];
   };
 
   f32x4 o[F];
@@ -201,9 +214,8 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
   float top = -INFINITY, sum = 0.f;   // of this lane's query: the maximum so far (all groups'), this group's share of the sum
   int attended = 0;
 
-  auto compute = [&](Tile& tile) {
-    attended += tile.valid[0] + tile.valid[1];
-    f32x4 s[2];
+  f32x4 s[2];
+  auto scores = [&]() {
 #pragma unroll
     for (int a = 0; a < 2; ++a) s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -212,10 +224,10 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
       for (int a = 0; a < 2; ++a) {
         u32x4 fk;
         if constexpr (E8) {
-          const unsigned c0 = tile.k[a][e / 2][e % 2 * 2], c1 = tile.k[a][e / 2][e % 2 * 2 + 1];
+          const unsigned c0 = key[a][e / 2][e % 2 * 2], c1 = key[a][e / 2][e % 2 * 2 + 1];
           fk = u32x4{widen_pair<BF16, false>(c0), widen_pair<BF16, true>(c0), widen_pair<BF16, false>(c1), widen_pair<BF16, true>(c1)};
         } else {
-          fk = tile.k[a][e];
+          fk = key[a][e];
         }
         s[a] = mfma_16x16x32<BF16>(fk, fq[e], s[a]);
       }
@@ -223,18 +235,22 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[a][r] *= power_of_two(tile.ke[a] >> (r * 8) & 0xFFu);
+        for (int r = 0; r < 4; ++r) s[a][r] *= power_of_two(ke[a] >> (r * 8) & 0xFFu);
     }
-    if (tile.valid[0] + tile.valid[1] != 32) {   // (uniform) tokens that are not attended to leave no trace, infinities and NaN included
+  };
+  u32x4 hi, lo;
+  auto weights = [&](const Where& w) {
+    attended += w.valid[0] + w.valid[1];
+    if (w.valid[0] + w.valid[1] != 32) {   // (uniform) tokens that are not attended to leave no trace, infinities and NaN included
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (g * 4 + r >= tile.valid[a]) {
+          if (g * 4 + r >= w.valid[a]) {
             s[a][r] = -INFINITY;
 #pragma unroll
-            for (int d = 0; d < VD; ++d) tile.v[a][r][d] = 0u;
-            if constexpr (E8) tile.ve[a] = (tile.ve[a] & ~(0xFFu << (r * 8))) | 0x7Fu << (r * 8);
+            for (int h = 0; h < VWORDS; ++h) value[a][r][h] = VWord{};
+            if constexpr (E8) ve[a] = (ve[a] & ~(0xFFu << (r * 8))) | 0x7Fu << (r * 8);
           }
     }
     float m = s[0][0];
@@ -256,14 +272,13 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
       }
     }
     const float shift = top == -INFINITY ? 0.f : -top * p.scale_log2;
-    u32x4 hi, lo;
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         s[a][r] = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.scale_log2, shift));   // (exp2(-infinity) = 0)
         sum += s[a][r];
-        if constexpr (E8) s[a][r] *= power_of_two(tile.ve[a] >> (r * 8) & 0xFFu);
+        if constexpr (E8) s[a][r] *= power_of_two(ve[a] >> (r * 8) & 0xFFu);
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -273,6 +288,8 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
         lo[a * 2 + r] = pack_pair<PV_BF16>(s[a][2 * r] - h0, s[a][2 * r + 1] - h1);
       }
     }
+  };
+  auto weigh_values = [&]() {
 #pragma unroll
     for (int j = 0; j < F; ++j) {
       u32x4 fv;
@@ -281,10 +298,10 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
         const int a = w / 2, r = w % 2 * 2;   // tokens r and r + 1 of the four in subtile a
         if constexpr (E8) {
           // byte j of both rows side by side, then widened
-          const unsigned pair = __builtin_amdgcn_perm(tile.v[a][r + 1][j / 4], tile.v[a][r][j / 4], (j % 4) | (4 + j % 4) << 8);
+          const unsigned pair = __builtin_amdgcn_perm(value_dword(a, r + 1, j / 4), value_dword(a, r, j / 4), (j % 4) | (4 + j % 4) << 8);
           fv[w] = widen_pair<PV_BF16, false>(pair);
         } else {
-          fv[w] = __builtin_amdgcn_perm(tile.v[a][r + 1][j / 2], tile.v[a][r][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+          fv[w] = __builtin_amdgcn_perm(value_dword(a, r + 1, j / 2), value_dword(a, r, j / 2), j % 2 ? 0x07060302u : 0x05040100u);
         }
       }
       o[j] = mfma_16x16x32<PV_BF16>(fv, hi, o[j]);
@@ -292,19 +309,27 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
     }
   };
 
-  // ---- the part's tiles, a wavefront's in turn, the next one's loads ahead of the present one's products ----
-  Tile one, two;
+  // ---- the part's tiles, a wavefront's in turn.  A tile's values are asked for before its keys are waited for, the next tile's
+  // keys as soon as this one's have been multiplied: half a tile is in flight at any time, in one set of registers.  (The last
+  // tile is written out behind the loop, so that a wait knows on every path how many loads are behind the ones it is for.)
   int t = begin + wave * 32;
-  constexpr int STEP = kPagedWaves * 32;
-  if (t < end) load(t, one);
-  while (t < end) {
-    if (t + STEP < end) load(t + STEP, two);
-    compute(one);
-    t += STEP;
-    if (t >= end) break;
-    if (t + STEP < end) load(t + STEP, one);
-    compute(two);
-    t += STEP;
+  constexpr int STEP = WAVES * 32;
+  if (t < end && cache.pages > 0) {
+    Where now = find(t);
+    load_keys(now);
+    for (; t + STEP < end; t += STEP) {
+      load_values(now);
+      const Where next = find(t + STEP);
+      scores();
+      load_keys(next);
+      weights(now);
+      weigh_values();
+      now = next;
+    }
+    load_values(now);
+    scores();
+    weights(now);
+    weigh_values();
   }
 
   // ---- the wavefronts meet ----
@@ -312,7 +337,7 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
   sum += __shfl_xor(sum, 32);
   if (attended == 0) sum = -1.f;   // no token at all: zeros, whatever the formula says of an empty sum
   float* sums = smem;                                  // [wave][row][D]
-  float* tops = smem + kPagedWaves * rows * D;         // [wave][row] (maximum, sum)
+  float* tops = smem + WAVES * rows * D;         // [wave][row] (maximum, sum)
   if (col < rows) {
     float* mine = sums + (wave * rows + col) * D;
 #pragma unroll
@@ -326,79 +351,96 @@ __global__ __launch_bounds__(kPagedWaves * 64, D == 256 && !E8 ? 1 : 2) void pag
     if (g == 0) tops[(wave * rows + col) * 2] = top, tops[(wave * rows + col) * 2 + 1] = sum;
   }
   __syncthreads();
-  const bool whole = item.parts == 1;
-  const size_t result = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
-  for (int i = threadIdx.x; i < rows * D; i += kPagedWaves * 64) {
+  for (int i = threadIdx.x; i < rows * D; i += WAVES * 64) {
     const int row = i / D, d = i % D;
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) m = fmaxf(m, tops[(w * rows + row) * 2]);
-    float total = 0.f, acc = 0.f;
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, tops[(w * rows + row) * 2]);
+    float all = 0.f, acc = 0.f;
     bool any = false;
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) {
-      const float mine = tops[(w * rows + row) * 2], part = tops[(w * rows + row) * 2 + 1];
-      if (part == -1.f) continue;
+    for (int w = 0; w < WAVES; ++w) {
+      const float mine = tops[(w * rows + row) * 2], share = tops[(w * rows + row) * 2 + 1];
+      if (share == -1.f) continue;
       any = true;
       const float keep = mine == m ? 1.f : __builtin_amdgcn_exp2f((mine - m) * p.scale_log2);
-      total += keep * part;
+      all += keep * share;
       acc += keep * sums[(w * rows + row) * D + d];
     }
-    if (whole) {
+    if (part.whole) {
       const int head = kv_head * p.group + group_tile * 16 + row;
-      p.out[seq * p.out_strides[0] + head * p.out_strides[1] + d * p.out_strides[2]] = f32_to_16(any ? acc / total : 0.f, BF16);
+      p.out[seq * p.out_strides[0] + head * p.out_strides[1] + d * p.out_strides[2]] = f32_to_16(any ? acc / all : 0.f, BF16);
     } else {
-      p.partial[(result * p.pitch + row) * D + d] = acc;
-      if (d == 0) p.stats[(result * p.pitch + row) * 2] = m, p.stats[(result * p.pitch + row) * 2 + 1] = any ? total : -1.f;
+      const size_t to = (size_t)part.place * p.pitch + row;
+      p.partial[to * D + d] = acc;
+      if (d == 0) p.stats[to * 2] = m, p.stats[to * 2 + 1] = any ? all : -1.f;
     }
+  }
+  if (p.whole_rows) return;
+  at = row0 + part.to;
+  if (at >= stretch_end) return;
+  row0 = at;   // (the row is through: the stretch goes on)
+  if (++seq == cache.seqs) seq = 0, ++block;
+  __syncthreads();   // everybody has read the sums
   }
 }
 
-// Parts of a sequence into its result, a workgroup per sequence and query head: 256 / (D / 4) parts side by side, a thread four
-// features with a running maximum; they meet in LDS.
+// Parts of a row into its result, a workgroup per sequence and query head: the parts' weights first, 256 at a time, then
+// 256 / (D / 4) parts side by side, a thread four features; they meet in LDS.
 template <bool BF16, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p, int items) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p, int workgroups) {
   constexpr int LANES = D / 4, SIDE = 256 / LANES;   // threads of a row; parts side by side
   __shared__ float4 accs[SIDE][LANES];
-  __shared__ float tops[SIDE][2];
-  const int seq = blockIdx.x, head = blockIdx.y;
+  __shared__ float weights[256], tops[4], sums[4];
+  const int seq = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
   const int kv_head = head / p.group, in_group = head % p.group;
-  PagedItem item;
-  if (!paged_find(p, [&](int s, int, int) { return s == seq; }, item)) return;
-  if (item.parts == 1) return;
-  const int lane = threadIdx.x % LANES, side = threadIdx.x / LANES;
-  const size_t y = (size_t)kv_head * p.group_tiles + in_group / 16, row = in_group % 16;
+  const int of_all = all_tiles(p), block = kv_head * p.group_tiles + in_group / 16;
+  const long long blocks = (long long)p.cache.kv_heads * p.group_tiles, row = (long long)block * of_all + tiles_before(p, seq);
+  const PagedParts parts = paged_parts(row, paged_tiles(row_tokens(p, seq)), paged_stretch(of_all * blocks, workgroups, kPagedLeast));
+  if (parts.first == parts.last) return;
+  const int number = parts.last - parts.first + 1;
+  auto place = [&](int i) { return (size_t)((parts.first + i) * 2 + (i == 0 && parts.second ? 1 : 0)) * p.pitch + in_group % 16; };
+  const int lane = tid % LANES, side = tid / LANES;
   float4 acc = {0.f, 0.f, 0.f, 0.f};
-  float top = -INFINITY, sum = -1.f;
-  for (int i = side; i < item.parts; i += SIDE) {
-    const size_t result = (y * items + item.first_item + i) * p.pitch + row;
-    const float m = p.stats[result * 2], part = p.stats[result * 2 + 1];
-    const float4 x = *reinterpret_cast<const float4*>(p.partial + result * D + lane * 4);
-    if (part == -1.f) continue;
-    const float now = fmaxf(top, m);
-    const float keep = top == now ? 1.f : __builtin_amdgcn_exp2f((top - now) * p.scale_log2), in = m == now ? 1.f : __builtin_amdgcn_exp2f((m - now) * p.scale_log2);
-    sum = (sum == -1.f ? 0.f : sum * keep) + part * in;
-    acc.x = acc.x * keep + x.x * in, acc.y = acc.y * keep + x.y * in, acc.z = acc.z * keep + x.z * in, acc.w = acc.w * keep + x.w * in;
+  float top = -INFINITY, total = 0.f;
+  bool any = false;
+  for (int i0 = 0; i0 < number; i0 += 256) {
+    const int i = i0 + tid;
+    float m = -INFINITY, part = -1.f;
+    if (i < number) {
+      const float2 both = *reinterpret_cast<const float2*>(p.stats + place(i) * 2);
+      m = both.x, part = both.y;
+    }
+    const bool counts = part != -1.f;   // (NaN is a sum)
+    const float most = wave_max(counts ? m : -INFINITY);
+    if (lane_id() == 0) tops[tid >> 6] = most;
+    any |= __syncthreads_or(counts);
+    const float now = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), top);
+    const float keep = top == now ? 1.f : __builtin_amdgcn_exp2f((top - now) * p.scale_log2);
+    const float weight = !counts ? 0.f : m == now ? 1.f : __builtin_amdgcn_exp2f((m - now) * p.scale_log2);
+    weights[tid] = weight;
+    const float share = wave_sum(counts ? weight * part : 0.f);
+    if (lane_id() == 0) sums[tid >> 6] = share;
+    __syncthreads();
+    total = total * keep + (sums[0] + sums[1] + sums[2] + sums[3]);
+    acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
     top = now;
+    const int n = min(256, number - i0);
+#pragma unroll 4
+    for (int j = side; j < n; j += SIDE) {   // (a part without a token left zeros)
+      const float w = weights[j];
+      const float4 x = *reinterpret_cast<const float4*>(p.partial + place(i0 + j) * D + lane * 4);
+      acc.x = fmaf(w, x.x, acc.x), acc.y = fmaf(w, x.y, acc.y), acc.z = fmaf(w, x.z, acc.z), acc.w = fmaf(w, x.w, acc.w);
+    }
+    __syncthreads();
   }
   accs[side][lane] = acc;
-  if (lane == 0) tops[side][0] = top, tops[side][1] = sum;
   __syncthreads();
-  if (threadIdx.x >= D) return;
-  float m = -INFINITY;
+  if (tid >= D) return;
+  float x = 0.f;
 #pragma unroll
-  for (int i = 0; i < SIDE; ++i) m = fmaxf(m, tops[i][0]);
-  float total = 0.f, x = 0.f;
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < SIDE; ++i) {
-    if (tops[i][1] == -1.f) continue;
-    any = true;
-    const float keep = tops[i][0] == m ? 1.f : __builtin_amdgcn_exp2f((tops[i][0] - m) * p.scale_log2);
-    total += keep * tops[i][1];
-    x += keep * reinterpret_cast<const float*>(accs[i])[threadIdx.x];
-  }
-  p.out[seq * p.out_strides[0] + head * p.out_strides[1] + threadIdx.x * p.out_strides[2]] = f32_to_16(any ? x / total : 0.f, BF16);
+  for (int i = 0; i < SIDE; ++i) x += reinterpret_cast<const float*>(accs[i])[tid];
+  p.out[seq * p.out_strides[0] + head * p.out_strides[1] + tid * p.out_strides[2]] = f32_to_16(any ? x / total : 0.f, BF16);
 }
 
 }  // namespace iex

@@ -16,29 +16,47 @@ IEX_HD int cached_length(int length, int table_width, int page_size) {
   return length < 0 ? 0 : length > most ? most : length;
 }
 
-// ---- attention: a sequence in parts -----------------------------------------------------------------------------------
-constexpr int kPagedTile = 128;   // tokens of one step of a workgroup: the unit in which lengths are split
+// ---- attention: rows in parts -----------------------------------------------------------------------------------------
+// A row is a sequence with one block of up to 16 query heads of a key head.  Rows are tiles of kPagedTile tokens, at least one (an
+// empty sequence's zeros are work too); all tiles, the rows of a block after each other, block by block, are one line that the
+// workgroups cut into equal stretches.  So a workgroup has the end of one row, whole rows, the beginning of another; a row that is
+// not whole anywhere is joined from what its workgroups leave, at most two parts each.
+constexpr int kPagedTile = 128;   // tokens
 
-IEX_HD int paged_tiles(int tokens) { return tokens / kPagedTile + (tokens % kPagedTile != 0); }
+IEX_HD int paged_tiles(int tokens) { return tokens <= kPagedTile ? 1 : tokens / kPagedTile + (tokens % kPagedTile != 0); }
 
-// Tiles of a part where `total` tiles (of all sequences, one head) go to about `slots` workgroups: the parts of all sequences
-// are at most `slots` more than there are sequences, since a sequence has one part more than whole parts fit into it.
-// slots == 0: never split.
-IEX_HD int paged_part_tiles(int total, int slots, int least) {
-  if (slots == 0) return 1 << 30;
-  const int even = total / slots + (total % slots != 0);
+// Tiles of a workgroup's stretch.  `least`: fewer are not worth a workgroup.
+IEX_HD long long paged_stretch(long long tiles, int workgroups, int least) {
+  const long long even = tiles / workgroups + (tiles % workgroups != 0);
   return even > least ? even : least;
 }
 
-// ... and the parts of one sequence: at least one, which writes the zeros of an empty sequence.
-IEX_HD int paged_parts(int tiles, int part_tiles) { return tiles <= part_tiles ? 1 : tiles / part_tiles + (tiles % part_tiles != 0); }
-
-// Workgroups per head that are worth having beyond one per sequence: none where no sequence can be long enough to be split.
-// (the workgroups of a launch and the room for their partial results go by it)
-IEX_HD long long paged_slots(long long wanted, long long seqs, long long most_tokens, int least_tiles) {
-  const long long tiles = (most_tokens + kPagedTile - 1) / kPagedTile;
-  const long long most = seqs * ((tiles + least_tiles - 1) / least_tiles - 1);
-  return most < wanted ? (most < 0 ? 0 : most) : wanted;
+// A row's part in a workgroup: tiles from .. to of the row, and where the workgroup leaves its sums if that is not all of them.
+struct PagedPart {
+  int from, to, place;
+  bool whole;
+};
+// `row`: the line's tile that is the row's first; `tiles`: how many it has; `at`: the line's tile that the workgroup has come to;
+// `begin`, `end`: its stretch.
+IEX_HD PagedPart paged_part(long long row, int tiles, long long at, long long begin, long long end, int workgroup) {
+  PagedPart p;
+  p.from = (int)(at - row);
+  p.to = end - row < tiles ? (int)(end - row) : tiles;
+  p.whole = p.from == 0 && p.to == tiles;
+  p.place = workgroup * 2 + (at > begin ? 1 : 0);
+  return p;
+}
+// The parts of a row, for who joins them: workgroups first .. last, a place each.
+struct PagedParts {
+  int first, last;
+  bool second;   // the first workgroup's part is its second place
+};
+IEX_HD PagedParts paged_parts(long long row, int tiles, long long stretch) {
+  PagedParts p;
+  p.first = (int)(row / stretch);
+  p.last = (int)((row + tiles - 1) / stretch);
+  p.second = row % stretch != 0;
+  return p;
 }
 
 // Where 16 tokens of a sequence from `token` on lie (16 divides token and the page): entry `entry` of the sequence's table (or

@@ -18,6 +18,17 @@ struct PagedParams {
 
 __device__ __forceinline__ float power_of_two(int biased) { return __uint_as_float((unsigned)biased << 23); }
 
+// Sums of lanes 0 .. this one; the last lane's is the total.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // An element of either 16-bit type in 32 bits.
 template <bool BF16>
 __device__ __forceinline__ float f32_of_16(unsigned short bits) {

@@ -34,6 +34,9 @@ inline int check_paged_cache(const iex_paged_cache* c, const char* what, bool wr
   return 0;
 }
 
+// Rows of whole aligned 16-byte chunks.
+inline bool rows_of_chunks(const void* x, const long long* strides) { return aligned(x, 16) && strides[2] == 1 && strides[0] % 8 == 0 && strides[1] % 8 == 0; }
+
 inline PagedParams paged_params(const iex_paged_cache& c) {
   return PagedParams{c.pages, log2_of(c.page_size), c.kv_heads, c.seqs, c.table_width, c.key_page_stride, c.value_page_stride, c.table_stride,
                      c.keys, c.values, c.key_exponents, c.value_exponents, c.table, c.lengths};

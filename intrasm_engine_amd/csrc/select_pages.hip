@@ -47,7 +47,7 @@ __device__ __forceinline__ double group_sum64(double v) {
 }
 
 template <bool BF16, int D>
-__global__ __launch_bounds__(256) void page_score_kernel(SelectParams p) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void page_score_kernel(SelectParams p) {
   constexpr int L = D / 8, P = kWave / L, STEPS = kScorePages / 4 / P;   // lanes of a page, pages of a step
   const PagedParams& c = p.cache;
   const int row = blockIdx.y, seq = row / c.kv_heads, head = row % c.kv_heads;
