@@ -27,7 +27,8 @@ void check_no_gradient(const Tensor& t, const char* op) {
 
 struct Strides {
   long long of[3];
-  explicit Strides(const Tensor& t) : of{t.stride(0), t.stride(1), t.stride(2)} {}
+  // (of a single token or head none is used)
+  explicit Strides(const Tensor& t) : of{t.size(0) == 1 ? 0 : t.stride(0), t.size(1) == 1 ? 0 : t.stride(1), t.stride(2)} {}
 };
 
 // The cache as the C entry points take it; q is (rows, heads, head_dim).  keys / values undefined: bounds only.
@@ -134,7 +135,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& keys, const Tensor& values
     count = as_int(pages->size(2), op);
   }
   const c10::DeviceGuard guard(q.device());
-  if (pages && count == 0) return at::zeros_like(q);   // nothing to attend to
+  if ((pages && count == 0) || c.pages == 0) return at::zeros_like(q);   // nothing to attend to
   const Tensor out = at::empty_like(q);
   const int heads = as_int(q.size(1), op);
   const Strides qs(q), os(out);

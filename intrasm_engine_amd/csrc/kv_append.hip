@@ -5,18 +5,42 @@
 namespace iex {
 namespace {
 
-template <bool BF16, int D, bool E8, bool STAGED>
-int launch(const AppendParams& p, bool interleaved, dim3 grid, hipStream_t stream) {
-  note_kernel("kv_append_kernel<%s, %d, %s, %s, %s>", BF16 ? "bf16" : "f16", D, E8 ? "e4m3" : "16", STAGED ? "staged" : "rows", interleaved ? "interleaved" : "halves");
-  if (interleaved) hipLaunchKernelGGL((kv_append_kernel<BF16, D, E8, STAGED, true>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((kv_append_kernel<BF16, D, E8, STAGED, false>), grid, dim3(256), 0, stream, p);
+// Features whose tokens are whole aligned 16-byte chunks (up to the last ones).
+bool columns_of_chunks(const void* x, const long long* strides) { return aligned(x, 16) && strides[0] == 1 && strides[1] % 8 == 0 && strides[2] % 8 == 0; }
+
+template <bool BF16, int D, bool E8, bool INTERLEAVED>
+int launch(const AppendParams& p, bool rows, hipStream_t s) {
+  const char* type = BF16 ? "bf16" : "f16";
+  const char* stored = E8 ? "e4m3" : "16";
+  constexpr int per_step = 256 / (D / 16);   // rows of 256 threads
+  const int kv_heads = p.cache.kv_heads, kv_groups = ceil_div(kv_heads, p.per_group);
+  if (!p.offsets) {
+    note_kernel("kv_append_step_kernel<%s, %d, %s, %s>", type, D, stored, rows ? "rows" : "staged");
+    const dim3 grid(ceil_div(p.tokens, per_step), 2 * kv_heads + p.heads);
+    if (rows) hipLaunchKernelGGL((kv_append_step_kernel<BF16, D, E8, INTERLEAVED, false>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((kv_append_step_kernel<BF16, D, E8, INTERLEAVED, true>), grid, dim3(256), 0, s, p);
+    return check_hip(hipGetLastError(), "kv_append launch");
+  }
+  const dim3 grid((unsigned)append_most_spans(p.tokens, p.cache.seqs, append_span(1 << p.cache.page_shift)),
+                  (p.bounds ? kv_heads : kv_groups) + kv_groups + ceil_div(p.heads, p.per_group));
+  const int lds = (rows ? 0 : kColumnTokens * D * 2) + (p.bounds ? per_step * D * 4 : 0);
+  note_kernel("%s<%s, %d, %s>", rows ? "kv_append_kernel" : "kv_append_columns_kernel", type, D, stored);
+  if (!rows) hipLaunchKernelGGL((kv_append_columns_kernel<BF16, D, E8, INTERLEAVED>), grid, dim3(256), lds, s, p);
+  else if (p.per_group == 1) hipLaunchKernelGGL((kv_append_kernel<BF16, D, E8, INTERLEAVED, 1>), grid, dim3(256), lds, s, p);
+  else hipLaunchKernelGGL((kv_append_kernel<BF16, D, E8, INTERLEAVED, 4>), grid, dim3(256), lds, s, p);
   return check_hip(hipGetLastError(), "kv_append launch");
 }
 
-template <bool BF16, int D>
-int launch_forms(const AppendParams& p, bool e8, bool staged, bool interleaved, dim3 grid, hipStream_t s) {
-  if (e8) return staged ? launch<BF16, D, true, true>(p, interleaved, grid, s) : launch<BF16, D, true, false>(p, interleaved, grid, s);
-  return staged ? launch<BF16, D, false, true>(p, interleaved, grid, s) : launch<BF16, D, false, false>(p, interleaved, grid, s);
+template <bool BF16, int D, bool E8>
+int launch_forms(const AppendParams& p, bool rows, bool interleaved, hipStream_t s) {
+  return interleaved ? launch<BF16, D, E8, true>(p, rows, s) : launch<BF16, D, E8, false>(p, rows, s);
+}
+
+template <bool BF16>
+int launch_type(const AppendParams& p, int head_dim, bool e8, bool rows, bool interleaved, hipStream_t s) {
+  if (head_dim == 64) return e8 ? launch_forms<BF16, 64, true>(p, rows, interleaved, s) : launch_forms<BF16, 64, false>(p, rows, interleaved, s);
+  if (head_dim == 128) return e8 ? launch_forms<BF16, 128, true>(p, rows, interleaved, s) : launch_forms<BF16, 128, false>(p, rows, interleaved, s);
+  return e8 ? launch_forms<BF16, 256, true>(p, rows, interleaved, s) : launch_forms<BF16, 256, false>(p, rows, interleaved, s);
 }
 
 }  // namespace
@@ -42,30 +66,22 @@ extern "C" int iex_kv_append(const iex_paged_cache* cache, int tokens, const int
   AppendParams p{};
   p.cache = paged_params(*cache);
   p.tokens = tokens, p.heads = heads, p.rotary = rotary, p.offsets = offsets, p.rotation = rotation;
-  p.k = static_cast<const unsigned short*>(k), p.v = static_cast<const unsigned short*>(v);
-  p.q = static_cast<const unsigned short*>(q), p.q_out = static_cast<unsigned short*>(q_out);
-  p.bounds = static_cast<unsigned short*>(cache->bounds);
-  for (int i = 0; i < 3; ++i) {
-    p.k_strides[i] = k_strides[i], p.v_strides[i] = v_strides[i];
-    if (heads) p.q_strides[i] = q_strides[i], p.out_strides[i] = q_out_strides[i];
+  auto operand = [](const void* x, const long long* strides) { return AppendOperand{static_cast<const unsigned short*>(x), strides[0], strides[1], strides[2]}; };
+  p.k = operand(k, k_strides), p.v = operand(v, v_strides);
+  if (heads) {
+    p.q = operand(q, q_strides), p.q_out = static_cast<unsigned short*>(q_out);
+    p.out_token = q_out_strides[0], p.out_head = q_out_strides[1], p.out_feature = q_out_strides[2];
   }
-  const bool staged = !(rows_of_chunks(k, k_strides) && rows_of_chunks(v, v_strides) && (heads == 0 || (rows_of_chunks(q, q_strides) && rows_of_chunks(q_out, q_out_strides))));
+  p.bounds = static_cast<unsigned short*>(cache->bounds);
+  const bool rows = rows_of_chunks(k, k_strides) && rows_of_chunks(v, v_strides) && (heads == 0 || (rows_of_chunks(q, q_strides) && rows_of_chunks(q_out, q_out_strides)));
+  p.columns = columns_of_chunks(k, k_strides) && columns_of_chunks(v, v_strides) &&
+              (heads == 0 || (columns_of_chunks(q, q_strides) && columns_of_chunks(q_out, q_out_strides)));
   const long long spans = offsets ? append_most_spans(tokens, cache->seqs, append_span(cache->page_size)) : tokens;
   // one head to a workgroup until there are workgroups enough; then as many as share what they read of the rotation
   const long long all = spans * (2ll * cache->kv_heads + heads);
-  p.per_group = all > 8 * 2048 ? 8 : all > 2048 ? (int)(all / 2048) : 1;
-  const int kv_groups = ceil_div(cache->kv_heads, p.per_group);
-  const long long groups = (cache->bounds ? cache->kv_heads : kv_groups) + kv_groups + ceil_div(heads, p.per_group);
-  IEX_REQUIRE(spans < (1ll << 31) && groups < 65536, IEX_ERR_TOO_LARGE, "kv_append: too many tokens or heads");
-  const dim3 grid((unsigned)spans, (unsigned)groups);
+  p.per_group = all >= 16384 ? 8 : all >= 4096 ? 4 : 1;
+  IEX_REQUIRE(spans < (1ll << 31) && 2ll * cache->kv_heads + heads < 65536, IEX_ERR_TOO_LARGE, "kv_append: too many tokens or heads");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool e8 = cache->eight_bits;
-  if (cache->dtype == IEX_BF16) {
-    if (cache->head_dim == 64) return launch_forms<true, 64>(p, e8, staged, interleaved, grid, s);
-    if (cache->head_dim == 128) return launch_forms<true, 128>(p, e8, staged, interleaved, grid, s);
-    return launch_forms<true, 256>(p, e8, staged, interleaved, grid, s);
-  }
-  if (cache->head_dim == 64) return launch_forms<false, 64>(p, e8, staged, interleaved, grid, s);
-  if (cache->head_dim == 128) return launch_forms<false, 128>(p, e8, staged, interleaved, grid, s);
-  return launch_forms<false, 256>(p, e8, staged, interleaved, grid, s);
+  return cache->dtype == IEX_BF16 ? launch_type<true>(p, cache->head_dim, cache->eight_bits, rows, interleaved, s)
+                                  : launch_type<false>(p, cache->head_dim, cache->eight_bits, rows, interleaved, s);
 }

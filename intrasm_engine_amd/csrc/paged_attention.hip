@@ -5,29 +5,38 @@
 namespace iex {
 namespace {
 
-// Workgroups that are resident at once: three, four or five of four wavefronts on each of the 256 CUs, by their registers.
+// Workgroups of four wavefronts that are resident at once: by their registers one to four on each of the 256 CUs.
 int resident(int head_dim, bool e8) { return 256 * paged_simd_waves(head_dim, e8); }
 
-// Rows up to this many tiles of keys stay whole: a workgroup each, of eight wavefronts, and no second launch.
+// Rows of up to this many tiles stay whole, and there is no second launch: 32 x 700 tokens of 128 12.8 us, cut 14.5; 16 x 32 rows of
+// 600 .. 1023 39.7 and 44; 32 x 2000, the other side, 16 cut and 24 whole.
 constexpr int kWholeTiles = 8;
+// Whole rows go to eight wavefronts each where four would leave CUs without work: 128 rows of 700 13.1 us by eight, 17.5 by four; 512 of
+// 500 30.5 and 24.8.
+constexpr int kWideRows = 512;
+// Parts: one round of resident workgroups where rows are few (131071 tokens, 8 rows: 92.8 us, two rounds 99.8), two where rows of unequal
+// lengths come anyway (512 rows of 4000 .. 16384, e4m3: 225.6 one, 207.6 two, 207.7 three).
+constexpr int kTwoRounds = 256;
 
 struct Split {
-  long long blocks, workgroups;   // blocks of up to 16 heads of a key head; workgroups of the launch
+  long long blocks, slots, workgroups;   // blocks of up to 16 heads of a key head; parts beyond one per sequence; workgroups of the launch
   int pitch;
-  bool whole_rows;
+  bool wide;
 };
 Split split_of(const iex_paged_cache& c, int heads, int count) {
   const int group = heads / c.kv_heads, most = paged_tiles((count ? count : c.table_width) * c.page_size);
   Split s;
   s.blocks = (long long)c.kv_heads * ceil_div(group, 16);
   s.pitch = group < 16 ? group : 16;
-  s.whole_rows = most <= kWholeTiles;
-  const long long rows = s.blocks * c.seqs, stretches = rows * ((most + kPagedLeast - 1) / kPagedLeast);
-  s.workgroups = s.whole_rows ? rows : stretches < resident(c.head_dim, c.eight_bits) ? stretches : resident(c.head_dim, c.eight_bits);
+  const long long rows = s.blocks * c.seqs;
+  const bool whole = most <= kWholeTiles;
+  s.wide = whole && rows < kWideRows;
+  s.slots = whole ? 0 : paged_slots(resident(c.head_dim, c.eight_bits) * (rows < kTwoRounds ? 1 : 2) / s.blocks, c.seqs, most, kPagedLeast);
+  s.workgroups = s.blocks * (c.seqs + s.slots);
   return s;
 }
-// (two parts a workgroup, each rows x head_dim sums and rows pairs)
-size_t partial_floats(const iex_paged_cache& c, const Split& s) { return (size_t)s.workgroups * 2 * s.pitch * c.head_dim; }
+// (per part: rows x head_dim sums, then rows pairs)
+size_t partial_floats(const iex_paged_cache& c, const Split& s) { return (size_t)s.workgroups * s.pitch * c.head_dim; }
 
 template <bool BF16, int D, bool E8, int WAVES>
 int launch(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
@@ -45,16 +54,16 @@ int launch(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
   note_kernel("paged_attention_kernel<%s, %d, %s, %d>", BF16 ? "bf16" : "f16", D, E8 ? "e4m3" : "16", WAVES);
   hipLaunchKernelGGL(kern, dim3((unsigned)s.workgroups), dim3(WAVES * kWave), lds, stream, p);
   if (int rc = check_hip(hipGetLastError(), "paged attention launch")) return rc;
-  if (s.whole_rows) return 0;
+  if (s.slots == 0) return 0;
   note_kernel("paged_join_kernel<%s, %d>", BF16 ? "bf16" : "f16", D);
-  hipLaunchKernelGGL((paged_join_kernel<BF16, D>), dim3((unsigned)p.cache.seqs, (unsigned)p.heads), dim3(256), 0, stream, p, (int)s.workgroups);
+  hipLaunchKernelGGL((paged_join_kernel<BF16, D>), dim3((unsigned)p.cache.seqs, (unsigned)p.heads), dim3(256), 0, stream, p);
   return check_hip(hipGetLastError(), "paged attention join launch");
 }
 
 template <bool BF16, int D, bool E8>
 int launch_waves(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
   constexpr int wide = paged_simd_waves(D, E8) > 1 ? 8 : 4;
-  return s.whole_rows ? launch<BF16, D, E8, wide>(p, s, stream) : launch<BF16, D, E8, 4>(p, s, stream);
+  return s.wide ? launch<BF16, D, E8, wide>(p, s, stream) : launch<BF16, D, E8, 4>(p, s, stream);
 }
 
 template <bool BF16>
@@ -78,8 +87,8 @@ extern "C" size_t iex_paged_attention_workspace_bytes(const iex_paged_cache* cac
   using namespace iex;
   if (check_paged_cache(cache, "paged_attention", false) || check_heads(cache, heads, "paged_attention") || heads == 0 || cache->seqs == 0 || count < 0) return 0;
   const Split s = split_of(*cache, heads, count);
-  if (s.whole_rows) return 0;
-  return partial_floats(*cache, s) * 4 + (size_t)s.workgroups * 2 * s.pitch * 8;
+  if (s.slots == 0) return 0;
+  return partial_floats(*cache, s) * 4 + (size_t)s.workgroups * s.pitch * 8;
 }
 
 extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, float scale, const int* listed, int count,
@@ -92,6 +101,7 @@ extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, cons
   IEX_REQUIRE(listed || count == 0, IEX_ERR_BAD_ARGUMENT, "paged_attention: null pointer argument");
   IEX_REQUIRE((long long)count * cache->page_size < (1ll << 30), IEX_ERR_TOO_LARGE, "paged_attention: up to 2^30 tokens in a list of pages");
   if (cache->seqs == 0 || heads == 0) return 0;
+  IEX_REQUIRE(cache->pages > 0, IEX_ERR_BAD_ARGUMENT, "paged_attention: a cache without pages");
   IEX_REQUIRE(q && q_strides && out && out_strides, IEX_ERR_BAD_ARGUMENT, "paged_attention: null pointer argument");
   IEX_REQUIRE(aligned(q, 2) && aligned(out, 2), IEX_ERR_UNSUPPORTED, "paged_attention: operands must be aligned to their elements");
   IEX_REQUIRE(scale > 0.f && scale < 1e30f, IEX_ERR_UNSUPPORTED, "paged_attention: the scale must be positive and finite");
@@ -104,7 +114,7 @@ extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, cons
   PagedAttentionParams p{};
   p.cache = paged_params(*cache);
   p.heads = heads, p.group = heads / cache->kv_heads, p.group_tiles = ceil_div(p.group, 16), p.pitch = s.pitch;
-  p.count = count, p.listed = listed, p.whole_rows = s.whole_rows;
+  p.count = count, p.listed = listed, p.blocks = (int)s.blocks, p.slots = (int)s.slots;
   p.q = static_cast<const unsigned short*>(q), p.out = static_cast<unsigned short*>(out);
   for (int i = 0; i < 3; ++i) p.q_strides[i] = q_strides[i], p.out_strides[i] = out_strides[i];
   p.q_rows = rows_of_chunks(q, q_strides);

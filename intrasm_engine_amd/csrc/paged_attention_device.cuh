@@ -25,7 +25,7 @@ struct PagedAttentionParams {
   PagedParams cache;
   int heads, group, group_tiles;   // query heads, those of a key head, blocks of 16 of them
   int pitch, count;                // query rows of a part's result; pages listed per sequence and key head, 0: all of the table
-  bool whole_rows;                 // a workgroup per row, else equal stretches of all tiles
+  int blocks, slots;               // blocks of up to 16 query heads of a key head; parts beyond one per sequence (0: rows are whole)
   const int* listed;
   const unsigned short* q;
   unsigned short* out;
@@ -38,36 +38,47 @@ struct PagedAttentionParams {
 
 constexpr int kPagedLeast = 2;   // tiles that are worth a workgroup
 
-__device__ __forceinline__ int row_tokens(const PagedAttentionParams& p, int seq) {
-  const int length = cached_length(p.cache.lengths[seq], p.cache.table_width, 1 << p.cache.page_shift);
-  return p.count && length ? p.count << p.cache.page_shift : length;
+// The lengths of 64 sequences, one a lane.
+struct LaneLengths {
+  int from = -kWave, mine = 0;
+  __device__ __forceinline__ void load(const PagedParams& c, int first) {
+    const int s = first + lane_id();
+    from = first;
+    mine = s < c.seqs ? cached_length(c.lengths[s], c.table_width, 1 << c.page_shift) : 0;
+  }
+  __device__ __forceinline__ int of(const PagedParams& c, int seq) {
+    if (seq < from || seq >= from + kWave) load(c, seq);
+    return bcast_i(mine, seq - from);
+  }
+};
+// Tokens that a sequence of this length is work for: itself, or as many pages as are listed.
+__device__ __forceinline__ int row_tokens(const PagedAttentionParams& p, int length) { return p.count && length ? p.count << p.cache.page_shift : length; }
+__device__ __forceinline__ int lane_tiles(const PagedAttentionParams& p, const LaneLengths& l) {
+  return l.from + lane_id() < p.cache.seqs ? paged_tiles(row_tokens(p, l.mine)) : 0;
 }
-__device__ __forceinline__ int lane_tiles(const PagedAttentionParams& p, int seq) { return seq < p.cache.seqs ? paged_tiles(row_tokens(p, seq)) : 0; }
-// Tiles of all sequences (of one block of heads).
-__device__ __forceinline__ int all_tiles(const PagedAttentionParams& p) {
+
+// The first sequence that `match` says yes to (its number, its first part's, its parts), by the lengths; `lengths` holds its.
+template <typename MATCH>
+__device__ __forceinline__ bool find_part(const PagedAttentionParams& p, LaneLengths& lengths, MATCH match, int& seq, int& first, int& parts, int& tiles) {
   int total = 0;
-  for (int s0 = 0; s0 < p.cache.seqs; s0 += kWave) total += lane_tiles(p, s0 + lane_id());
-  return bcast_i(wave_scan(total), kWave - 1);
-}
-// The sequence that has tile `at` of them, and the first of its tiles.
-__device__ __forceinline__ int sequence_at(const PagedAttentionParams& p, int at, int& first) {
+  for (int s0 = 0; s0 < p.cache.seqs; s0 += kWave) {
+    lengths.load(p.cache, s0);
+    total += lane_tiles(p, lengths);
+  }
+  const int most = paged_part_most(bcast_i(wave_scan(total), kWave - 1), p.slots, kPagedLeast);
   int before = 0;
-  for (int s0 = 0;; s0 += kWave) {
-    const int tiles = lane_tiles(p, s0 + lane_id()), upto = before + wave_scan(tiles);
-    const unsigned long long past = __ballot(upto > at);
-    if (past || s0 + kWave >= p.cache.seqs) {   // (the latter: never, at < all_tiles())
-      const int lane = past ? __ffsll(past) - 1 : 0;
-      first = bcast_i(upto - tiles, lane);
-      return min(s0 + lane, p.cache.seqs - 1);
+  for (int s0 = 0; s0 < p.cache.seqs; s0 += kWave) {
+    if (p.cache.seqs > kWave) lengths.load(p.cache, s0);
+    const int mine = lane_tiles(p, lengths), n = s0 + lane_id() < p.cache.seqs ? paged_parts(mine, most) : 0, upto = before + wave_scan(n);
+    const unsigned long long hit = __ballot(match(s0 + lane_id(), upto - n, n));
+    if (hit) {
+      const int lane = __ffsll(hit) - 1;
+      seq = s0 + lane, first = bcast_i(upto - n, lane), parts = bcast_i(n, lane), tiles = bcast_i(mine, lane);
+      return true;
     }
     before = bcast_i(upto, kWave - 1);
   }
-}
-// ... and the first tile of a sequence.
-__device__ __forceinline__ int tiles_before(const PagedAttentionParams& p, int seq) {
-  int total = 0;
-  for (int s0 = 0; s0 < seq; s0 += kWave) total += s0 + lane_id() < seq ? lane_tiles(p, s0 + lane_id()) : 0;
-  return bcast_i(wave_scan(total), kWave - 1);
+  return false;
 }
 
 // Two e4m3 codes of a dword to a pair of 16-bit values (exact).
@@ -75,6 +86,13 @@ template <bool BF16, bool HIGH>
 __device__ __forceinline__ unsigned widen_pair(unsigned codes) {
   if constexpr (BF16) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.f, HIGH));
   else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, HIGH));
+}
+
+// A load, with the streaming hint where what is read is far larger than the caches.
+template <bool STREAM, typename T>
+__device__ __forceinline__ T load_from(const T* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
 }
 
 // Wavefronts of a SIMD that the registers are cut for.
@@ -93,35 +111,24 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   extern __shared__ __align__(16) float smem[];
   const int wave = uniform(threadIdx.x >> 6);
   const PagedParams& cache = p.cache;
+  LaneLengths lengths;
 
-  // ---- this workgroup's stretch of the line of tiles ----
-  int seq, block, total = 0;
-  long long at = 0, stretch_begin = 0, stretch_end = 0, row0 = 0;
-  if (p.whole_rows) {
-    seq = blockIdx.x % cache.seqs, block = blockIdx.x / cache.seqs;
+  // ---- whose part ----
+  const int block = blockIdx.x % p.blocks, item = blockIdx.x / p.blocks;
+  int seq = item, part = 0, parts = 1, tiles = 1;
+  if (p.slots == 0) {
+    lengths.load(cache, seq);
+    tiles = paged_tiles(row_tokens(p, lengths.of(cache, seq)));
+  } else if (!find_part(p, lengths, [&](int, int first, int n) { return first + n > item; }, seq, part, parts, tiles)) {
+    return;
   } else {
-    total = all_tiles(p);
-    const long long line = (long long)total * (cache.kv_heads * p.group_tiles), stretch = paged_stretch(line, gridDim.x, kPagedLeast);
-    at = stretch_begin = stretch * blockIdx.x;
-    stretch_end = min(line, stretch_begin + stretch);
-    if (at >= line) return;
-    block = (int)(at / total);
-    int first;
-    seq = sequence_at(p, (int)(at - (long long)block * total), first);
-    row0 = (long long)block * total + first;
+    part = item - part;
   }
-
-  for (;;) {   // the rows of the stretch
-  int lane = threadIdx.x & 63;
-  asm volatile("" : "+v"(lane));   // (what follows from the lane is worked out again for each row: kept for all of them it is spilled)
-  const int col = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int kv_head = block / p.group_tiles, group_tile = block % p.group_tiles;
   const int rows = min(16, p.group - group_tile * 16);   // queries
-  const int length = cached_length(cache.lengths[seq], cache.table_width, 1 << cache.page_shift);
-  const int tokens = p.count && length ? p.count << cache.page_shift : length, tiles = paged_tiles(tokens);
-  PagedPart part{0, tiles, 0, true};
-  if (!p.whole_rows) part = paged_part(row0, tiles, at, stretch_begin, stretch_end, blockIdx.x);
-  const int begin = part.from * kPagedTile, end = min(tokens, part.to * kPagedTile);
+  const int length = lengths.of(cache, seq), tokens = row_tokens(p, length);
+  const int begin = paged_part_begin(tiles, parts, part) * kPagedTile, end = min(tokens, paged_part_begin(tiles, parts, part + 1) * kPagedTile);
 
   // ---- queries: columns of the first product ----
   u32x4 fq[KS];
@@ -129,12 +136,13 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   for (int s = 0; s < KS; ++s) fq[s] = u32x4{0u, 0u, 0u, 0u};
   if (col < rows) {
     const u16* q = p.q + seq * p.q_strides[0] + (long long)(kv_head * p.group + group_tile * 16 + col) * p.q_strides[1];
+    if (p.q_rows) {   // rows of aligned 16-byte chunks
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = E8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8;
-      if (p.q_rows) {   // rows of aligned 16-byte chunks
-        fq[s] = *reinterpret_cast<const u32x4*>(q + d);
-      } else {
+      for (int s = 0; s < KS; ++s) fq[s] = *reinterpret_cast<const u32x4*>(q + (E8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8));
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = E8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8;
         unsigned w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = q[(d + 2 * j) * p.q_strides[2]] | (unsigned)q[(d + 2 * j + 1) * p.q_strides[2]] << 16;
@@ -172,8 +180,8 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
       if (place.entry >= window + kWave) look_up(place.entry);
       const int page = bcast_i(entry_page, place.entry - window), logical = bcast_i(entry_logical, place.entry - window);
       w.valid[a] = place.entry < entries ? paged_valid(logical, place.slot, cache.page_shift, page, cache.pages, length) : 0;
-      w.page[a] = w.valid[a] ? page : 0;
-      w.row[a] = (kv_head << cache.page_shift) + place.slot;
+      w.page[a] = page, w.row[a] = (kv_head << cache.page_shift) + place.slot;
+      if (w.valid[a] == 0) w.page[a] = a ? w.page[0] : 0, w.row[a] = a ? w.row[0] : w.row[a];
     }
     return w;
   };
@@ -185,7 +193,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
     for (int a = 0; a < 2; ++a) {
       const unsigned char* k = static_cast<const unsigned char*>(cache.keys) + (w.page[a] * cache.key_page + (long long)w.row[a] * D) * ES;
 #pragma unroll
-      for (int s = 0; s < KW; ++s) key[a][s] = *reinterpret_cast<const u32x4*>(k + (col * (D * ES) + s * 64 + g * 16));
+      for (int s = 0; s < KW; ++s) key[a][s] = load_from<WAVES == 4>(reinterpret_cast<const u32x4*>(k + (col * (D * ES) + s * 64 + g * 16)));
       if constexpr (E8)
         ke[a] = *reinterpret_cast<const unsigned*>(cache.key_exponents + (((long long)w.page[a] * cache.kv_heads) << cache.page_shift) + w.row[a] + g * 4);
     }
@@ -198,7 +206,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int h = 0; h < VWORDS; ++h) value[a][i][h] = *reinterpret_cast<const VWord*>(v + ((g * 4 + i) * (D * ES) + h * 256 + col * (int)sizeof(VWord)));
+        for (int h = 0; h < VWORDS; ++h) value[a][i][h] = load_from<WAVES == 4>(reinterpret_cast<const VWord*>(v + ((g * 4 + i) * (D * ES) + h * 256 + col * (int)sizeof(VWord))));
       if constexpr (E8)
         ve[a] = *reinterpret_cast<const unsigned*>(cache.value_exponents + (((long long)w.page[a] * cache.kv_heads) << cache.page_shift) + w.row[a] + g * 4);
     }
@@ -367,39 +375,31 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
       all += keep * share;
       acc += keep * sums[(w * rows + row) * D + d];
     }
-    if (part.whole) {
+    if (parts == 1) {
       const int head = kv_head * p.group + group_tile * 16 + row;
       p.out[seq * p.out_strides[0] + head * p.out_strides[1] + d * p.out_strides[2]] = f32_to_16(any ? acc / all : 0.f, BF16);
     } else {
-      const size_t to = (size_t)part.place * p.pitch + row;
+      const size_t to = (size_t)blockIdx.x * p.pitch + row;
       p.partial[to * D + d] = acc;
       if (d == 0) p.stats[to * 2] = m, p.stats[to * 2 + 1] = any ? all : -1.f;
     }
-  }
-  if (p.whole_rows) return;
-  at = row0 + part.to;
-  if (at >= stretch_end) return;
-  row0 = at;   // (the row is through: the stretch goes on)
-  if (++seq == cache.seqs) seq = 0, ++block;
-  __syncthreads();   // everybody has read the sums
   }
 }
 
 // Parts of a row into its result, a workgroup per sequence and query head: the parts' weights first, 256 at a time, then
 // 256 / (D / 4) parts side by side, a thread four features; they meet in LDS.
 template <bool BF16, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p, int workgroups) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p) {
   constexpr int LANES = D / 4, SIDE = 256 / LANES;   // threads of a row; parts side by side
   __shared__ float4 accs[SIDE][LANES];
   __shared__ float weights[256], tops[4], sums[4];
   const int seq = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
   const int kv_head = head / p.group, in_group = head % p.group;
-  const int of_all = all_tiles(p), block = kv_head * p.group_tiles + in_group / 16;
-  const long long blocks = (long long)p.cache.kv_heads * p.group_tiles, row = (long long)block * of_all + tiles_before(p, seq);
-  const PagedParts parts = paged_parts(row, paged_tiles(row_tokens(p, seq)), paged_stretch(of_all * blocks, workgroups, kPagedLeast));
-  if (parts.first == parts.last) return;
-  const int number = parts.last - parts.first + 1;
-  auto place = [&](int i) { return (size_t)((parts.first + i) * 2 + (i == 0 && parts.second ? 1 : 0)) * p.pitch + in_group % 16; };
+  LaneLengths lengths;
+  int found, first, number, tiles;
+  if (!find_part(p, lengths, [&](int s, int, int) { return s == seq; }, found, first, number, tiles) || number == 1) return;
+  const int block = kv_head * p.group_tiles + in_group / 16;
+  auto place = [&](int i) { return ((size_t)(first + i) * p.blocks + block) * p.pitch + in_group % 16; };
   const int lane = tid % LANES, side = tid / LANES;
   float4 acc = {0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, total = 0.f;

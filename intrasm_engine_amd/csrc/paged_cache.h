@@ -17,46 +17,27 @@ IEX_HD int cached_length(int length, int table_width, int page_size) {
 }
 
 // ---- attention: rows in parts -----------------------------------------------------------------------------------------
-// A row is a sequence with one block of up to 16 query heads of a key head.  Rows are tiles of kPagedTile tokens, at least one (an
-// empty sequence's zeros are work too); all tiles, the rows of a block after each other, block by block, are one line that the
-// workgroups cut into equal stretches.  So a workgroup has the end of one row, whole rows, the beginning of another; a row that is
-// not whole anywhere is joined from what its workgroups leave, at most two parts each.
+// A row is a sequence with one block of up to 16 query heads of a key head.  Rows of more than a certain number of tiles are cut
+// into equal parts, a workgroup each; an empty sequence is one part too, which writes its zeros.
 constexpr int kPagedTile = 128;   // tokens
 
 IEX_HD int paged_tiles(int tokens) { return tokens <= kPagedTile ? 1 : tokens / kPagedTile + (tokens % kPagedTile != 0); }
 
-// Tiles of a workgroup's stretch.  `least`: fewer are not worth a workgroup.
-IEX_HD long long paged_stretch(long long tiles, int workgroups, int least) {
-  const long long even = tiles / workgroups + (tiles % workgroups != 0);
+// Tiles that a part has at most, where `total` tiles (of all sequences, one block of heads) go to about `slots` workgroups.  The
+// parts of all sequences are at most `slots` more than there are sequences: one has one more than whole parts fit into it.
+IEX_HD int paged_part_most(int total, int slots, int least) {
+  if (slots == 0) return 1 << 30;
+  const int even = total / slots + (total % slots != 0);
   return even > least ? even : least;
 }
+IEX_HD int paged_parts(int tiles, int most) { return tiles <= most ? 1 : tiles / most + (tiles % most != 0); }
+// The first tile of a part (of part number `parts`: the end).
+IEX_HD int paged_part_begin(int tiles, int parts, int part) { return (int)((long long)tiles * part / parts); }
 
-// A row's part in a workgroup: tiles from .. to of the row, and where the workgroup leaves its sums if that is not all of them.
-struct PagedPart {
-  int from, to, place;
-  bool whole;
-};
-// `row`: the line's tile that is the row's first; `tiles`: how many it has; `at`: the line's tile that the workgroup has come to;
-// `begin`, `end`: its stretch.
-IEX_HD PagedPart paged_part(long long row, int tiles, long long at, long long begin, long long end, int workgroup) {
-  PagedPart p;
-  p.from = (int)(at - row);
-  p.to = end - row < tiles ? (int)(end - row) : tiles;
-  p.whole = p.from == 0 && p.to == tiles;
-  p.place = workgroup * 2 + (at > begin ? 1 : 0);
-  return p;
-}
-// The parts of a row, for who joins them: workgroups first .. last, a place each.
-struct PagedParts {
-  int first, last;
-  bool second;   // the first workgroup's part is its second place
-};
-IEX_HD PagedParts paged_parts(long long row, int tiles, long long stretch) {
-  PagedParts p;
-  p.first = (int)(row / stretch);
-  p.last = (int)((row + tiles - 1) / stretch);
-  p.second = row % stretch != 0;
-  return p;
+// Slots that are worth having: none where no sequence can be long enough to be cut.
+IEX_HD long long paged_slots(long long wanted, long long seqs, int most_tiles, int least) {
+  const long long most = seqs * ((most_tiles + least - 1) / least - 1);
+  return most < wanted ? (most < 0 ? 0 : most) : wanted < 1 ? 1 : wanted;
 }
 
 // Where 16 tokens of a sequence from `token` on lie (16 divides token and the page): entry `entry` of the sequence's table (or
@@ -81,8 +62,7 @@ IEX_HD int append_span(int page_size) { return page_size > 64 ? page_size : 64; 
 // The new tokens of one sequence: tokens first .. first + count of the call at positions from `position` on.  Not `sound`: it
 // has no place for them (a length beyond its table or short of its new tokens); they are passed over.
 struct Appended {
-  int first, count, position;
-  bool sound;
+  int first, count, position, sound;
 };
 // offsets == nullptr: one token per sequence.  Sequence number `seqs` stands for the tokens behind the last sequence's.
 IEX_HD Appended appended(int s, int seqs, int tokens, int begin, int end, int length, int most) {

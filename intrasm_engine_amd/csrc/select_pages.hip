@@ -5,9 +5,10 @@
 // last to be selected does not depend on the order of summation.  (64-bit multiply-adds run at the rate of 32-bit ones here, and
 // reading the bounds is what takes the time.)
 //
-// Two launches: scores as whole numbers in their order (a wavefront's 16-lane group, or 8 or 32 lanes, reads a page's bounds, 16
-// bytes a lane), then per sequence and key head the count-th largest by four rounds of histograms of 8 bits, and the pages above
-// it in ascending order.
+// Scores are whole numbers in the scores' order (a wavefront's 16-lane group, or 8 or 32 lanes, reads a page's bounds, 16 bytes a
+// lane); then the count-th largest by four rounds of histograms of 8 bits, and the pages above it in ascending order.  One workgroup
+// does both for a sequence and key head, its scores in LDS, where that keeps the chip busy or the scores are few; else the scores
+// come from a launch of their own.
 #include "paged_cache_host.h"
 
 namespace iex {
@@ -16,6 +17,7 @@ namespace {
 struct SelectParams {
   PagedParams cache;
   int group, count, first, last;
+  int per_group;   // pages of a workgroup that only scores
   const unsigned short* q;
   long long q_strides[3];
   const unsigned short* bounds;
@@ -23,105 +25,163 @@ struct SelectParams {
   int* out;         // (seqs * kv_heads, count)
 };
 
-constexpr int kScorePages = 128, kSelectThreads = 512, kSelectKept = 12288;   // pages of a workgroup; ... whose keys fit in LDS
+constexpr int kSelectThreads = 1024, kSelectKept = 12288;   // ... whose pages' scores fit in LDS
+constexpr int chunk_of(int head_dim) { return head_dim == 256 ? 16 : 32; }   // pages that a wavefront scores at a time
 
 __device__ __forceinline__ int used_pages(const PagedParams& c, int seq) {
   const int length = cached_length(c.lengths[seq], c.table_width, 1 << c.page_shift);
   return (length + (1 << c.page_shift) - 1) >> c.page_shift;
 }
 
-template <int CTRL>
-__device__ __forceinline__ double dpp_add(double v) {
-  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
-  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true);
-  return v + __hiloint2double(hi, lo);
+// The value of the lane whose number differs in bit BIT.
+template <int BIT>
+__device__ __forceinline__ int from_neighbour(int v) {
+  if constexpr (BIT == 0) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);        // quad_perm [1,0,3,2]
+  else if constexpr (BIT == 1) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);   // quad_perm [2,3,0,1]
+  else if constexpr (BIT == 2) return __builtin_amdgcn_ds_swizzle(v, 0x101F);                    // xor 4
+  else if constexpr (BIT == 3) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, true);  // row_ror 8
+  else return __shfl_xor(v, 1 << BIT);
 }
-template <int LANES>
-__device__ __forceinline__ double group_sum64(double v) {
-  v = dpp_add<0xB1>(v);
-  v = dpp_add<0x4E>(v);
-  v = dpp_add<0x141>(v);
-  if (LANES >= 16) v = dpp_add<0x140>(v);
-  if (LANES >= 32) v += __shfl_xor(v, 16);
-  return v;
+template <int BIT>
+__device__ __forceinline__ double from_neighbour(double v) {
+  return __hiloint2double(from_neighbour<BIT>(__double2hiint(v)), from_neighbour<BIT>(__double2loint(v)));
+}
+// COUNT sums over LANES lanes each, at once: in the end lane l has sum number l % COUNT.  (One by one they take four times the additions
+// and exchanges.)
+template <int COUNT, int LANES, int BIT = 0>
+__device__ __forceinline__ double group_sums(double (&v)[COUNT]) {
+  if constexpr ((1 << BIT) == LANES) {
+    return v[0];
+  } else if constexpr ((1 << BIT) < COUNT) {
+    const bool odd = lane_id() >> BIT & 1;
+    // (the sums left are COUNT >> BIT; every second one goes to the neighbour)
+#pragma unroll
+    for (int k = 0; k < (COUNT >> BIT) / 2; ++k) {
+      const double mine = odd ? v[2 * k + 1] : v[2 * k], other = odd ? v[2 * k] : v[2 * k + 1];
+      v[k] = mine + from_neighbour<BIT>(other);
+    }
+    return group_sums<COUNT, LANES, BIT + 1>(v);
+  } else {
+    v[0] += from_neighbour<BIT>(v[0]);
+    return group_sums<COUNT, LANES, BIT + 1>(v);
+  }
+}
+
+// The weights of smallest and largest keys for a sequence and key head, into LDS (by all threads; a barrier follows).
+template <bool BF16, int D>
+__device__ __forceinline__ void page_weights(const SelectParams& p, int seq, int head, double (&weights)[2 * D]) {
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    double low = 0.0, high = 0.0;
+    const unsigned short* q = p.q + seq * p.q_strides[0] + (long long)head * p.group * p.q_strides[1] + d * p.q_strides[2];
+    for (int g0 = 0; g0 < p.group; g0 += 8) {   // (eight loads at a time: one after the other they take a microsecond each)
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = f32_of_16<BF16>(q[min(g0 + i, p.group - 1) * p.q_strides[1]]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (g0 + i >= p.group) break;
+        low += x[i] > 0.f ? 0.0 : (double)x[i];   // (a NaN is in both)
+        high += x[i] < 0.f ? 0.0 : (double)x[i];
+      }
+    }
+    weights[d] = low, weights[D + d] = high;
+  }
+}
+
+// The scores of chunks of a row's pages from page0 on, every `step` pages, to keys[].  `all`: there are no more pages than are
+// wanted, so each that exists is.
+template <bool BF16, int D>
+__device__ __forceinline__ void score_pages(const SelectParams& p, int seq, int head, int used, int page0, int step, int end, bool all, const double (&weights)[2 * D],
+                                            unsigned* keys) {
+  constexpr int L = D / 8, P = kWave / L, CHUNK = chunk_of(D), STEPS = CHUNK / P;   // lanes of a page, pages of a step
+  const PagedParams& c = p.cache;
+  const int lane = lane_id(), d = lane % L * 8;
+  const int* table = c.table + (size_t)seq * c.table_row;
+  auto find = [&](int first) {   // where a chunk's pages lie, one a lane
+    const int number = first + lane;
+    const int at = lane < CHUNK && number < used ? table[number] : -1;
+    return (unsigned)at < (unsigned)c.pages ? at : -1;
+  };
+  if (page0 >= end) return;
+  int at = find(page0);
+  if (all) {
+    for (; page0 < end; page0 += step) {
+      if (lane < CHUNK && page0 + lane < used) keys[page0 + lane] = at < 0 ? 0u : kSelectAlways;
+      if (page0 + step < end) at = find(page0 + step);
+    }
+    return;
+  }
+  double wl[8], wh[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) wl[j] = weights[d + j], wh[j] = weights[D + d + j];
+  for (; page0 < end; page0 += step) {
+    u32x4 lo[STEPS], hi[STEPS];
+    const int instead = max(0, bcast_i(at, 0));
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {   // (in the place of a page that is not there: the chunk's first)
+      const int page = __shfl(at, i * P + lane / L);
+      const unsigned short* b = p.bounds + ((size_t)(page < 0 ? instead : page) * c.kv_heads + head) * (2 * D) + d;
+      lo[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(b));
+      hi[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(b + D));
+    }
+    const int next = page0 + step < end ? find(page0 + step) : -1;
+    double sums[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) sums[i] = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)   // (the steps side by side: one sum is a chain)
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        float a, b;
+        unpack_pair<BF16>(lo[i][j], a, b);
+        sums[i] = fma((double)a, wl[2 * j], sums[i]);
+        sums[i] = fma((double)b, wl[2 * j + 1], sums[i]);
+        unpack_pair<BF16>(hi[i][j], a, b);
+        sums[i] = fma((double)a, wh[2 * j], sums[i]);
+        sums[i] = fma((double)b, wh[2 * j + 1], sums[i]);
+      }
+    const double sum = group_sums<STEPS, L>(sums);
+    const int in_chunk = lane % STEPS * P + lane / L, number = page0 + in_chunk, page = __shfl(at, in_chunk);
+    const bool always = number < p.first || number >= used - p.last;
+    if (lane % L < STEPS && number < used) keys[number] = page < 0 ? 0u : always ? kSelectAlways : select_key(__float_as_uint((float)sum));
+    at = next;
+  }
 }
 
 template <bool BF16, int D>
 __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void page_score_kernel(SelectParams p) {
-  constexpr int L = D / 8, P = kWave / L, STEPS = kScorePages / 4 / P;   // lanes of a page, pages of a step
+  __shared__ double weights[2 * D];
   const PagedParams& c = p.cache;
-  const int row = blockIdx.y, seq = row / c.kv_heads, head = row % c.kv_heads;
-  const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), used = used_pages(c, seq);
-  const int page0 = blockIdx.x * kScorePages + wave * (kScorePages / 4);
-  if (page0 >= used) return;
-  // where the wavefront's pages lie
-  int at = -1;
-  if (lane < kScorePages / 4 && page0 + lane < used) at = c.table[(size_t)seq * c.table_row + page0 + lane];
-  if ((unsigned)at >= (unsigned)c.pages) at = -1;
-  const int d = lane % L * 8;
-  u32x4 lo[STEPS], hi[STEPS];
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int page = __shfl(at, i * P + lane / L);
-    lo[i] = hi[i] = u32x4{0u, 0u, 0u, 0u};
-    if (page >= 0) {
-      const unsigned short* b = p.bounds + ((size_t)page * c.kv_heads + head) * (2 * D) + d;
-      lo[i] = *reinterpret_cast<const u32x4*>(b);
-      hi[i] = *reinterpret_cast<const u32x4*>(b + D);
-    }
-  }
-  double wl[8], wh[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) wl[j] = wh[j] = 0.0;
-  for (int g = 0; g < p.group; ++g) {
-    const unsigned short* q = p.q + seq * p.q_strides[0] + (long long)(head * p.group + g) * p.q_strides[1] + d * p.q_strides[2];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = f32_of_16<BF16>(q[j * p.q_strides[2]]);
-      // (a NaN is in both)
-      wl[j] += x > 0.f ? 0.0 : (double)x;
-      wh[j] += x < 0.f ? 0.0 : (double)x;
-    }
-  }
-  unsigned* keys = p.keys + (size_t)row * c.table_width;
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float a, b;
-      unpack_pair<BF16>(lo[i][j], a, b);
-      sum = fma((double)a, wl[2 * j], sum);
-      sum = fma((double)b, wl[2 * j + 1], sum);
-      unpack_pair<BF16>(hi[i][j], a, b);
-      sum = fma((double)a, wh[2 * j], sum);
-      sum = fma((double)b, wh[2 * j + 1], sum);
-    }
-    sum = group_sum64<L>(sum);
-    const int number = page0 + i * P + lane / L, page = __shfl(at, i * P + lane / L);
-    if (lane % L == 0 && number < used) {
-      const bool always = number < p.first || number >= used - p.last;
-      keys[number] = page < 0 ? 0u : always ? kSelectAlways : select_key(__float_as_uint((float)sum));
-    }
-  }
+  const int row = blockIdx.y, seq = row / c.kv_heads, head = row % c.kv_heads, wave = uniform(threadIdx.x >> 6);
+  const int used = used_pages(c, seq), first = blockIdx.x * p.per_group, end = min(used, first + p.per_group);
+  if (first >= end) return;
+  page_weights<BF16, D>(p, seq, head, weights);
+  __syncthreads();
+  score_pages<BF16, D>(p, seq, head, used, first + wave * chunk_of(D), 4 * chunk_of(D), end, used <= p.count || c.pages == 0, weights, p.keys + (size_t)row * c.table_width);
 }
 
-// KEPT: the row's keys stay in LDS, else every round reads them again.
-template <bool KEPT>
+// KEPT: the row's keys stay in LDS, else every round reads them again.  SCORED: they are in p.keys, else they are worked out here
+// (from D features of 16 bits; KEPT only).
+template <bool KEPT, bool SCORED, bool BF16, int D>
 __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParams p) {
   constexpr int WAVES = kSelectThreads / kWave;
   extern __shared__ unsigned kept[];
+  __shared__ double weights[SCORED ? 2 : 2 * D];
   __shared__ unsigned histogram[256];
-  __shared__ int chosen[2], totals[2][WAVES];
+  __shared__ int chosen[3], totals[2][WAVES];
   const PagedParams& c = p.cache;
   const int row = blockIdx.x, seq = row / c.kv_heads, tid = threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
   const int used = used_pages(c, seq);
-  const unsigned* keys = p.keys + (size_t)row * c.table_width;
+  const unsigned* keys = SCORED ? p.keys + (size_t)row * c.table_width : nullptr;
   int* out = p.out + (size_t)row * p.count;
-  if (KEPT) {
-    for (int i = tid; i < used; i += kSelectThreads) kept[i] = keys[i];
+  if constexpr (!SCORED) {
+    page_weights<BF16, D>(p, seq, row % c.kv_heads, weights);
     __syncthreads();
+    score_pages<BF16, D>(p, seq, row % c.kv_heads, used, wave * chunk_of(D), WAVES * chunk_of(D), used, used <= p.count || c.pages == 0, weights, kept);
+  } else if (KEPT) {
+    for (int i = tid; i < used; i += kSelectThreads) kept[i] = keys[i];
   }
+  __syncthreads();
   auto key_of = [&](int i) { return KEPT ? kept[i] : keys[i]; };
 
   // ---- the count-th largest key ----
@@ -129,9 +189,10 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
   int need = p.count;   // of the keys that agree with it in the bits found so far, the need-th largest
   if (used > p.count) {
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelectThreads) histogram[i] = 0;
+      if (tid < 256) histogram[tid] = 0;
       __syncthreads();
-      for (int i = tid; i < (used + kWave - 1) / kWave * kWave; i += kSelectThreads) {
+      for (int i0 = wave * kWave; i0 < used; i0 += kSelectThreads) {
+        const int i = i0 + lane;
         const unsigned key = i < used ? key_of(i) : 0u;
         const bool mine = i < used && (shift == 24 || key >> (shift + 8) == threshold >> (shift + 8));
         const int bin = key >> shift & 255;
@@ -149,61 +210,92 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
         unsigned four[4], mine = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) mine += four[j] = histogram[255 - (lane * 4 + j)];
-        unsigned upto = mine;
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-          const unsigned other = __shfl_up(upto, d);
-          if (lane >= d) upto += other;
-        }
-        unsigned above = upto - mine;
+        unsigned above = (unsigned)wave_scan((int)mine) - mine;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (above < (unsigned)need && above + four[j] >= (unsigned)need) chosen[0] = 255 - (lane * 4 + j), chosen[1] = need - (int)above;
+          if (above < (unsigned)need && above + four[j] >= (unsigned)need)
+            chosen[0] = 255 - (lane * 4 + j), chosen[1] = need - (int)above, chosen[2] = above + four[j] == (unsigned)need;
           above += four[j];
         }
       }
       __syncthreads();
       threshold |= (unsigned)chosen[0] << shift;
       need = chosen[1];
+      if (chosen[2] && threshold != 0) {   // all that agree so far are wanted: whatever follows (and nothing below)
+        --threshold, need = 0;
+        break;
+      }
     }
   }
 
-  // ---- pages above it, and the first `need` that equal it, in ascending order ----
-  int written = 0, equal = 0;
-  for (int i0 = 0; i0 < used; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    const unsigned key = i < used ? key_of(i) : 0u;
+  // ---- pages above it, and the first `need` that equal it, in ascending order: a wavefront has a stretch of pages ----
+  const int stretch = (used + kSelectThreads - 1) / kSelectThreads * kWave, begin = min(used, wave * stretch), end = min(used, begin + stretch);
+  int above = 0, equal = 0;
+  for (int i0 = begin; i0 < end; i0 += kWave) {
+    const unsigned key = i0 + lane < end ? key_of(i0 + lane) : 0u;
+    above += __popcll(__ballot(key > threshold));
+    equal += __popcll(__ballot(key == threshold && key != 0));
+  }
+  if (lane == 0) totals[0][wave] = above, totals[1][wave] = equal;
+  __syncthreads();
+  int written = 0, equals = 0, all = 0;   // before this wavefront's stretch; all pages that are taken
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int taken = min(totals[1][w], max(0, need - equals));
+    if (w < wave) written += totals[0][w] + taken;
+    all += totals[0][w] + taken;
+    equals += totals[1][w];
+  }
+  equals = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) equals += w < wave ? totals[1][w] : 0;
+  for (int i0 = begin; i0 < end; i0 += kWave) {
+    const unsigned key = i0 + lane < end ? key_of(i0 + lane) : 0u;
     const bool same = key == threshold && key != 0;
     const unsigned long long sames = __ballot(same), below = (1ull << lane) - 1;
-    if (lane == 0) totals[0][wave] = __popcll(sames);
-    __syncthreads();
-    int before = equal;
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) before += totals[0][w];
-      equal += totals[0][w];
-    }
-    const bool take = key > threshold || (same && before + __popcll(sames & below) < need);
+    const bool take = key > threshold || (same && equals + __popcll(sames & below) < need);
     const unsigned long long takes = __ballot(take);
-    if (lane == 0) totals[1][wave] = __popcll(takes);
-    __syncthreads();
-    int to = written;
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) to += totals[1][w];
-      written += totals[1][w];
-    }
-    to += __popcll(takes & below);
-    if (take && to < p.count) out[to] = i;
+    const int to = written + __popcll(takes & below);
+    if (take && to < p.count) out[to] = i0 + lane;
+    written += __popcll(takes), equals += __popcll(sames);
   }
-  for (int i = written + tid; i < p.count; i += kSelectThreads) out[i] = -1;
+  for (int i = all + tid; i < p.count; i += kSelectThreads) out[i] = -1;
+}
+
+// One launch where the scores are few (a row's pages on one CU: 256 9.1 us against 10.3, 512 11.1 against 9.9, 2048 31 against 13) or rows
+// enough for the chip (256 of 1024 28.1 against 31.8, 128 of 1024 21.3 against 20.1).
+bool one_launch(const iex_paged_cache& c) {
+  return c.table_width <= kSelectKept && (c.table_width <= 256 || c.seqs * c.kv_heads >= 256);
+}
+
+template <bool BF16, int D>
+void launch_forms(const SelectParams& p, bool once, hipStream_t s) {
+  const int rows = p.cache.seqs * p.cache.kv_heads, width = p.cache.table_width;
+  if (once) {
+    note_kernel("page_select_kernel<%s, %d>", BF16 ? "bf16" : "f16", D);
+    hipLaunchKernelGGL((page_select_kernel<true, false, BF16, D>), dim3(rows), dim3(kSelectThreads), width * 4, s, p);
+    return;
+  }
+  note_kernel("page_score_kernel<%s, %d>", BF16 ? "bf16" : "f16", D);
+  // a chunk for each of four wavefronts, more where there are workgroups enough (the weights are made once a workgroup)
+  SelectParams scores = p;
+  const long long chunks = (long long)ceil_div(width, 4 * chunk_of(D)) * rows;
+  scores.per_group = 4 * chunk_of(D) * (chunks >= 8 * 512 ? 8 : chunks >= 512 ? (int)(chunks / 512) : 1);
+  hipLaunchKernelGGL((page_score_kernel<BF16, D>), dim3(ceil_div(width, scores.per_group), rows), dim3(256), 0, s, scores);
+  if (width <= kSelectKept) {
+    note_kernel("page_select_kernel<kept>");
+    hipLaunchKernelGGL((page_select_kernel<true, true, true, 64>), dim3(rows), dim3(kSelectThreads), width * 4, s, p);
+  } else {
+    note_kernel("page_select_kernel<read again>");
+    hipLaunchKernelGGL((page_select_kernel<false, true, true, 64>), dim3(rows), dim3(kSelectThreads), 0, s, p);
+  }
 }
 
 template <bool BF16>
-void launch_scores(const SelectParams& p, int head_dim, hipStream_t s) {
-  const dim3 grid(ceil_div(p.cache.table_width, kScorePages), p.cache.seqs * p.cache.kv_heads);
-  note_kernel("page_score_kernel<%s, %d>", BF16 ? "bf16" : "f16", head_dim);
-  if (head_dim == 64) hipLaunchKernelGGL((page_score_kernel<BF16, 64>), grid, dim3(256), 0, s, p);
-  else if (head_dim == 128) hipLaunchKernelGGL((page_score_kernel<BF16, 128>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((page_score_kernel<BF16, 256>), grid, dim3(256), 0, s, p);
+void launch_dim(const SelectParams& p, int head_dim, bool once, hipStream_t s) {
+  if (head_dim == 64) launch_forms<BF16, 64>(p, once, s);
+  else if (head_dim == 128) launch_forms<BF16, 128>(p, once, s);
+  else launch_forms<BF16, 256>(p, once, s);
 }
 
 }  // namespace
@@ -212,7 +304,7 @@ void launch_scores(const SelectParams& p, int head_dim, hipStream_t s) {
 extern "C" size_t iex_select_pages_workspace_bytes(const iex_paged_cache* cache) {
   using namespace iex;
   if (check_paged_cache(cache, "select_pages", false)) return 0;
-  return (size_t)cache->seqs * cache->kv_heads * cache->table_width * 4;
+  return one_launch(*cache) ? 0 : (size_t)cache->seqs * cache->kv_heads * cache->table_width * 4;
 }
 
 extern "C" int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, int count, int first, int last, int* out,
@@ -238,15 +330,7 @@ extern "C" int iex_select_pages(const iex_paged_cache* cache, int heads, const v
   for (int i = 0; i < 3; ++i) p.q_strides[i] = heads ? q_strides[i] : 0;
   p.keys = static_cast<unsigned*>(workspace), p.out = out;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (need) {
-    if (cache->dtype == IEX_BF16) launch_scores<true>(p, cache->head_dim, s);
-    else launch_scores<false>(p, cache->head_dim, s);
-    if (int rc = check_hip(hipGetLastError(), "select_pages score launch")) return rc;
-  }
-  const bool kept = cache->table_width <= kSelectKept;
-  note_kernel("page_select_kernel<%s>", kept ? "kept" : "read again");
-  const dim3 grid(cache->seqs * cache->kv_heads);
-  if (kept) hipLaunchKernelGGL((page_select_kernel<true>), grid, dim3(kSelectThreads), cache->table_width * 4, s, p);
-  else hipLaunchKernelGGL((page_select_kernel<false>), grid, dim3(kSelectThreads), 0, s, p);
+  if (cache->dtype == IEX_BF16) launch_dim<true>(p, cache->head_dim, one_launch(*cache), s);
+  else launch_dim<false>(p, cache->head_dim, one_launch(*cache), s);
   return check_hip(hipGetLastError(), "select_pages launch");
 }

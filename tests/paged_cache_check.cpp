@@ -69,80 +69,47 @@ static int append() {
 }
 
 static int attend() {
-  const int shift = draw(4, 8), page = 1 << shift, seqs = draw(1, 150), width = draw(0, 4) == 0 ? draw(0, 2) : draw(1, 60), pages = draw(0, 50), blocks = draw(1, 5);
-  const int count = draw(0, 1) ? 0 : draw(1, 20), entries = count ? count : width, workgroups = draw(1, 300), least = draw(1, 4);
-  std::vector<int> lengths(seqs), tokens(seqs), first(seqs);
+  const int shift = draw(4, 8), page = 1 << shift, seqs = draw(1, 150), width = draw(0, 4) == 0 ? draw(0, 2) : draw(1, 60), pages = draw(1, 50);
+  const int count = draw(0, 1) ? 0 : draw(1, 20), least = draw(1, 4), entries = count ? count : width;
+  std::vector<int> lengths(seqs), tokens(seqs);
   for (int& l : lengths) l = draw(0, 9) == 0 ? (int)rng() : draw(0, width * page);
+  const int slots = draw(0, 5) == 0 ? 0 : (int)paged_slots(draw(0, 300), seqs, paged_tiles(entries * page), least), grid = seqs + slots;
   int total = 0;
   for (int s = 0; s < seqs; ++s) {
     const int n = cached_length(lengths[s], width, page);
     CHECK(n >= 0 && n <= width * page, "length %d of %d", n, width * page);
     tokens[s] = count && n ? count * page : n;
-    first[s] = total;
     total += paged_tiles(tokens[s]);
   }
-  const long long line = (long long)total * blocks, stretch = paged_stretch(line, workgroups, least);
-  CHECK(stretch * workgroups >= line, "%lld tiles in %d stretches of %lld", line, workgroups, stretch);
-  // what the workgroups leave, by place: (row, tiles from .. to), and the rows that one has whole
-  struct Left { long long row = -1; int from = 0, to = 0; };
-  std::vector<Left> left(2 * workgroups);
-  std::vector<std::vector<int>> met(blocks * seqs);
-  for (int r = 0; r < blocks * seqs; ++r) met[r].assign(tokens[r % seqs] + 1, 0);
-  std::vector<int> whole(blocks * seqs, 0);
-  for (int w = 0; w < workgroups; ++w) {
-    const long long begin = stretch * w, end = std::min(line, begin + stretch);
-    if (begin >= line) break;
-    int block = (int)(begin / total), seq = 0;
-    while (seq + 1 < seqs && first[seq + 1] <= begin - (long long)block * total) ++seq;
-    long long row = (long long)block * total + first[seq], at = begin;
-    for (;;) {
-      CHECK(block < blocks && seq < seqs, "row %d of block %d", seq, block);
-      const int tiles = paged_tiles(tokens[seq]);
-      const PagedPart part = paged_part(row, tiles, at, begin, end, w);
-      CHECK(part.from >= 0 && part.from < part.to && part.to <= tiles && part.place < 2 * workgroups, "tiles %d .. %d of %d", part.from, part.to, tiles);
-      if (part.whole) ++whole[block * seqs + seq];
-      else {
-        CHECK(left[part.place].row < 0, "place %d taken twice", part.place);
-        left[part.place].row = (long long)block * seqs + seq, left[part.place].from = part.from, left[part.place].to = part.to;
-      }
-      // the tokens of the part
-      std::vector<int> table(width), list(count);
-      for (int& p : table) p = draw(0, 5) == 0 ? (int)rng() : pages ? draw(0, pages - 1) : 0;
-      for (int& p : list) p = draw(0, 5) == 0 ? (int)rng() : draw(0, width);
-      const int n = cached_length(lengths[seq], width, page), from = part.from * kPagedTile, to = std::min(tokens[seq], part.to * kPagedTile), waves = draw(0, 1) ? 4 : 8;
+  const int most = paged_part_most(total, slots, least);
+  int items = 0;
+  for (int s = 0; s < seqs; ++s) {
+    const int tiles = paged_tiles(tokens[s]), parts = paged_parts(tiles, most), n = cached_length(lengths[s], width, page);
+    std::vector<int> table(width), list(count), met(tokens[s] + 1, 0);
+    for (int& p : table) p = draw(0, 5) == 0 ? (int)rng() : draw(0, pages - 1);
+    for (int& p : list) p = draw(0, 5) == 0 ? (int)rng() : draw(0, width);
+    CHECK(paged_part_begin(tiles, parts, 0) == 0 && paged_part_begin(tiles, parts, parts) == tiles, "%d parts of %d tiles", parts, tiles);
+    for (int i = 0; i < parts; ++i, ++items) {
+      const int from = paged_part_begin(tiles, parts, i), to = paged_part_begin(tiles, parts, i + 1);
+      CHECK(from < to && to - from <= most, "part of %d tiles, at most %d", to - from, most);
+      const int begin = from * kPagedTile, end = std::min(tokens[s], to * kPagedTile), waves = draw(0, 1) ? 4 : 8;
       for (int wave = 0; wave < waves; ++wave)
-        for (int t = from + wave * 32; t < to; t += waves * 32)
+        for (int t = begin + wave * 32; t < end; t += waves * 32)
           for (int a = 0; a < 2; ++a) {
             const PagedPlace place = paged_place(t + a * 16, shift);
             CHECK(place.slot % 16 == 0 && place.slot + 16 <= page, "slot %d of %d", place.slot, page);
             if (place.entry >= entries) continue;
             const int logical = count ? list[place.entry] : place.entry;
-            const int where = (unsigned)logical < (unsigned)width ? table[logical] : -1;
-            const int valid = paged_valid((unsigned)logical < (unsigned)width ? logical : 0, place.slot, shift, where, pages, n);
-            CHECK(valid >= 0 && valid <= 16 && (valid == 0 || (where >= 0 && where < pages)), "page %d of %d", where, pages);
-            for (int x = 0; x < 16 && t + a * 16 + x < tokens[seq]; ++x) ++met[block * seqs + seq][t + a * 16 + x];
-            if (!count && where >= 0 && where < pages) CHECK(valid == std::max(0, std::min(16, n - (t + a * 16))), "%d attended to", valid);
+            const int at = (unsigned)logical < (unsigned)width ? table[logical] : -1;
+            const int valid = paged_valid((unsigned)logical < (unsigned)width ? logical : 0, place.slot, shift, at, pages, n);
+            CHECK(valid >= 0 && valid <= 16 && (valid == 0 || (at >= 0 && at < pages)), "page %d of %d", at, pages);
+            for (int x = 0; x < 16 && t + a * 16 + x < tokens[s]; ++x) ++met[t + a * 16 + x];
+            if (!count && at >= 0 && at < pages) CHECK(valid == std::max(0, std::min(16, n - (t + a * 16))), "%d attended to", valid);
           }
-      at = row + part.to;
-      if (at >= end) break;
-      row = at;
-      if (++seq == seqs) seq = 0, ++block;
     }
+    for (int t = 0; t < tokens[s]; ++t) CHECK(met[t] == 1, "sequence %d token %d met %d times", s, t, met[t]);
   }
-  for (int r = 0; r < blocks * seqs; ++r) {
-    for (int t = 0; t < tokens[r % seqs]; ++t) CHECK(met[r][t] == 1, "row %d token %d met %d times", r, t, met[r][t]);
-    const int tiles = paged_tiles(tokens[r % seqs]);
-    const PagedParts parts = paged_parts((long long)(r / seqs) * total + first[r % seqs], tiles, stretch);
-    if (parts.first == parts.last) { CHECK(whole[r] == 1, "row %d whole %d times", r, whole[r]); continue; }
-    CHECK(whole[r] == 0, "row %d in parts is whole somewhere", r);
-    int next = 0;
-    for (int w = parts.first; w <= parts.last; ++w) {
-      const Left& l = left[w * 2 + (w == parts.first && parts.second ? 1 : 0)];
-      CHECK(l.row == r && l.from == next, "row %d: workgroup %d left row %lld from tile %d, not %d", r, w, l.row, l.from, next);
-      next = l.to;
-    }
-    CHECK(next == tiles, "row %d joined to tile %d of %d", r, next, tiles);
-  }
+  CHECK(items <= grid, "%d parts in %d workgroups", items, grid);
   return 0;
 }
 
