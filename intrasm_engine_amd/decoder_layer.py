@@ -7,7 +7,8 @@ probabilities in registers (heads of 64 or 128; else heads are split off and sco
 context are batched MFMA GEMMs around PyTorch's softmax).  Included element-wise steps,
 done by the epilogues of the products before them: SiLU(gate) * up and the two residual
 additions.  Not included (the configuration
-names none of them): RoPE, normalisation layers, causal masking, KV cache.
+names none of them): normalisation layers, causal masking; position rotation and a cache of keys and values are what generation
+adds (``prompt`` and ``decode`` below), the configuration's passes have none.
 
 Three ways to run the same arithmetic, mirroring how the reference's harness compares
 "serialized" with "interleaved" (tests/test_interleaving.py:348-369, 434-476):
@@ -31,6 +32,7 @@ from . import interleaving as IL
 from . import _iex_host, _lib
 from .pytorch import ops as _pyops
 from .pytorch.cpp_extensions.cuda_graph_constructor import TorchCUDAGraphConstructor
+from .pytorch.paged_attention import KVCache
 
 ops = torch.ops.iex_ops
 
@@ -166,6 +168,30 @@ class SparseDecoderLayer:
         """x: (hidden, seqs*L) fp16, contiguous -> same shape."""
         q, k, v = self.proj("q", x), self.proj("k", x), self.proj("v", x)
         h = self._proj_with("o", self.attention(q, k, v, seqs), x, 1)
+        return self.mlp_block(h)
+
+    # ---- generation: a token of every sequence at a time over a paged cache --------------------
+    def new_cache(self, pages: int, page_size: int = 64, eight_bits: bool = False, bounds: bool = False) -> KVCache:
+        """A cache for this layer's keys and values (heads of 64, 128 or 256)."""
+        return KVCache(pages, page_size, self.heads, self.head_dim, torch.float16, self.device, eight_bits, bounds)
+
+    def _tokens(self, t: torch.Tensor) -> torch.Tensor:
+        """(hidden, tokens) as (tokens, heads, head_dim), where it lies."""
+        return t.view(self.heads, self.head_dim, t.shape[1]).permute(2, 0, 1)
+
+    def prompt(self, x: torch.Tensor, cache: KVCache, page_table, lengths, offsets, rotation=None) -> None:
+        """Keys and values of prompts into the cache: columns ``offsets[s] .. offsets[s + 1]`` of x (hidden, tokens) are sequence s's
+        newest, ``lengths`` counts them."""
+        cache.append_(self._tokens(self.proj("k", x)), self._tokens(self.proj("v", x)), page_table, lengths, offsets, None, rotation)
+
+    def decode(self, x: torch.Tensor, cache: KVCache, page_table, lengths, rotation=None, pages: int = 0) -> torch.Tensor:
+        """One new token of every sequence: x (hidden, sequences) fp16 -> same shape.  Its key and value go into the cache (``lengths``
+        counts it) and it attends to all of its sequence, or to the ``pages`` pages that its query can score highest with (a cache
+        with bounds).  Capturable: a graph follows ``page_table`` and ``lengths``."""
+        q = cache.append_(self._tokens(self.proj("k", x)), self._tokens(self.proj("v", x)), page_table, lengths, None, self._tokens(self.proj("q", x)), rotation)
+        selected = cache.select(q, page_table, lengths, pages) if pages else None
+        attended = cache.attend(q, page_table, lengths, None, selected)
+        h = self._proj_with("o", attended.permute(1, 2, 0).reshape(self.hidden, x.shape[1]), x, 1)
         return self.mlp_block(h)
 
     # ---- fused schedule over two half-batches ----------------------------------------------

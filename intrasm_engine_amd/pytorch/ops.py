@@ -21,6 +21,7 @@ Registered operators
     csr_softmax_                     in-place softmax over CSR rows         [new]
     gemm_mfma                        bf16/fp16 dense companion GEMM         [replaces torch.matmul / CUTLASS / Triton companions]
     fused_spmm_gemm                  single-launch sparse + dense           [new]
+    kv_append_, paged_attention, select_pages   generation over a paged cache (csrc/host/paged_ops.h, pytorch/paged_attention.py) [new]
 """
 from __future__ import annotations
 

@@ -83,8 +83,7 @@ def test_pages_that_are_refused(call, other, code, text):
     (attend, dict(count=3), -1, "null"), (attend, dict(listed=A), -1, "must have entries"), (attend, dict(listed=A, count=-1), -1, "must have entries"),
     (attend, dict(listed=A, count=1 << 25), -3, "2^30"), (attend, dict(q=A + 1), -2, "aligned"),
     (select, dict(heads=3), -1, "multiple of key heads"), (select, dict(count=0), -1, "at least one page"), (select, dict(count=3, first=2, last=2), -1, "among them"),
-    (select, dict(first=-1), -1, "at least one page"), (select, dict(q=None), -1, "null"), (select, dict(out=None), -1, "null"), (select, dict(ws=None), -1, "workspace"),
-    (select, dict(ws=A + 16), -1, "workspace"), (select, dict(ws_bytes=4), -1, "workspace"),
+    (select, dict(first=-1), -1, "at least one page"), (select, dict(q=None), -1, "null"), (select, dict(out=None), -1, "null"),
 ])
 def test_arguments_that_are_refused(call, arguments, code, text):
     assert call(cache(bounds=A), **arguments) == code and text in _lib.last_error()
@@ -97,6 +96,10 @@ def test_workspaces_and_null_caches():
     assert need > 0 and attend(long, ws=None) == -1 and "workspace" in _lib.last_error()
     assert attend(long, ws_bytes=need - 1) == -1 and attend(long, ws=A + 64) == -1
     assert lib.iex_paged_attention_workspace_bytes(ctypes.byref(cache(table_width=1)), 4, 0) == 0
+    many = cache(bounds=A, table_width=1 << 12, seqs=1, table_stride=1 << 12)
+    assert lib.iex_select_pages_workspace_bytes(ctypes.byref(many)) == 2 * 4096 * 4 and lib.iex_select_pages_workspace_bytes(ctypes.byref(cache(bounds=A))) == 0
+    for given in (dict(ws=None), dict(ws=A + 16), dict(ws_bytes=4)):
+        assert select(many, **given) == -1 and "workspace" in _lib.last_error()
     assert select(cache()) == -1 and "null" in _lib.last_error()
     for call in (append, attend, select):
         assert call(None) == -1 and "null" in _lib.last_error()
