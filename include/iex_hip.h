@@ -446,7 +446,7 @@ int iex_sparse_attention(int dtype, int heads, int tokens, int head_dim, int non
 /* ---- a paged cache of keys and values, and single new tokens attending to it (no counterpart in the reference) ----
  * keys, values: (pages, kv_heads, page_size, head_dim), a page's elements contiguous, pages `*_page_stride` elements apart; of
  * type `dtype`, or (eight_bits) e4m3 codes whose rows have an exponent each: (pages, kv_heads, page_size), value = code *
- * 2^(exponent - 127).  table: the pages of every sequence, (seqs, table_width) with rows table_stride apart; lengths: tokens of
+ * 2^(exponent - 127), exponents 1 .. 254.  table: the pages of every sequence, (seqs, table_width) with rows table_stride apart; lengths: tokens of
  * every sequence (int32).  bounds (may be null): smallest and largest stored key per page, head and feature, (pages, kv_heads, 2,
  * head_dim) of type `dtype`.  Tables and lengths are read on the device at every call (a replayed graph follows them); a length
  * is cut to what the table holds, a page outside the cache counts as given back: nothing is written to it and nothing of it is
@@ -473,7 +473,8 @@ typedef struct iex_paged_cache {
  * can hold; the first `rotary` features (a multiple of 16, 0: none) turn in pairs (j, j + rotary / 2), or (2j, 2j + 1) where
  * interleaved.  A sequence longer than its table or shorter than its new tokens is passed over, tokens behind the last
  * sequence's too: nothing is written to the cache, their rows of q_out are zeros.  Two sequences that append to the same page
- * in one call leave one of the two in it.  In an 8-bit cache infinities become NaN. */
+ * in one call leave one of the two in it.  In an 8-bit cache infinities become NaN.  Bounds begin anew with a page's first token:
+ * tokens that are taken back (a shorter length) and written again widen them at most. */
 int iex_kv_append(const iex_paged_cache* cache, int tokens, const int* offsets, int heads, const void* k, const long long* k_strides,
                   const void* v, const long long* v_strides, const void* q, const long long* q_strides, void* q_out,
                   const long long* q_out_strides, const float* rotation, int positions, int rotary, int interleaved, void* stream);

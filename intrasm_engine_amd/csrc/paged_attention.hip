@@ -2,6 +2,8 @@
 #include "paged_attention_device.cuh"
 #include "paged_cache_host.h"
 
+#include <climits>
+
 namespace iex {
 namespace {
 
@@ -20,7 +22,7 @@ constexpr int kTwoRounds = 256;
 
 struct Split {
   long long blocks, slots, workgroups;   // blocks of up to 16 heads of a key head; parts beyond one per sequence; workgroups of the launch
-  int pitch;
+  int fixed, pitch;                      // parts of every row (0: by the lengths)
   bool wide;
 };
 Split split_of(const iex_paged_cache& c, int heads, int count) {
@@ -32,7 +34,12 @@ Split split_of(const iex_paged_cache& c, int heads, int count) {
   const bool whole = most <= kWholeTiles;
   s.wide = whole && rows < kWideRows;
   s.slots = whole ? 0 : paged_slots(resident(c.head_dim, c.eight_bits) * (rows < kTwoRounds ? 1 : 2) / s.blocks, c.seqs, most, kPagedLeast);
-  s.workgroups = s.blocks * (c.seqs + s.slots);
+  s.fixed = whole ? 1 : 0;
+  if (count && !whole) {   // (every row is as long)
+    const long long total = (long long)c.seqs * most;
+    s.fixed = paged_parts(most, paged_part_most(total < INT_MAX ? (int)total : INT_MAX, (int)s.slots, kPagedLeast));
+  }
+  s.workgroups = s.blocks * (s.fixed ? (long long)c.seqs * s.fixed : c.seqs + s.slots);
   return s;
 }
 // (per part: rows x head_dim sums, then rows pairs)
@@ -43,18 +50,20 @@ int launch(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
   const int lds = WAVES * s.pitch * (D + 2) * 4;
   auto kern = paged_attention_kernel<BF16, D, E8, WAVES>;
   if (lds > 64 * 1024) {
-    static thread_local bool raised = false;   // per instantiation
-    if (!raised) {
+    static thread_local unsigned long long raised = 0;   // per instantiation: on which devices
+    int device = 0;
+    if (int rc = check_hip(hipGetDevice(&device), "hipGetDevice")) return rc;
+    if (!(raised >> (device & 63) & 1)) {
       if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, WAVES * 16 * (D + 2) * 4),
                              "hipFuncSetAttribute(LDS size)"))
         return rc;
-      raised = true;
+      raised |= 1ull << (device & 63);
     }
   }
   note_kernel("paged_attention_kernel<%s, %d, %s, %d>", BF16 ? "bf16" : "f16", D, E8 ? "e4m3" : "16", WAVES);
   hipLaunchKernelGGL(kern, dim3((unsigned)s.workgroups), dim3(WAVES * kWave), lds, stream, p);
   if (int rc = check_hip(hipGetLastError(), "paged attention launch")) return rc;
-  if (s.slots == 0) return 0;
+  if (s.fixed == 1) return 0;
   note_kernel("paged_join_kernel<%s, %d>", BF16 ? "bf16" : "f16", D);
   hipLaunchKernelGGL((paged_join_kernel<BF16, D>), dim3((unsigned)p.cache.seqs, (unsigned)p.heads), dim3(256), 0, stream, p);
   return check_hip(hipGetLastError(), "paged attention join launch");
@@ -87,7 +96,7 @@ extern "C" size_t iex_paged_attention_workspace_bytes(const iex_paged_cache* cac
   using namespace iex;
   if (check_paged_cache(cache, "paged_attention", false) || check_heads(cache, heads, "paged_attention") || heads == 0 || cache->seqs == 0 || count < 0) return 0;
   const Split s = split_of(*cache, heads, count);
-  if (s.slots == 0) return 0;
+  if (s.fixed == 1) return 0;
   return partial_floats(*cache, s) * 4 + (size_t)s.workgroups * s.pitch * 8;
 }
 
@@ -114,7 +123,7 @@ extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, cons
   PagedAttentionParams p{};
   p.cache = paged_params(*cache);
   p.heads = heads, p.group = heads / cache->kv_heads, p.group_tiles = ceil_div(p.group, 16), p.pitch = s.pitch;
-  p.count = count, p.listed = listed, p.blocks = (int)s.blocks, p.slots = (int)s.slots;
+  p.count = count, p.listed = listed, p.blocks = (int)s.blocks, p.slots = (int)s.slots, p.fixed = s.fixed;
   p.q = static_cast<const unsigned short*>(q), p.out = static_cast<unsigned short*>(out);
   for (int i = 0; i < 3; ++i) p.q_strides[i] = q_strides[i], p.out_strides[i] = out_strides[i];
   p.q_rows = rows_of_chunks(q, q_strides);

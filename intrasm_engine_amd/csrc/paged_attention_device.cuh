@@ -2,7 +2,7 @@
 // head; the query heads of a group share a key head.
 //
 // Every key and value is read once and multiplied with at most 16 queries: memory is what bounds it, so the design keeps loads in
-// flight and everything else out of their way.  Tiles of 32 tokens go from the pages straight into registers as matrix-core
+// flight and everything else out of their way.  Tiles of 32 or 64 tokens go from the pages straight into registers as matrix-core
 // operands, no LDS:
 //   S^T = K Q^T    MFMA rows = tokens, columns = queries: a lane's operand is 16 bytes of one token's key.  Lane (column c, group
 //                  g = lane / 16) gets the scores of query c with tokens 4g .. 4g + 3 of each 16 ...
@@ -25,7 +25,8 @@ struct PagedAttentionParams {
   PagedParams cache;
   int heads, group, group_tiles;   // query heads, those of a key head, blocks of 16 of them
   int pitch, count;                // query rows of a part's result; pages listed per sequence and key head, 0: all of the table
-  int blocks, slots;               // blocks of up to 16 query heads of a key head; parts beyond one per sequence (0: rows are whole)
+  int blocks, slots;               // blocks of up to 16 query heads of a key head; parts beyond one per sequence
+  int fixed;                       // parts of every row, where that does not go by the lengths (whole rows, listed pages); else 0
   const int* listed;
   const unsigned short* q;
   unsigned short* out;
@@ -51,11 +52,7 @@ struct LaneLengths {
     return bcast_i(mine, seq - from);
   }
 };
-// Tokens that a sequence of this length is work for: itself, or as many pages as are listed.
-__device__ __forceinline__ int row_tokens(const PagedAttentionParams& p, int length) { return p.count && length ? p.count << p.cache.page_shift : length; }
-__device__ __forceinline__ int lane_tiles(const PagedAttentionParams& p, const LaneLengths& l) {
-  return l.from + lane_id() < p.cache.seqs ? paged_tiles(row_tokens(p, l.mine)) : 0;
-}
+__device__ __forceinline__ int lane_tiles(const PagedAttentionParams& p, const LaneLengths& l) { return l.from + lane_id() < p.cache.seqs ? paged_tiles(l.mine) : 0; }
 
 // The first sequence that `match` says yes to (its number, its first part's, its parts), by the lengths; `lengths` holds its.
 template <typename MATCH>
@@ -95,6 +92,8 @@ __device__ __forceinline__ T load_from(const T* p) {
   else return *p;
 }
 
+// Places of 16 tokens of a wavefront's tile.  (Heads of 64 in 16 bits by four: 512 x 16 rows of 128 tokens 54.5 -> 63.7 us.)
+constexpr int paged_places(int head_dim, bool eight_bits) { return eight_bits && head_dim <= 128 ? 4 : 2; }
 // Wavefronts of a SIMD that the registers are cut for.
 constexpr int paged_simd_waves(int head_dim, bool eight_bits) { return head_dim == 256 ? (eight_bits ? 2 : 1) : head_dim == 128 ? 3 : 4; }
 
@@ -107,6 +106,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   constexpr int F = D / 16;                    // features of a value row that a lane has: operands of the second product
   constexpr int VD = F * ES / 4, VWORDS = VD == 8 ? 2 : 1;   // ... in dwords: 1, 2, 4 or 8
   typedef std::conditional_t<VD == 1, unsigned, std::conditional_t<VD == 2, u32x2, u32x4>> VWord;
+  constexpr int SUB = paged_places(D, E8);     // places of 16 tokens of a tile
   constexpr bool PV_BF16 = BF16 || E8;         // (an e4m3 value's power of two goes to the probability, which fp16 has not the range for)
   extern __shared__ __align__(16) float smem[];
   const int wave = uniform(threadIdx.x >> 6);
@@ -116,19 +116,32 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   // ---- whose part ----
   const int block = blockIdx.x % p.blocks, item = blockIdx.x / p.blocks;
   int seq = item, part = 0, parts = 1, tiles = 1;
-  if (p.slots == 0) {
+  const int lane = threadIdx.x & 63, entries = p.count ? p.count : cache.table_width;
+  const int kv_head = block / p.group_tiles, group_tile = block % p.group_tiles;
+  auto entry_at = [&](int e) -> int {   // of the sequence's list, or of its table
+    if (e >= entries) return -1;
+    return p.count ? p.listed[((size_t)seq * cache.kv_heads + kv_head) * p.count + e] : cache.table[(size_t)seq * cache.table_row + e];
+  };
+  int first_entry = 0, first_found = -1;
+  if (p.fixed) {
+    parts = p.fixed, seq = item / parts, part = item % parts;
+    if (p.count) {
+      tiles = paged_tiles(p.count << cache.page_shift);
+      first_entry = paged_place(paged_part_begin(tiles, parts, part) * kPagedTile, cache.page_shift).entry;
+    }
+    first_found = entry_at(first_entry + lane);   // (beside the lengths, which it does not need)
     lengths.load(cache, seq);
-    tiles = paged_tiles(row_tokens(p, lengths.of(cache, seq)));
+    if (!p.count) tiles = paged_tiles(lengths.of(cache, seq));
   } else if (!find_part(p, lengths, [&](int, int first, int n) { return first + n > item; }, seq, part, parts, tiles)) {
     return;
   } else {
     part = item - part;
   }
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int kv_head = block / p.group_tiles, group_tile = block % p.group_tiles;
+  const int col = lane & 15, g = lane >> 4;
   const int rows = min(16, p.group - group_tile * 16);   // queries
-  const int length = lengths.of(cache, seq), tokens = row_tokens(p, length);
-  const int begin = paged_part_begin(tiles, parts, part) * kPagedTile, end = min(tokens, paged_part_begin(tiles, parts, part + 1) * kPagedTile);
+  const int length = lengths.of(cache, seq), tokens = p.count && length ? p.count << cache.page_shift : length;
+  const int begin = paged_part_begin(tiles, parts, part) * kPagedTile;
+  int end = min(tokens, paged_part_begin(tiles, parts, part + 1) * kPagedTile);
 
   // ---- queries: columns of the first product ----
   u32x4 fq[KS];
@@ -152,45 +165,46 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   }
 
   // ---- the pages of the part: 64 entries of the table (or list) in the lanes ----
-  const int* table = cache.table + (size_t)seq * cache.table_row;
-  const int* listed = p.count ? p.listed + ((size_t)seq * cache.kv_heads + kv_head) * p.count : nullptr;
-  const int entries = p.count ? p.count : cache.table_width;
   int window = -(1 << 30), entry_logical = 0, entry_page = -1;
-  auto look_up = [&](int entry) {
-    window = entry;
-    const int e = entry + lane;
-    entry_page = -1, entry_logical = 0;
-    if (e < entries) {
-      entry_logical = listed ? listed[e] : e;
-      if ((unsigned)entry_logical < (unsigned)cache.table_width) entry_page = table[entry_logical];
+  auto take_entries = [&](int from, int found) {
+    window = from, entry_logical = from + lane, entry_page = found;
+    if (p.count) {
+      entry_logical = found, entry_page = -1;
+      if ((unsigned)found < (unsigned)cache.table_width) entry_page = cache.table[(size_t)seq * cache.table_row + found];
       else entry_logical = 0;
     }
   };
+  if (p.fixed) take_entries(first_entry, first_found);
+  if (p.count && paged_place(end - 1, cache.page_shift).entry < window + kWave) {   // nothing behind the last page that is there (a sequence of fewer pages)
+    const unsigned long long there = __ballot((unsigned)entry_page < (unsigned)cache.pages);
+    end = min(end, (window + (there ? 64 - __builtin_clzll(there) : 0)) << cache.page_shift);
+  }
 
-  // Where 32 tokens lie: two places of 16.  Loads take no branch: what is not attended to is read from a place that exists and
+  // Where a tile's tokens lie, 16 at a place.  Loads take no branch: what is not attended to is read from a place that exists and
   // masked where it is used.
   struct Where {
-    int page[2], row[2], valid[2];
+    int page[SUB], row[SUB], valid[SUB];
   };
   auto find = [&](int t) {
     Where w;
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < SUB; ++a) {
       const PagedPlace place = paged_place(t + a * 16, cache.page_shift);
-      if (place.entry >= window + kWave) look_up(place.entry);
+      if (place.entry >= window + kWave) take_entries(place.entry, entry_at(place.entry + lane));
       const int page = bcast_i(entry_page, place.entry - window), logical = bcast_i(entry_logical, place.entry - window);
       w.valid[a] = place.entry < entries ? paged_valid(logical, place.slot, cache.page_shift, page, cache.pages, length) : 0;
       w.page[a] = page, w.row[a] = (kv_head << cache.page_shift) + place.slot;
-      if (w.valid[a] == 0) w.page[a] = a ? w.page[0] : 0, w.row[a] = a ? w.row[0] : w.row[a];
+      if (w.valid[a] == 0) w.page[a] = a ? w.page[a ? a - 1 : 0] : 0, w.row[a] = a ? w.row[a ? a - 1 : 0] : w.row[a];
     }
     return w;
   };
-  u32x4 key[2][KW];
-  VWord value[2][4][VWORDS];
-  unsigned ke[2], ve[2];   // exponents of this lane's four tokens
+  u32x4 key[SUB][KW];
+  VWord value[SUB][4][VWORDS];
+  typedef unsigned Places __attribute__((ext_vector_type(SUB)));
+  Places ke, ve;   // exponents of this lane's four tokens at each place
   auto load_keys = [&](const Where& w) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < SUB; ++a) {
       const unsigned char* k = static_cast<const unsigned char*>(cache.keys) + (w.page[a] * cache.key_page + (long long)w.row[a] * D) * ES;
 #pragma unroll
       for (int s = 0; s < KW; ++s) key[a][s] = load_from<WAVES == 4>(reinterpret_cast<const u32x4*>(k + (col * (D * ES) + s * 64 + g * 16)));
@@ -200,7 +214,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   };
   auto load_values = [&](const Where& w) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < SUB; ++a) {
       const unsigned char* v = static_cast<const unsigned char*>(cache.values) + (w.page[a] * cache.value_page + (long long)w.row[a] * D) * ES;
       // (heads of 256 in 16 bits: two halves of 128, so that a load of 16 lanes is 256 consecutive bytes)
 #pragma unroll
@@ -222,14 +236,14 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   float top = -INFINITY, sum = 0.f;   // of this lane's query: the maximum so far (all groups'), this group's share of the sum
   int attended = 0;
 
-  f32x4 s[2];
+  f32x4 s[SUB];
   auto scores = [&]() {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int a = 0; a < SUB; ++a) s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < KS; ++e)
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
+      for (int a = 0; a < SUB; ++a) {
         u32x4 fk;
         if constexpr (E8) {
           const unsigned c0 = key[a][e / 2][e % 2 * 2], c1 = key[a][e / 2][e % 2 * 2 + 1];
@@ -241,17 +255,20 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
       }
     if constexpr (E8) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < SUB; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[a][r] *= power_of_two(ke[a] >> (r * 8) & 0xFFu);
     }
   };
-  u32x4 hi, lo;
+  u32x4 hi[SUB / 2], lo[SUB / 2];
   auto weights = [&](const Where& w) {
-    attended += w.valid[0] + w.valid[1];
-    if (w.valid[0] + w.valid[1] != 32) {   // (uniform) tokens that are not attended to leave no trace, infinities and NaN included
+    int valid = 0;
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < SUB; ++a) valid += w.valid[a];
+    attended += valid;
+    if (valid != SUB * 16) {   // (uniform) tokens that are not attended to leave no trace, infinities and NaN included
+#pragma unroll
+      for (int a = 0; a < SUB; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (g * 4 + r >= w.valid[a]) {
@@ -263,7 +280,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
     }
     float m = s[0][0];
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < SUB; ++a)
 #pragma unroll
       for (int r = 0; r < 4; ++r) m = fmaxf(m, s[a][r]);
     if (__ballot(m > top)) {
@@ -281,7 +298,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
     }
     const float shift = top == -INFINITY ? 0.f : -top * p.scale_log2;
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < SUB; ++a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         s[a][r] = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.scale_log2, shift));   // (exp2(-infinity) = 0)
@@ -290,38 +307,40 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        hi[a * 2 + r] = pack_pair<PV_BF16>(s[a][2 * r], s[a][2 * r + 1]);
+        hi[a / 2][a % 2 * 2 + r] = pack_pair<PV_BF16>(s[a][2 * r], s[a][2 * r + 1]);
         float h0, h1;
-        unpack_pair<PV_BF16>(hi[a * 2 + r], h0, h1);
-        lo[a * 2 + r] = pack_pair<PV_BF16>(s[a][2 * r] - h0, s[a][2 * r + 1] - h1);
+        unpack_pair<PV_BF16>(hi[a / 2][a % 2 * 2 + r], h0, h1);
+        lo[a / 2][a % 2 * 2 + r] = pack_pair<PV_BF16>(s[a][2 * r] - h0, s[a][2 * r + 1] - h1);
       }
     }
   };
   auto weigh_values = [&]() {
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
-      u32x4 fv;
+    for (int j = 0; j < F; ++j)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int a = w / 2, r = w % 2 * 2;   // tokens r and r + 1 of the four in subtile a
-        if constexpr (E8) {
-          // byte j of both rows side by side, then widened
-          const unsigned pair = __builtin_amdgcn_perm(value_dword(a, r + 1, j / 4), value_dword(a, r, j / 4), (j % 4) | (4 + j % 4) << 8);
-          fv[w] = widen_pair<PV_BF16, false>(pair);
-        } else {
-          fv[w] = __builtin_amdgcn_perm(value_dword(a, r + 1, j / 2), value_dword(a, r, j / 2), j % 2 ? 0x07060302u : 0x05040100u);
+      for (int two = 0; two < SUB / 2; ++two) {
+        u32x4 fv;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int a = two * 2 + w / 2, r = w % 2 * 2;   // tokens r and r + 1 of the four at place a
+          if constexpr (E8) {
+            // byte j of both rows side by side, then widened
+            const unsigned pair = __builtin_amdgcn_perm(value_dword(a, r + 1, j / 4), value_dword(a, r, j / 4), (j % 4) | (4 + j % 4) << 8);
+            fv[w] = widen_pair<PV_BF16, false>(pair);
+          } else {
+            fv[w] = __builtin_amdgcn_perm(value_dword(a, r + 1, j / 2), value_dword(a, r, j / 2), j % 2 ? 0x07060302u : 0x05040100u);
+          }
         }
+        o[j] = mfma_16x16x32<PV_BF16>(fv, hi[two], o[j]);
+        o[j] = mfma_16x16x32<PV_BF16>(fv, lo[two], o[j]);
       }
-      o[j] = mfma_16x16x32<PV_BF16>(fv, hi, o[j]);
-      o[j] = mfma_16x16x32<PV_BF16>(fv, lo, o[j]);
-    }
   };
 
   // ---- the part's tiles, a wavefront's in turn.  A tile's values are asked for before its keys are waited for, the next tile's
   // keys as soon as this one's have been multiplied: half a tile is in flight at any time, in one set of registers.  (The last
   // tile is written out behind the loop, so that a wait knows on every path how many loads are behind the ones it is for.)
-  int t = begin + wave * 32;
-  constexpr int STEP = WAVES * 32;
+  int t = begin + wave * (SUB * 16);
+  constexpr int STEP = WAVES * SUB * 16;
   if (t < end && cache.pages > 0) {
     Where now = find(t);
     load_keys(now);
@@ -396,16 +415,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p)
   const int seq = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
   const int kv_head = head / p.group, in_group = head % p.group;
   LaneLengths lengths;
-  int found, first, number, tiles;
-  if (!find_part(p, lengths, [&](int s, int, int) { return s == seq; }, found, first, number, tiles) || number == 1) return;
+  int found, first = seq * p.fixed, number = p.fixed, tiles;
+  if (!p.fixed && (!find_part(p, lengths, [&](int s, int, int) { return s == seq; }, found, first, number, tiles) || number == 1)) return;
   const int block = kv_head * p.group_tiles + in_group / 16;
   auto place = [&](int i) { return ((size_t)(first + i) * p.blocks + block) * p.pitch + in_group % 16; };
   const int lane = tid % LANES, side = tid / LANES;
   float4 acc = {0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, total = 0.f;
   bool any = false;
+  constexpr int AHEAD = 4;
   for (int i0 = 0; i0 < number; i0 += 256) {
-    const int i = i0 + tid;
+    const int i = i0 + tid, n = min(256, number - i0);
+    float4 ahead[AHEAD];   // the first parts' sums, beside the weights
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (side + k * SIDE < n) ahead[k] = *reinterpret_cast<const float4*>(p.partial + place(i0 + side + k * SIDE) * D + lane * 4);
     float m = -INFINITY, part = -1.f;
     if (i < number) {
       const float2 both = *reinterpret_cast<const float2*>(p.stats + place(i) * 2);
@@ -425,9 +449,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p)
     total = total * keep + (sums[0] + sums[1] + sums[2] + sums[3]);
     acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
     top = now;
-    const int n = min(256, number - i0);
+    // (a part without a token left zeros)
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (side + k * SIDE < n) {
+        const float w = weights[side + k * SIDE];
+        acc.x = fmaf(w, ahead[k].x, acc.x), acc.y = fmaf(w, ahead[k].y, acc.y), acc.z = fmaf(w, ahead[k].z, acc.z), acc.w = fmaf(w, ahead[k].w, acc.w);
+      }
 #pragma unroll 4
-    for (int j = side; j < n; j += SIDE) {   // (a part without a token left zeros)
+    for (int j = side + AHEAD * SIDE; j < n; j += SIDE) {
       const float w = weights[j];
       const float4 x = *reinterpret_cast<const float4*>(p.partial + place(i0 + j) * D + lane * 4);
       acc.x = fmaf(w, x.x, acc.x), acc.y = fmaf(w, x.y, acc.y), acc.z = fmaf(w, x.z, acc.z), acc.w = fmaf(w, x.w, acc.w);

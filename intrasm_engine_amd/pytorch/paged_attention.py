@@ -35,7 +35,8 @@ class KVCache:
 
     ``eight_bits``: e4m3 codes and, per token and head, the least power of two as their scale that brings the largest magnitude to
     448 (one byte), in place of ``dtype``: half the memory, and half the time of reading it.  ``bounds``: also keep the smallest and
-    largest key of every page, head and feature, which :meth:`select` reads.  Who has which page is the caller's business: two
+    largest key of every page, head and feature, which :meth:`select` reads (they begin anew with a page's first token; tokens that are
+    taken back, by a shorter length, and written again widen them at most).  Who has which page is the caller's business: two
     sequences may share pages that neither appends to (a common prefix)."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.float16, device="cuda", eight_bits: bool = False,

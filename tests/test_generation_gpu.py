@@ -285,6 +285,20 @@ def test_caches_beyond_32_bit_offsets(dev, ops):
         torch.cuda.empty_cache()
 
 
+def test_what_an_eight_bit_cache_holds_of_infinities(dev, ops):
+    """NaN codes come out as NaN where they are attended to and leave no trace where they are not."""
+    c = Cache(dev, [20, 20, 20], 1, 64, 16, F16, e8=True)
+    c.keys.view(torch.uint8)[c.table[0, 1], 0, 2, 5] = 0x7F
+    c.values.view(torch.uint8)[c.table[1, 1], 0, 3, 7] = 0xFF
+    q = torch.randn(3, 2, 64, device=dev).half()
+    out = ops.paged_attention(q, c.keys, c.values, c.table, c.lengths, None, None, *c.exponents())
+    assert out[0].isnan().all() and out[1, :, 7].isnan().all() and out[1].isnan().sum() == 2
+    first = torch.zeros(3, 1, 1, dtype=torch.int32, device=dev)
+    out = ops.paged_attention(q, c.keys, c.values, c.table, c.lengths, None, first, *c.exponents())
+    want, allowed = c.attend(q, 1 / 8, first)
+    assert ((out.double() - want).abs() <= allowed).all()
+
+
 def test_changes_are_counted(dev, ops):
     c = Cache(dev, [5], 1, 64, 16, F16, bounds=True)
     k = torch.randn(1, 1, 64, device=dev).half()
@@ -372,5 +386,8 @@ def test_empty_caches_and_no_sequences(dev, ops):
     assert (ops.select_pages(q, c.bounds, c.table[:, :0], c.lengths, 16, 2) == -1).all()
     assert ops.paged_attention(q[:0], c.keys, c.values, c.table[:0], c.lengths[:0]).shape == (0, 4, 64)
     assert ops.select_pages(q[:0], c.bounds, c.table[:0], c.lengths[:0], 16, 2).shape == (0, 2, 2)
+    nobody = torch.zeros(1, dtype=torch.int32, device=dev)      # tokens behind the last of no sequences
+    rest = ops.kv_append_(q[:, :2], q[:, :2], c.keys, c.values, c.table[:0], c.lengths[:0], nobody, q)
+    assert (rest == 0).all()
     alike = feature_major(q)
     assert torch.equal(ops.paged_attention(alike, c.keys, c.values, c.table, c.lengths), ops.paged_attention(q, c.keys, c.values, c.table, c.lengths))
