@@ -10,8 +10,7 @@
 //                  if group g's share of the sum over tokens is those very tokens.  A lane loads 16 bytes (features c * 8 ..) of
 //                  each of them; one byte permute per dword pairs tokens, and operand j has features c * 8 + j as its rows.
 // The running maximum and sum are per query; sums follow a new maximum only where some score has passed it.  Probabilities go
-// in as two 16-bit parts, p = hi + lo (bf16), so that they keep 16 bits: matrix cores idle otherwise, and one part rounded costs
-// about half again the error of the rounded result.
+// in as two 16-bit parts: matrix cores idle otherwise, and one part rounded costs about half again the error of the rounded result.
 //
 // A sequence is split over its length into parts, a workgroup each (paged_cache.h: parts are cut from the lengths on the device,
 // so a replayed graph follows them); four wavefronts take a part's tiles in turn and meet in LDS, parts meet in a second launch.
@@ -85,6 +84,31 @@ __device__ __forceinline__ unsigned widen_pair(unsigned codes) {
   else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, HIGH));
 }
 
+// Two weights as pairs of 16-bit parts, p = hi + lo.  bf16: 16 bits of p, 2^-16 of it at most are lost; fp16: 21.  Where values can be
+// infinite (16-bit caches) both parts are positive, hi rounded down and lo never zero (p's lowest bit is set), so that weight times
+// infinity is infinity and not inf - inf or 0 inf (in fp16 down to 2^-16 of the row's largest weight, below which lo can be lost).
+struct Parts {
+  unsigned hi, lo;
+};
+template <bool BF16, bool E8>
+__device__ __forceinline__ Parts split_pair(float a, float b) {
+  Parts p;
+  float h0, h1;
+  if constexpr (E8) {
+    p.hi = pack_pair<true>(a, b);
+    unpack_pair<true>(p.hi, h0, h1);
+    p.lo = pack_pair<true>(a - h0, b - h1);
+  } else {
+    const unsigned ia = __float_as_uint(a) | 1u, ib = __float_as_uint(b) | 1u;
+    a = __uint_as_float(ia), b = __uint_as_float(ib);
+    if constexpr (BF16) p.hi = __builtin_amdgcn_perm(ib, ia, 0x07060302u);
+    else p.hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b));
+    unpack_pair<BF16>(p.hi, h0, h1);
+    p.lo = pack_pair<BF16>(a - h0, b - h1);
+  }
+  return p;
+}
+
 // A load, with the streaming hint where what is read is far larger than the caches.
 template <bool STREAM, typename T>
 __device__ __forceinline__ T load_from(const T* p) {
@@ -108,6 +132,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   typedef std::conditional_t<VD == 1, unsigned, std::conditional_t<VD == 2, u32x2, u32x4>> VWord;
   constexpr int SUB = paged_places(D, E8);     // places of 16 tokens of a tile
   constexpr bool PV_BF16 = BF16 || E8;         // (an e4m3 value's power of two goes to the probability, which fp16 has not the range for)
+  constexpr float kTopWeight = PV_BF16 ? 0.f : 15.f;   // weights up to 2^15 in fp16, so that small ones are not below its range
   extern __shared__ __align__(16) float smem[];
   const int wave = uniform(threadIdx.x >> 6);
   const PagedParams& cache = p.cache;
@@ -296,7 +321,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
           for (int r = 0; r < 4; ++r) o[j][r] *= keep;
       }
     }
-    const float shift = top == -INFINITY ? 0.f : -top * p.scale_log2;
+    const float shift = top == -INFINITY ? 0.f : fmaf(-top, p.scale_log2, kTopWeight);
 #pragma unroll
     for (int a = 0; a < SUB; ++a) {
 #pragma unroll
@@ -307,10 +332,8 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        hi[a / 2][a % 2 * 2 + r] = pack_pair<PV_BF16>(s[a][2 * r], s[a][2 * r + 1]);
-        float h0, h1;
-        unpack_pair<PV_BF16>(hi[a / 2][a % 2 * 2 + r], h0, h1);
-        lo[a / 2][a % 2 * 2 + r] = pack_pair<PV_BF16>(s[a][2 * r] - h0, s[a][2 * r + 1] - h1);
+        const Parts two = split_pair<BF16, E8>(s[a][2 * r], s[a][2 * r + 1]);
+        hi[a / 2][a % 2 * 2 + r] = two.hi, lo[a / 2][a % 2 * 2 + r] = two.lo;
       }
     }
   };

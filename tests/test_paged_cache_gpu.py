@@ -315,6 +315,25 @@ def test_attention_shows_what_it_attends_to(ops, dev):
     within(got[[0, 2]], want[[0, 2]], allowed[[0, 2]], "beside them")
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_of_infinite_values(ops, dev, dtype, dim):
+    """Infinities among the values come out with their sign whatever the bits of their weight (one, a power of two, any) and wherever
+    the token is; both signs in a feature, and NaN, are NaN."""
+    lengths = [1, 2, 4, 17, 60, 333, 1500, 60] + list(range(3, 43))
+    c = Cache(dev, lengths, 2, dim, 16, dtype, poison=False, seed=7)
+    q = queries(dev, len(lengths), 8, dim, dtype) * 0.25   # (weights of a row within a factor of 2^16)
+    q[:3] = 0.0                                            # equal weights: 1, 1/2, 1/4
+    for s, n in enumerate(lengths):
+        for h in range(2):
+            for d, (token, x) in enumerate(((0, math.inf), (n - 1, -math.inf), (n // 2, math.inf), (n // 3, math.nan))):
+                c.values[c.table[s, token // 16], h, token % 16, d * 9 + h] = x
+    c.values[c.table[7, 0], :, :2, 50] = torch.tensor([math.inf, -math.inf], device=dev, dtype=dtype)
+    want, allowed = c.attend(q, dim ** -0.5)
+    assert want[:, :, 9].isinf().any() and want[7, :, 50].isnan().all()
+    within(attend(ops, c, q), want, allowed, "infinite values")
+
+
 def test_scores_of_large_magnitude(ops, dev):
     """A score far above the rest after many small ones, and below: maxima that grow late and never."""
     c = Cache(dev, [400, 400], 1, 64, 16, BF16, poison=False)
