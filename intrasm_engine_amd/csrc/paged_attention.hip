@@ -17,12 +17,17 @@ constexpr int kWholeTiles = 8;
 // 500 30.5 and 24.8.
 constexpr int kWideRows = 512;
 // Parts: one round of resident workgroups where rows are few (131071 tokens, 8 rows: 92.8 us, two rounds 99.8), two where rows of unequal
-// lengths come anyway (512 rows of 4000 .. 16384, e4m3: 225.6 one, 207.6 two, 207.7 three).
-constexpr int kTwoRounds = 256;
+// lengths come anyway (512 rows of 4000 .. 16384, e4m3: 221 one, 205.7 two, 206.3 three, 207.7 four; 2048 of 1 .. 4096, heads of 64: 65.7,
+// 62.4, 62.6, 63.2), and more of them where a CU has one workgroup (256 rows of 100 .. 20000, heads of 256 in 16 bits: 512 workgroups 199,
+// 1024 184, 1536 193).
+constexpr int kTwoRounds = 256, kUneven = 1024;
+// Tiles have a workgroup each, if that makes at most this many: 8 rows of 4000 tokens 13.8 us, by two tiles 15.6, by four 18.6 (8192: 15.4,
+// 16.8 and 19.3); 32 rows of 3000, the other side, 18.9, 17.3 and 20.1.
+constexpr int kFew = 512;
 
 struct Split {
   long long blocks, slots, workgroups;   // blocks of up to 16 heads of a key head; parts beyond one per sequence; workgroups of the launch
-  int fixed, pitch;                      // parts of every row (0: by the lengths)
+  int few, fixed, pitch;                 // (PagedAttentionParams); parts of every row (0: by the lengths)
   bool wide;
 };
 Split split_of(const iex_paged_cache& c, int heads, int count) {
@@ -33,11 +38,14 @@ Split split_of(const iex_paged_cache& c, int heads, int count) {
   const long long rows = s.blocks * c.seqs;
   const bool whole = most <= kWholeTiles;
   s.wide = whole && rows < kWideRows;
-  s.slots = whole ? 0 : paged_slots(resident(c.head_dim, c.eight_bits) * (rows < kTwoRounds ? 1 : 2) / s.blocks, c.seqs, most, kPagedLeast);
+  const int round = resident(c.head_dim, c.eight_bits), wanted = rows < kTwoRounds ? round : 2 * round < kUneven ? kUneven : 2 * round;
+  s.slots = whole ? 0 : paged_slots(wanted / s.blocks, c.seqs, most);
+  s.few = (int)(kFew / s.blocks);
   s.fixed = whole ? 1 : 0;
   if (count && !whole) {   // (every row is as long)
-    const long long total = (long long)c.seqs * most;
-    s.fixed = paged_parts(most, paged_part_most(total < INT_MAX ? (int)total : INT_MAX, (int)s.slots, kPagedLeast));
+    const long long all = (long long)c.seqs * most;
+    const int total = all < INT_MAX ? (int)all : INT_MAX;
+    s.fixed = paged_parts(most, paged_part_most(total, (int)s.slots, paged_least(total, s.few)));
   }
   s.workgroups = s.blocks * (s.fixed ? (long long)c.seqs * s.fixed : c.seqs + s.slots);
   return s;
@@ -123,7 +131,7 @@ extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, cons
   PagedAttentionParams p{};
   p.cache = paged_params(*cache);
   p.heads = heads, p.group = heads / cache->kv_heads, p.group_tiles = ceil_div(p.group, 16), p.pitch = s.pitch;
-  p.count = count, p.listed = listed, p.blocks = (int)s.blocks, p.slots = (int)s.slots, p.fixed = s.fixed;
+  p.count = count, p.listed = listed, p.blocks = (int)s.blocks, p.slots = (int)s.slots, p.few = s.few, p.fixed = s.fixed;
   p.q = static_cast<const unsigned short*>(q), p.out = static_cast<unsigned short*>(out);
   for (int i = 0; i < 3; ++i) p.q_strides[i] = q_strides[i], p.out_strides[i] = out_strides[i];
   p.q_rows = rows_of_chunks(q, q_strides);

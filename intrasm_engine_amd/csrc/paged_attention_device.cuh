@@ -25,6 +25,7 @@ struct PagedAttentionParams {
   int heads, group, group_tiles;   // query heads, those of a key head, blocks of 16 of them
   int pitch, count;                // query rows of a part's result; pages listed per sequence and key head, 0: all of the table
   int blocks, slots;               // blocks of up to 16 query heads of a key head; parts beyond one per sequence
+  int few;                         // tiles (of all sequences) that get a workgroup each
   int fixed;                       // parts of every row, where that does not go by the lengths (whole rows, listed pages); else 0
   const int* listed;
   const unsigned short* q;
@@ -35,8 +36,6 @@ struct PagedAttentionParams {
   float* partial;   // per part: group_rows x D sums, then per part group_rows maxima and sums
   float* stats;
 };
-
-constexpr int kPagedLeast = 2;   // tiles that are worth a workgroup
 
 // The lengths of 64 sequences, one a lane.
 struct LaneLengths {
@@ -61,7 +60,8 @@ __device__ __forceinline__ bool find_part(const PagedAttentionParams& p, LaneLen
     lengths.load(p.cache, s0);
     total += lane_tiles(p, lengths);
   }
-  const int most = paged_part_most(bcast_i(wave_scan(total), kWave - 1), p.slots, kPagedLeast);
+  total = bcast_i(wave_scan(total), kWave - 1);
+  const int most = paged_part_most(total, p.slots, paged_least(total, p.few));
   int before = 0;
   for (int s0 = 0; s0 < p.cache.seqs; s0 += kWave) {
     if (p.cache.seqs > kWave) lengths.load(p.cache, s0);

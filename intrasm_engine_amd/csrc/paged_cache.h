@@ -30,13 +30,15 @@ IEX_HD int paged_part_most(int total, int slots, int least) {
   const int even = total / slots + (total % slots != 0);
   return even > least ? even : least;
 }
+// The `least` above: one tile where all of them (at most `few`) can have a workgroup each, else two.
+IEX_HD int paged_least(int total, int few) { return total <= few ? 1 : 2; }
 IEX_HD int paged_parts(int tiles, int most) { return tiles <= most ? 1 : tiles / most + (tiles % most != 0); }
 // The first tile of a part (of part number `parts`: the end).
 IEX_HD int paged_part_begin(int tiles, int parts, int part) { return (int)((long long)tiles * part / parts); }
 
 // Slots that are worth having: none where no sequence can be long enough to be cut.
-IEX_HD long long paged_slots(long long wanted, long long seqs, int most_tiles, int least) {
-  const long long most = seqs * ((most_tiles + least - 1) / least - 1);
+IEX_HD long long paged_slots(long long wanted, long long seqs, int most_tiles) {
+  const long long most = seqs * (most_tiles - 1);
   return most < wanted ? (most < 0 ? 0 : most) : wanted < 1 ? 1 : wanted;
 }
 

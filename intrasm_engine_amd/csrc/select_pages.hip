@@ -277,10 +277,11 @@ void launch_forms(const SelectParams& p, bool once, hipStream_t s) {
     return;
   }
   note_kernel("page_score_kernel<%s, %d>", BF16 ? "bf16" : "f16", D);
-  // a chunk for each of four wavefronts, more where there are workgroups enough (the weights are made once a workgroup)
+  // a chunk for each of four wavefronts, two where there are workgroups enough (the weights are made once a workgroup): 8 rows of 2048 pages
+  // 13.3 us by one, 15.7 by two; 32 of 8192 42.2, 40.5, by four 41.2
   SelectParams scores = p;
   const long long chunks = (long long)ceil_div(width, 4 * chunk_of(D)) * rows;
-  scores.per_group = 4 * chunk_of(D) * (chunks >= 8 * 512 ? 8 : chunks >= 512 ? (int)(chunks / 512) : 1);
+  scores.per_group = 4 * chunk_of(D) * (chunks >= 1024 ? 2 : 1);
   hipLaunchKernelGGL((page_score_kernel<BF16, D>), dim3(ceil_div(width, scores.per_group), rows), dim3(256), 0, s, scores);
   if (width <= kSelectKept) {
     note_kernel("page_select_kernel<kept>");

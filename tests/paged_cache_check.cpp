@@ -70,10 +70,14 @@ static int append() {
 
 static int attend() {
   const int shift = draw(4, 8), page = 1 << shift, seqs = draw(1, 150), width = draw(0, 4) == 0 ? draw(0, 2) : draw(1, 60), pages = draw(1, 50);
-  const int count = draw(0, 1) ? 0 : draw(1, 20), least = draw(1, 4), entries = count ? count : width;
+  const int count = draw(0, 1) ? 0 : draw(1, 20), few = draw(0, 400), entries = count ? count : width;
   std::vector<int> lengths(seqs), tokens(seqs);
   for (int& l : lengths) l = draw(0, 9) == 0 ? (int)rng() : draw(0, width * page);
-  const int slots = draw(0, 5) == 0 ? 0 : (int)paged_slots(draw(0, 300), seqs, paged_tiles(entries * page), least), grid = seqs + slots;
+  const int slots = draw(0, 5) == 0 ? 0 : (int)paged_slots(draw(0, 300), seqs, paged_tiles(entries * page));
+  // parts of every row: whole rows, listed pages; 0: by the lengths
+  const int longest = paged_tiles(entries * page), fixed = slots == 0 ? 1 : count ? paged_parts(longest, paged_part_most(seqs * longest, slots, paged_least(seqs * longest, few))) : 0;
+  const int grid = fixed ? seqs * fixed : seqs + slots;
+  CHECK(!fixed || fixed <= 1 + slots / seqs, "%d parts, %d slots for %d", fixed, slots, seqs);
   int total = 0;
   for (int s = 0; s < seqs; ++s) {
     const int n = cached_length(lengths[s], width, page);
@@ -81,10 +85,10 @@ static int attend() {
     tokens[s] = count && n ? count * page : n;
     total += paged_tiles(tokens[s]);
   }
-  const int most = paged_part_most(total, slots, least);
+  const int most = paged_part_most(fixed ? seqs * longest : total, slots, paged_least(fixed ? seqs * longest : total, few));
   int items = 0;
   for (int s = 0; s < seqs; ++s) {
-    const int tiles = paged_tiles(tokens[s]), parts = paged_parts(tiles, most), n = cached_length(lengths[s], width, page);
+    const int tiles = paged_tiles(fixed && count ? count * page : tokens[s]), parts = fixed ? fixed : paged_parts(tiles, most), n = cached_length(lengths[s], width, page);
     std::vector<int> table(width), list(count), met(tokens[s] + 1, 0);
     for (int& p : table) p = draw(0, 5) == 0 ? (int)rng() : draw(0, pages - 1);
     for (int& p : list) p = draw(0, 5) == 0 ? (int)rng() : draw(0, width);
@@ -92,10 +96,10 @@ static int attend() {
     for (int i = 0; i < parts; ++i, ++items) {
       const int from = paged_part_begin(tiles, parts, i), to = paged_part_begin(tiles, parts, i + 1);
       CHECK(from < to && to - from <= most, "part of %d tiles, at most %d", to - from, most);
-      const int begin = from * kPagedTile, end = std::min(tokens[s], to * kPagedTile), waves = draw(0, 1) ? 4 : 8;
+      const int begin = from * kPagedTile, end = std::min(tokens[s], to * kPagedTile), waves = draw(0, 1) ? 4 : 8, places = draw(0, 1) ? 2 : 4;
       for (int wave = 0; wave < waves; ++wave)
-        for (int t = begin + wave * 32; t < end; t += waves * 32)
-          for (int a = 0; a < 2; ++a) {
+        for (int t = begin + wave * places * 16; t < end; t += waves * places * 16)
+          for (int a = 0; a < places; ++a) {
             const PagedPlace place = paged_place(t + a * 16, shift);
             CHECK(place.slot % 16 == 0 && place.slot + 16 <= page, "slot %d of %d", place.slot, page);
             if (place.entry >= entries) continue;
