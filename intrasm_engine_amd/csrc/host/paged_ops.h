@@ -47,8 +47,10 @@ iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys,
     check_tensor(values, q, 4, op, "values");
     TORCH_CHECK(values.sizes() == keys.sizes() && values.scalar_type() == keys.scalar_type(), op, ": keys and values must be alike");
     TORCH_CHECK(keys.size(3) == q.size(2), op, ": heads of ", q.size(2), " over a cache of heads of ", keys.size(3));
-    for (const Tensor* t : {&keys, &values})
+    for (const Tensor* t : {&keys, &values}) {
+      check_no_gradient(*t, op);
       TORCH_CHECK(t->numel() == 0 || t->select(0, 0).is_contiguous(), op, ": a page of keys or values must be contiguous");
+    }
     c.pages = as_int(keys.size(0), op), c.kv_heads = as_int(keys.size(1), op), c.page_size = as_int(keys.size(2), op), c.head_dim = as_int(keys.size(3), op);
     c.key_page_stride = keys.stride(0), c.value_page_stride = values.stride(0);
     c.keys = const_cast<void*>(keys.const_data_ptr()), c.values = const_cast<void*>(values.const_data_ptr());
@@ -68,6 +70,7 @@ iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys,
   }
   if (bounds) {
     check_tensor(*bounds, q, 4, op, "bounds");
+    check_no_gradient(*bounds, op);
     if (!keys.defined()) c.pages = as_int(bounds->size(0), op), c.kv_heads = as_int(bounds->size(1), op), c.head_dim = as_int(bounds->size(3), op);
     TORCH_CHECK(bounds->scalar_type() == q.scalar_type() && bounds->is_contiguous() && bounds->size(0) == c.pages && bounds->size(1) == c.kv_heads &&
                     bounds->size(2) == 2 && bounds->size(3) == c.head_dim && c.head_dim == q.size(2),
@@ -105,6 +108,7 @@ Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& keys, const Ten
   int rotary = 0, positions = 0;
   if (rotation) {
     check_tensor(*rotation, k, 2, op, "rotation");
+    check_no_gradient(*rotation, op);
     TORCH_CHECK(rotation->scalar_type() == at::kFloat && rotation->is_contiguous(), op, ": rotation must be contiguous float32 (positions, rotated features)");
     positions = as_int(rotation->size(0), op), rotary = as_int(rotation->size(1), op);
   }

@@ -344,6 +344,7 @@ def test_calls_that_are_refused(dev, ops):
     attend("exponents", key_exponents=e.key_exponents, value_exponents=e.value_exponents)
     attend("uint8", keys=e.keys, values=e.values, key_exponents=e.key_exponents.int(), value_exponents=e.value_exponents)
     attend("no gradient", q=q.clone().requires_grad_())
+    attend("no gradient", values=c.values.clone().requires_grad_())
 
     def append(match, k=k, v=k, keys=c.keys, values=c.values, table=c.table, lengths=c.lengths, *more, **named):
         with pytest.raises(RuntimeError, match=match):
@@ -360,12 +361,15 @@ def test_calls_that_are_refused(dev, ops):
     append("every position", rotation=rotation[:-1])
     append("bounds must be", bounds=c.bounds[:-1])
     append("no gradient", k=k.clone().requires_grad_())
+    append("no gradient", keys=c.keys.clone().requires_grad_())
+    append("no gradient", rotation=rotation.clone().requires_grad_())
 
     def select(match, q=q, bounds=c.bounds, count=2, first=1, last=1, page=16):
         with pytest.raises(RuntimeError, match=match):
             ops.select_pages(q, bounds, c.table, c.lengths, page, count, first, last)
 
     select("at least one page", count=0)
+    select("no gradient", bounds=c.bounds.clone().requires_grad_())
     select("among them", count=1)
     select("at least one page", first=-1)
     select("pages of 16", page=17)
