@@ -5,7 +5,8 @@
 namespace iex {
 namespace {
 
-// Features whose tokens are whole aligned 16-byte chunks (up to the last ones).
+// Features whose tokens are whole aligned 16-byte chunks (up to the last ones).  (At other alignments 16 bytes a lane cost more than two:
+// 5 x 1001 tokens of 32 + 2 x 8 heads 67 us against 43.)
 bool columns_of_chunks(const void* x, const long long* strides) { return aligned(x, 16) && strides[0] == 1 && strides[1] % 8 == 0 && strides[2] % 8 == 0; }
 
 template <bool BF16, int D, bool E8, bool INTERLEAVED>

@@ -415,6 +415,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_kernel(AppendParams p) {
 // % 8)).  Where tokens are next to each other (features x tokens, as a projection W @ X leaves them: p.columns) they are read and
 // written 16 bytes at a time, eight tokens of a feature, and turned around two bytes at a time in LDS; else two bytes at a time in memory.
 constexpr int kColumnTokens = 64;
+typedef u32x4 AnyChunk __attribute__((aligned(2)));
 template <bool BF16, int D, bool E8, bool INTERLEAVED>
 __global__ __launch_bounds__(256, 4) void kv_append_columns_kernel(AppendParams p) {
   typedef unsigned short u16;
@@ -434,7 +435,9 @@ __global__ __launch_bounds__(256, 4) void kv_append_columns_kernel(AppendParams 
   for (int block = w.low / T * T; block < w.high; block += T) {
     const int low = max(w.low, block) - block, high = min(w.high, block + T) - block;   // rows of the tile
     const int token0 = w.first_token + block;                                           // ... of row 0
-    const bool whole = low == 0 && high == T && token0 % 8 == 0;                        // 64 tokens in eight chunks of eight
+    // 64 tokens in eight chunks of eight, from any token on: sequences that begin off a chunk 16 x 511 tokens of 3 x 32 heads of 128 152 ->
+    // 126 us, but 3 x 1001 of 32 + 2 x 8 heads of 256 52 -> 64
+    const bool whole = low == 0 && high == T && (D < 256 || token0 % 8 == 0);
     for (int head = w.head0; head < w.head_end; ++head) {
       const u16* src = w.src + head * w.per_head;
       __syncthreads();   // the tile before has been read
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_columns_kernel(AppendParams 
         const int c = threadIdx.x % 8, f = threadIdx.x / 8;
         u32x4 x[LOADS];
 #pragma unroll
-        for (int k = 0; k < LOADS; ++k) x[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + (f + k * 32) * w.per_feature + token0 + c * 8));
+        for (int k = 0; k < LOADS; ++k) x[k] = __builtin_nontemporal_load(reinterpret_cast<const AnyChunk*>(src + (f + k * 32) * w.per_feature + token0 + c * 8));
 #pragma unroll
         for (int k = 0; k < LOADS; ++k) {
           u16* to = element(c * 8, f + k * 32);
@@ -521,7 +524,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_columns_kernel(AppendParams 
           u32x4 packed;
 #pragma unroll
           for (int j = 0; j < 4; ++j) packed[j] = x[2 * j * D] | (unsigned)x[(2 * j + 1) * D] << 16;
-          *reinterpret_cast<u32x4*>(out + (f + k * 32) * p.out_feature + token0 + c * 8) = packed;
+          *reinterpret_cast<AnyChunk*>(out + (f + k * 32) * p.out_feature + token0 + c * 8) = packed;
         }
       } else if (p.columns) {
         for (int i = threadIdx.x; i < T * D; i += 256) {

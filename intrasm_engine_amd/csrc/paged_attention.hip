@@ -7,8 +7,8 @@
 namespace iex {
 namespace {
 
-// Workgroups of four wavefronts that are resident at once: by their registers one to four on each of the 256 CUs.
-int resident(int head_dim, bool e8) { return 256 * paged_simd_waves(head_dim, e8); }
+// Workgroups of four wavefronts that are resident at once: by their registers two to four on each of the 256 CUs.
+int resident(int head_dim) { return 256 * paged_simd_waves(head_dim); }
 
 // Rows of up to this many tiles stay whole, and there is no second launch: 32 x 700 tokens of 128 12.8 us, cut 14.5; 16 x 32 rows of
 // 600 .. 1023 39.7 and 44; 32 x 2000, the other side, 16 cut and 24 whole.
@@ -16,11 +16,13 @@ constexpr int kWholeTiles = 8;
 // Whole rows go to eight wavefronts each where four would leave CUs without work: 128 rows of 700 13.1 us by eight, 17.5 by four; 512 of
 // 500 30.5 and 24.8.
 constexpr int kWideRows = 512;
+// Rows of up to this many tokens have a wavefront each: 4096 rows of 12 tokens in tables of 64 28.6 us by four, 14.3 by one; of 64 33.3 and
+// 24.9; of 128, the other side, 47.5 and 51.5.
+constexpr int kNarrow = 64;
 // Parts: one round of resident workgroups where rows are few (131071 tokens, 8 rows: 92.8 us, two rounds 99.8), two where rows of unequal
 // lengths come anyway (512 rows of 4000 .. 16384, e4m3: 221 one, 205.7 two, 206.3 three, 207.7 four; 2048 of 1 .. 4096, heads of 64: 65.7,
-// 62.4, 62.6, 63.2), and more of them where a CU has one workgroup (256 rows of 100 .. 20000, heads of 256 in 16 bits: 512 workgroups 199,
-// 1024 184, 1536 193).
-constexpr int kTwoRounds = 256, kUneven = 1024;
+// 62.4, 62.6, 63.2).
+constexpr int kTwoRounds = 256;
 // Tiles have a workgroup each, if that makes at most this many: 8 rows of 4000 tokens 13.8 us, by two tiles 15.6, by four 18.6 (8192: 15.4,
 // 16.8 and 19.3); 32 rows of 3000, the other side, 18.9, 17.3 and 20.1.
 constexpr int kFew = 512;
@@ -28,7 +30,7 @@ constexpr int kFew = 512;
 struct Split {
   long long blocks, slots, workgroups;   // blocks of up to 16 heads of a key head; parts beyond one per sequence; workgroups of the launch
   int few, fixed, pitch;                 // (PagedAttentionParams); parts of every row (0: by the lengths)
-  bool wide;
+  bool wide, narrow;
 };
 Split split_of(const iex_paged_cache& c, int heads, int count) {
   const int group = heads / c.kv_heads, most = paged_tiles((count ? count : c.table_width) * c.page_size);
@@ -37,8 +39,9 @@ Split split_of(const iex_paged_cache& c, int heads, int count) {
   s.pitch = group < 16 ? group : 16;
   const long long rows = s.blocks * c.seqs;
   const bool whole = most <= kWholeTiles;
+  s.narrow = (count ? count : c.table_width) * c.page_size <= kNarrow;
   s.wide = whole && rows < kWideRows;
-  const int round = resident(c.head_dim, c.eight_bits), wanted = rows < kTwoRounds ? round : 2 * round < kUneven ? kUneven : 2 * round;
+  const int round = resident(c.head_dim), wanted = rows < kTwoRounds ? round : 2 * round;
   s.slots = whole ? 0 : paged_slots(wanted / s.blocks, c.seqs, most);
   s.few = (int)(kFew / s.blocks);
   s.fixed = whole ? 1 : 0;
@@ -79,8 +82,8 @@ int launch(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
 
 template <bool BF16, int D, bool E8>
 int launch_waves(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
-  constexpr int wide = paged_simd_waves(D, E8) > 1 ? 8 : 4;
-  return s.wide ? launch<BF16, D, E8, wide>(p, s, stream) : launch<BF16, D, E8, 4>(p, s, stream);
+  if (s.narrow) return launch<BF16, D, E8, 1>(p, s, stream);
+  return s.wide ? launch<BF16, D, E8, 8>(p, s, stream) : launch<BF16, D, E8, 4>(p, s, stream);
 }
 
 template <bool BF16>

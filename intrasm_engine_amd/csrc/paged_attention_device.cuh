@@ -123,10 +123,10 @@ __device__ __forceinline__ T load_from(const T* p) {
 // Places of 16 tokens of a wavefront's tile.  (Heads of 64 in 16 bits by four: 512 x 16 rows of 128 tokens 54.5 -> 63.7 us.)
 constexpr int paged_places(int head_dim, bool eight_bits) { return eight_bits && head_dim <= 128 ? 4 : 2; }
 // Wavefronts of a SIMD that the registers are cut for.
-constexpr int paged_simd_waves(int head_dim, bool eight_bits) { return head_dim == 256 ? (eight_bits ? 2 : 1) : head_dim == 128 ? 3 : 4; }
+constexpr int paged_simd_waves(int head_dim) { return head_dim == 256 ? 2 : head_dim == 128 ? 3 : 4; }
 
 template <bool BF16, int D, bool E8, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_attention_kernel(PagedAttentionParams p) {
+__global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attention_kernel(PagedAttentionParams p) {
   typedef unsigned short u16;
   constexpr int ES = E8 ? 1 : 2;               // bytes of an element
   constexpr int KS = D / 32;                   // steps of the sum over features
@@ -135,6 +135,9 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   constexpr int VD = F * ES / 4, VWORDS = VD == 8 ? 2 : 1;   // ... in dwords: 1, 2, 4 or 8
   typedef std::conditional_t<VD == 1, unsigned, std::conditional_t<VD == 2, u32x2, u32x4>> VWord;
   constexpr int SUB = paged_places(D, E8);     // places of 16 tokens of a tile
+  // Queries stay in LDS (a column without one has the last one's, its results are not used): with them in registers a SIMD has room for
+  // one wavefront only (256 rows of 1007 .. 1693 tokens, 16 heads 123 -> 102 us; 64 of 8192 86 -> 88).
+  constexpr bool Q_LDS = D == 256 && !E8;
   constexpr bool PV_BF16 = BF16 || E8;         // (an e4m3 value's power of two goes to the probability, which fp16 has not the range for)
   constexpr float kTopWeight = PV_BF16 ? 0.f : 15.f;   // weights up to 2^15 in fp16, so that small ones are not below its range
   extern __shared__ __align__(16) float smem[];
@@ -173,23 +176,38 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   int end = min(tokens, paged_part_begin(tiles, parts, part + 1) * kPagedTile);
 
   // ---- queries: columns of the first product ----
-  u32x4 fq[KS];
+  // Rows of aligned chunks go straight into registers, queries of other strides through LDS.
+  u32x4 fq[Q_LDS ? 1 : KS];
+  auto feature = [&](int s) { return E8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8; };
+  u16* const q_rows = reinterpret_cast<u16*>(smem);   // (D + 8 apart: 16 columns are in different banks)
+  if (Q_LDS || !p.q_rows) {
+    for (int i = threadIdx.x; i < rows * (D / 8); i += WAVES * 64) {
+      const int row = i / (D / 8), d = i % (D / 8) * 8;
+      const u16* q = p.q + seq * p.q_strides[0] + (long long)(kv_head * p.group + group_tile * 16 + row) * p.q_strides[1];
+      u32x4 x;
+      if (p.q_rows) {
+        x = *reinterpret_cast<const u32x4*>(q + d);
+      } else {
 #pragma unroll
-  for (int s = 0; s < KS; ++s) fq[s] = u32x4{0u, 0u, 0u, 0u};
-  if (col < rows) {
-    const u16* q = p.q + seq * p.q_strides[0] + (long long)(kv_head * p.group + group_tile * 16 + col) * p.q_strides[1];
-    if (p.q_rows) {   // rows of aligned 16-byte chunks
-#pragma unroll
-      for (int s = 0; s < KS; ++s) fq[s] = *reinterpret_cast<const u32x4*>(q + (E8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8));
-    } else {
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d = E8 ? s / 2 * 64 + g * 16 + s % 2 * 8 : s * 32 + g * 8;
-        unsigned w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = q[(d + 2 * j) * p.q_strides[2]] | (unsigned)q[(d + 2 * j + 1) * p.q_strides[2]] << 16;
-        fq[s] = u32x4{w[0], w[1], w[2], w[3]};
+        for (int j = 0; j < 4; ++j) x[j] = q[(d + 2 * j) * p.q_strides[2]] | (unsigned)q[(d + 2 * j + 1) * p.q_strides[2]] << 16;
       }
+      *reinterpret_cast<u32x4*>(q_rows + row * (D + 8) + d) = x;
+    }
+    __syncthreads();
+  }
+  if constexpr (!Q_LDS) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) fq[s] = u32x4{0u, 0u, 0u, 0u};
+    if (!p.q_rows) {
+      if (col < rows) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) fq[s] = *reinterpret_cast<const u32x4*>(q_rows + col * (D + 8) + feature(s));
+      }
+      __syncthreads();   // (the wavefronts' results go there)
+    } else if (col < rows) {
+      const u16* q = p.q + seq * p.q_strides[0] + (long long)(kv_head * p.group + group_tile * 16 + col) * p.q_strides[1];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) fq[s] = *reinterpret_cast<const u32x4*>(q + feature(s));
     }
   }
 
@@ -269,8 +287,13 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   auto scores = [&]() {
 #pragma unroll
     for (int a = 0; a < SUB; ++a) s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int q_at = (min(col, rows - 1) * (D + 8) + g * 8) * 2;
+    if constexpr (Q_LDS) asm volatile("" : "+v"(q_at));   // (else all of them would be read ahead of the loop, into registers)
 #pragma unroll
-    for (int e = 0; e < KS; ++e)
+    for (int e = 0; e < KS; ++e) {
+      u32x4 f;
+      if constexpr (Q_LDS) f = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(smem) + q_at + e * 64);
+      else f = fq[e];
 #pragma unroll
       for (int a = 0; a < SUB; ++a) {
         u32x4 fk;
@@ -280,8 +303,9 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
         } else {
           fk = key[a][e];
         }
-        s[a] = mfma_16x16x32<BF16>(fk, fq[e], s[a]);
+        s[a] = mfma_16x16x32<BF16>(fk, f, s[a]);
       }
+    }
     if constexpr (E8) {
 #pragma unroll
       for (int a = 0; a < SUB; ++a)
@@ -387,6 +411,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D, E8)) void paged_att
   }
 
   // ---- the wavefronts meet ----
+  if constexpr (Q_LDS) __syncthreads();   // (in place of the queries)
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
   if (attended == 0) sum = -1.f;   // no token at all: zeros, whatever the formula says of an empty sum

@@ -238,6 +238,25 @@ def test_attention(ops, dev, dtype, e8, dim, page, kv_heads, heads, layout):
     assert torch.equal(attend(ops, c, q, scale), got)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [[77, 130, 200, 65], [129, 64, 1, 190], [5, 3, 376]])
+def test_append_columns_of_sequences_off_the_chunk(ops, dev, dim, new):
+    """Features of whole chunks of tokens whose sequences begin anywhere, in tiles of 64 and what is left of them."""
+    check_append(ops, dev, new, [0] * len(new), 2, 3, dim, 64, BF16, False, dim, False, True, "features", extra=-sum(new) % 8)
+    check_append(ops, dev, new, [64] + [63] * (len(new) - 1), 1, 2, dim, 16, F16, True, 64, True, False, "features", extra=8 - sum(new) % 8)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("e8", [False, True])
+@pytest.mark.parametrize("dim,kv_heads,heads,layout", [(64, 2, 6, "tokens"), (128, 1, 17, "features"), (256, 3, 3, "tokens"), (256, 1, 20, "features")])
+def test_attention_of_short_tables(ops, dev, dtype, e8, dim, kv_heads, heads, layout):
+    """Tables of up to 64 tokens, and one page more."""
+    for page, lengths in ((16, [0, 1, 15, 16]), (16, [3, 17, 33, 47, 48, 49, 63, 64]), (32, [31, 32, 33, 64, 0]), (64, [1, 64, 30]), (16, [65, 64, 80]), (64, [128, 7])):
+        c = Cache(dev, lengths, kv_heads, dim, page, dtype, e8=e8)
+        q = queries(dev, len(lengths), heads, dim, dtype, layout, size=2.0)
+        within(attend(ops, c, q), *c.attend(q, dim ** -0.5), f"{page} {lengths}")
+
+
 @pytest.mark.parametrize("e8", [False, True])
 @pytest.mark.parametrize("lengths,kv_heads,heads,dim,page", [([9000], 2, 4, 128, 64), ([5000, 3, 0, 1700], 1, 2, 64, 16), ([2500] * 3, 1, 5, 256, 256)])
 def test_attention_in_parts(ops, dev, e8, lengths, kv_heads, heads, dim, page):
