@@ -13,7 +13,7 @@
 // in as two 16-bit parts: matrix cores idle otherwise, and one part rounded costs about half again the error of the rounded result.
 //
 // A sequence is split over its length into parts, a workgroup each (paged_cache.h: parts are cut from the lengths on the device,
-// so a replayed graph follows them); four wavefronts take a part's tiles in turn and meet in LDS, parts meet in a second launch.
+// so a replayed graph follows them); one, four or eight wavefronts take its tiles in turn and meet in LDS, parts meet in a second launch.
 // An 8-bit cache (e4m3) widens to 16 bits in registers; its powers of two go to the scores and the probabilities.
 //
 // Measured: 131071 tokens, 8 key heads of 128, 64 query heads, bf16 87 us = 6.3 TB/s, its join 6; 64 sequences of 4000 .. 16384 in e4m3

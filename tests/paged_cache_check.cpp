@@ -96,7 +96,7 @@ static int attend() {
     for (int i = 0; i < parts; ++i, ++items) {
       const int from = paged_part_begin(tiles, parts, i), to = paged_part_begin(tiles, parts, i + 1);
       CHECK(from < to && to - from <= most, "part of %d tiles, at most %d", to - from, most);
-      const int begin = from * kPagedTile, end = std::min(tokens[s], to * kPagedTile), waves = draw(0, 1) ? 4 : 8, places = draw(0, 1) ? 2 : 4;
+      const int begin = from * kPagedTile, end = std::min(tokens[s], to * kPagedTile), waves = draw(0, 2) ? 4 << draw(0, 1) : 1, places = draw(0, 1) ? 2 : 4;
       for (int wave = 0; wave < waves; ++wave)
         for (int t = begin + wave * places * 16; t < end; t += waves * places * 16)
           for (int a = 0; a < places; ++a) {
