@@ -58,14 +58,14 @@ size_t partial_floats(const iex_paged_cache& c, const Split& s) { return (size_t
 
 template <bool BF16, int D, bool E8, int WAVES>
 int launch(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
-  const int lds = WAVES * s.pitch * (D + 2) * 4;
+  const int lds = WAVES * s.pitch * (paged_sum_pitch(D) + 2) * 4;
   auto kern = paged_attention_kernel<BF16, D, E8, WAVES>;
   if (lds > 64 * 1024) {
     static thread_local unsigned long long raised = 0;   // per instantiation: on which devices
     int device = 0;
     if (int rc = check_hip(hipGetDevice(&device), "hipGetDevice")) return rc;
     if (!(raised >> (device & 63) & 1)) {
-      if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, WAVES * 16 * (D + 2) * 4),
+      if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, WAVES * 16 * (paged_sum_pitch(D) + 2) * 4),
                              "hipFuncSetAttribute(LDS size)"))
         return rc;
       raised |= 1ull << (device & 63);
