@@ -10,7 +10,7 @@
 //                  if group g's share of the sum over tokens is those very tokens.  A lane loads 16 bytes (features c * 8 ..) of
 //                  each of them; one byte permute per dword pairs tokens, and operand j has features c * 8 + j as its rows.
 // The running maximum and sum are per query; sums follow a new maximum only where some score has passed it.  Probabilities go
-// in as two 16-bit parts: matrix cores idle otherwise, and one part rounded costs about half again the error of the rounded result.
+// in as 16-bit parts, three of bf16 or two of fp16, so that nothing is lost: matrix cores idle otherwise.
 //
 // A sequence is split over its length into parts, a workgroup each (paged_cache.h: parts are cut from the lengths on the device,
 // so a replayed graph follows them); one, four or eight wavefronts take its tiles in turn and meet in LDS, parts meet in a second launch.
@@ -88,29 +88,29 @@ __device__ __forceinline__ unsigned widen_pair(unsigned codes) {
   else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, HIGH));
 }
 
-// Two weights as pairs of 16-bit parts, p = hi + lo.  bf16: 16 bits of p, 2^-16 of it at most are lost; fp16: 21.  Where values can be
-// infinite (16-bit caches) both parts are positive, hi rounded down and lo never zero (p's lowest bit is set), so that weight times
-// infinity is infinity and not inf - inf or 0 inf (in fp16 down to 2^-16 of the row's largest weight, below which lo can be lost).
-struct Parts {
-  unsigned hi, lo;
-};
+// Two weights as 16-bit parts whose sum they are: three of bf16 hold all 24 bits, two of fp16 22 (a difference of 2^-22 beside a result
+// rounded at 2^-11).  Two of bf16 would hold 16, and results then differ more often by a bit from what 32-bit weights give (1.1e-4 of them in place
+// of 1.9e-5 over 64 pages of 64 tokens; the third part is 61.4 -> 61.9 us of 128 x 1 .. 4096 tokens in heads of 64, 206.4 -> 208.2 of 64 x 4000 .. 16384
+// in e4m3).  Where values can be infinite (16-bit caches) every part is positive: all but the last are rounded down and none is zero (the weight's lowest bit is set, and
+// a last part that would be zero is the smallest there is), so that weight times infinity is infinity and not inf - inf or 0 inf
+// (in fp16 down to 2^-16 of the row's largest weight, below which the last part can be lost).
+template <bool BF16>
+constexpr int kWeightParts = BF16 ? 3 : 2;
 template <bool BF16, bool E8>
-__device__ __forceinline__ Parts split_pair(float a, float b) {
-  Parts p;
-  float h0, h1;
-  if constexpr (E8) {
-    p.hi = pack_pair<true>(a, b);
-    unpack_pair<true>(p.hi, h0, h1);
-    p.lo = pack_pair<true>(a - h0, b - h1);
-  } else {
-    const unsigned ia = __float_as_uint(a) | 1u, ib = __float_as_uint(b) | 1u;
-    a = __uint_as_float(ia), b = __uint_as_float(ib);
-    if constexpr (BF16) p.hi = __builtin_amdgcn_perm(ib, ia, 0x07060302u);
-    else p.hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b));
-    unpack_pair<BF16>(p.hi, h0, h1);
-    p.lo = pack_pair<BF16>(a - h0, b - h1);
+__device__ __forceinline__ void split_pair(float a, float b, unsigned (&part)[kWeightParts<BF16>]) {
+  constexpr int N = kWeightParts<BF16>;
+  if constexpr (!E8) a = __uint_as_float(__float_as_uint(a) | 1u), b = __uint_as_float(__float_as_uint(b) | 1u);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (E8 || i == N - 1) part[i] = pack_pair<BF16>(a, b);
+    else if constexpr (BF16) part[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    else part[i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b));
+    if (i == N - 1) break;
+    float a0, b0;
+    unpack_pair<BF16>(part[i], a0, b0);
+    a -= a0, b -= b0;
+    if (!E8 && i == 1) a = fmaxf(a, 0x1p-126f), b = fmaxf(b, 0x1p-126f);   // (the first rest has the lowest bit)
   }
-  return p;
 }
 
 // A load, with the streaming hint where what is read is far larger than the caches.
@@ -318,7 +318,8 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
         for (int r = 0; r < 4; ++r) s[a][r] *= power_of_two(ke[a] >> (r * 8) & 0xFFu);
     }
   };
-  u32x4 hi[SUB / 2], lo[SUB / 2];
+  constexpr int PARTS = kWeightParts<PV_BF16>;
+  u32x4 weight[SUB / 2][PARTS];
   auto weights = [&](const Where& w) {
     int valid = 0;
 #pragma unroll
@@ -365,8 +366,10 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const Parts two = split_pair<BF16, E8>(s[a][2 * r], s[a][2 * r + 1]);
-        hi[a / 2][a % 2 * 2 + r] = two.hi, lo[a / 2][a % 2 * 2 + r] = two.lo;
+        unsigned part[PARTS];
+        split_pair<PV_BF16, E8>(s[a][2 * r], s[a][2 * r + 1], part);
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) weight[a / 2][i][a % 2 * 2 + r] = part[i];
       }
     }
   };
@@ -387,8 +390,8 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
             fv[w] = __builtin_amdgcn_perm(value_dword(a, r + 1, j / 2), value_dword(a, r, j / 2), j % 2 ? 0x07060302u : 0x05040100u);
           }
         }
-        o[j] = mfma_16x16x32<PV_BF16>(fv, hi[two], o[j]);
-        o[j] = mfma_16x16x32<PV_BF16>(fv, lo[two], o[j]);
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) o[j] = mfma_16x16x32<PV_BF16>(fv, weight[two][i], o[j]);
       }
   };
 
