@@ -484,9 +484,10 @@ int iex_kv_append(const iex_paged_cache* cache, int tokens, const int* offsets, 
  * count), the pages of the sequence's table to attend to; entries outside the table (-1) are passed over, one that comes twice
  * counts twice.  No token to attend to: zeros.  The sequences are split over their lengths; the parts meet in `workspace`
  * (iex_paged_attention_workspace_bytes, 0: none; 256-byte aligned), which the call uses until its work on the stream has run.
- * Scores, weights and sums are held in 32 bits; weights are multiplied with fp16 values in 22 of their 24 bits.
+ * Scores, weights and sums are held in 32 bits; weights are multiplied with fp16 values in 22 of their 24 bits, with e4m3 rows in fewer than 24
+ * where the row's exponent is below 48 (all of its values below 2^-70).
  * What is not attended to leaves no trace, infinities and NaN included; what is attended to shows as in the formula (infinite
- * values of fp16 caches down to 2^-16 of the row's largest weight, below which they can show as NaN).  scale > 0. */
+ * values of fp16 caches down to 2^-16 of the row's largest weight, of bf16 caches down to 2^-80, below which they can show as NaN).  scale > 0. */
 size_t iex_paged_attention_workspace_bytes(const iex_paged_cache* cache, int heads, int count);
 int iex_paged_attention(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, float scale,
                         const int* listed, int count, void* out, const long long* out_strides, void* workspace,

@@ -76,7 +76,7 @@ int launch(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
   if (int rc = check_hip(hipGetLastError(), "paged attention launch")) return rc;
   if (s.fixed == 1) return 0;
   note_kernel("paged_join_kernel<%s, %d>", BF16 ? "bf16" : "f16", D);
-  hipLaunchKernelGGL((paged_join_kernel<BF16, D>), dim3((unsigned)p.cache.seqs, (unsigned)p.heads), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((paged_join_kernel<BF16, D, E8>), dim3((unsigned)p.cache.seqs, (unsigned)p.heads), dim3(256), 0, stream, p);
   return check_hip(hipGetLastError(), "paged attention join launch");
 }
 

@@ -41,6 +41,16 @@ struct PagedAttentionParams {
   float* stats;
 };
 
+// Tokens that a sequence of `length` tokens attends to at most.
+__device__ __forceinline__ int row_tokens(const PagedAttentionParams& p, int length) { return p.count && length ? p.count << p.cache.page_shift : length; }
+
+// What weights, 1 at most, are multiplied with on their way to the values, and the sum of them when it divides.  Before bf16 and e4m3 values
+// they come to 1 at most all together, so that their sums stay within the values' range (two values of 2e38 came out infinite); before
+// fp16 values, far from 32 bits' ends, they go up to 2^15, so that small ones are not below fp16's range.
+__device__ __forceinline__ float weight_scale(bool range_of_bf16, int tokens) {
+  return power_of_two(range_of_bf16 ? 127 - (tokens > 1 ? 32 - __builtin_clz(tokens - 1) : 0) : 127 + 15);
+}
+
 // The lengths of 64 sequences, one a lane.
 struct LaneLengths {
   int from = -kWave, mine = 0;
@@ -89,11 +99,11 @@ __device__ __forceinline__ unsigned widen_pair(unsigned codes) {
 }
 
 // Two weights as 16-bit parts whose sum they are: three of bf16 hold all 24 bits, two of fp16 22 (a difference of 2^-22 beside a result
-// rounded at 2^-11).  Two of bf16 would hold 16, and results then differ more often by a bit from what 32-bit weights give (1.1e-4 of them in place
-// of 1.9e-5 over 64 pages of 64 tokens; the third part is 61.4 -> 61.9 us of 128 x 1 .. 4096 tokens in heads of 64, 206.4 -> 208.2 of 64 x 4000 .. 16384
-// in e4m3).  Where values can be infinite (16-bit caches) every part is positive: all but the last are rounded down and none is zero (the weight's lowest bit is set, and
-// a last part that would be zero is the smallest there is), so that weight times infinity is infinity and not inf - inf or 0 inf
-// (in fp16 down to 2^-16 of the row's largest weight, below which the last part can be lost).
+// rounded at 2^-11).  Two of bf16 would hold 16, and results then differ more often by a bit from what 32-bit weights give (1.1e-4 of them in
+// place of 1.9e-5 over 64 pages of 64 tokens; the third part is 61.4 -> 61.9 us of 128 x 1 .. 4096 tokens in heads of 64, 206.4 -> 208.2 of
+// 64 x 4000 .. 16384 in e4m3).  Where values can be infinite (16-bit caches) every part is positive: all but the last are rounded down and none
+// is zero (the weight's lowest bit is set, and a last part that would be zero is the smallest there is), so that weight times infinity is
+// infinity and not inf - inf or 0 inf (in fp16 down to 2^-16 of the row's largest weight, in bf16 2^-80: below, a part can be lost).
 template <bool BF16>
 constexpr int kWeightParts = BF16 ? 3 : 2;
 template <bool BF16, bool E8>
@@ -144,7 +154,6 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
   // one wavefront only (256 rows of 1007 .. 1693 tokens, 16 heads 123 -> 102 us; 64 of 8192 86 -> 88).
   constexpr bool Q_LDS = D == 256 && !E8;
   constexpr bool PV_BF16 = BF16 || E8;         // (an e4m3 value's power of two goes to the probability, which fp16 has not the range for)
-  constexpr float kTopWeight = PV_BF16 ? 0.f : 15.f;   // weights up to 2^15 in fp16, so that small ones are not below its range
   extern __shared__ __align__(16) float smem[];
   const int wave = uniform(threadIdx.x >> 6);
   const PagedParams& cache = p.cache;
@@ -176,7 +185,8 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
   }
   const int col = lane & 15, g = lane >> 4;
   const int rows = min(16, p.group - group_tile * 16);   // queries
-  const int length = lengths.of(cache, seq), tokens = p.count && length ? p.count << cache.page_shift : length;
+  const int length = lengths.of(cache, seq), tokens = row_tokens(p, length);
+  const float up = weight_scale(PV_BF16, tokens);
   const int begin = paged_part_begin(tiles, parts, part) * kPagedTile;
   int end = min(tokens, paged_part_begin(tiles, parts, part + 1) * kPagedTile);
 
@@ -355,14 +365,14 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
           for (int r = 0; r < 4; ++r) o[j][r] *= keep;
       }
     }
-    const float shift = top == -INFINITY ? 0.f : fmaf(-top, p.scale_log2, kTopWeight);
+    const float shift = top == -INFINITY ? 0.f : -top * p.scale_log2;
 #pragma unroll
     for (int a = 0; a < SUB; ++a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         s[a][r] = __builtin_amdgcn_exp2f(fmaf(s[a][r], p.scale_log2, shift));   // (exp2(-infinity) = 0)
         sum += s[a][r];
-        if constexpr (E8) s[a][r] *= power_of_two(ve[a] >> (r * 8) & 0xFFu);
+        s[a][r] *= E8 ? power_of_two(ve[a] >> (r * 8) & 0xFFu) * up : up;
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -456,7 +466,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
     }
     if (parts == 1) {
       const int head = kv_head * p.group + group_tile * 16 + row;
-      p.out[seq * p.out_strides[0] + head * p.out_strides[1] + d * p.out_strides[2]] = f32_to_16(any ? acc / all : 0.f, BF16);
+      p.out[seq * p.out_strides[0] + head * p.out_strides[1] + d * p.out_strides[2]] = f32_to_16(any ? acc / (all * up) : 0.f, BF16);
     } else {
       const size_t to = (size_t)blockIdx.x * p.pitch + row;
       p.partial[to * D + d] = acc;
@@ -467,7 +477,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
 
 // Parts of a row into its result, a workgroup per sequence and query head: the parts' weights first, 256 at a time, then
 // 256 / (D / 4) parts side by side, a thread four features; they meet in LDS.
-template <bool BF16, int D>
+template <bool BF16, int D, bool E8>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p) {
   constexpr int LANES = D / 4, SIDE = 256 / LANES;   // threads of a row; parts side by side
   __shared__ float4 accs[SIDE][LANES];
@@ -477,6 +487,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p)
   LaneLengths lengths;
   int found, first = seq * p.fixed, number = p.fixed, tiles;
   if (!p.fixed && (!find_part(p, lengths, [&](int s, int, int) { return s == seq; }, found, first, number, tiles) || number == 1)) return;
+  const float up = weight_scale(BF16 || E8, row_tokens(p, lengths.of(p.cache, seq)));
   const int block = kv_head * p.group_tiles + in_group / 16;
   auto place = [&](int i) { return ((size_t)(first + i) * p.blocks + block) * p.pitch + in_group % 16; };
   const int lane = tid % LANES, side = tid / LANES;
@@ -530,7 +541,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p)
   float x = 0.f;
 #pragma unroll
   for (int i = 0; i < SIDE; ++i) x += reinterpret_cast<const float*>(accs[i])[tid];
-  p.out[seq * p.out_strides[0] + head * p.out_strides[1] + tid * p.out_strides[2]] = f32_to_16(any ? x / total : 0.f, BF16);
+  p.out[seq * p.out_strides[0] + head * p.out_strides[1] + tid * p.out_strides[2]] = f32_to_16(any ? x / (total * up) : 0.f, BF16);
 }
 
 }  // namespace iex

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from _paged import E4M3, HALF_STEP, Cache
+from _paged import E4M3, HALF_STEP, Cache, power
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -57,3 +57,36 @@ def test_bits_of_the_weights(ops, dev, dtype, e8, dim):
         got = attend(ops, c, q).double()
         allowed = want.abs() * HALF_STEP[dtype] + (3 * 2.0 ** -23 + 2 * parts + 4 * 2.0 ** -23) / 1.9
         assert ((got - want).abs() <= allowed).all(), f"{n}: {float(((got - want).abs() - allowed).max()):.3g} beyond {float(allowed.min()):.3g}"
+
+
+@pytest.mark.parametrize("dim,e8", [(64, False), (128, False), (256, False), (128, True)])
+@pytest.mark.parametrize("n", [1, 2, 3, 33, 300, 1500, 9000])
+def test_values_at_the_ends_of_the_range(ops, dev, dim, e8, n):
+    """softmax . v of values near bf16's largest is no larger than they are, however many there are; of its smallest normal ones no smaller
+    (e4m3: of exponents from 48 on).
+
+    Allowed: as in _paged.Cache.attend, and for the smallest the sums' own smallest step over a weight of 1 / (2 n)."""
+    c = Cache(dev, [n, n, n, n], 1, dim, 64, BF16, e8=e8, poison=False)
+    largest = float(torch.finfo(BF16).max)
+    for s, (size, exponent) in enumerate(((2e38, 247), (1.3 * 2.0 ** 127 if e8 else largest, 247), (2.0 ** -73 if e8 else 2.0 ** -110, 48), (2.0 ** -71 if e8 else 2.0 ** -126, 48))):
+        rows = torch.full((n, dim), size, device=dev)
+        rows[:, 1::2] *= -1
+        if s == 2:
+            rows *= 1 + torch.rand(n, dim, device=dev)
+        pages = c.table[s, :-(-n // 64)].long()
+        rows = torch.cat([rows, torch.zeros(-n % 64, dim, device=dev)]).view(-1, 1, 64, dim).to(BF16)
+        if e8:
+            c.values.view(torch.uint8)[pages] = (rows.double() / power(torch.tensor(exponent))).float().to(E4M3).view(torch.uint8)
+            c.value_exponents[pages] = exponent
+        else:
+            c.values[pages] = rows
+    q = torch.randn(4, 3, dim, device=dev).to(BF16)
+    q[0] = 0.0
+    scale = dim ** -0.5
+    want, allowed = c.attend(q, scale)
+    assert want[:2].abs().max() <= largest * (1 + 2.0 ** -40)
+    allowed[2:] += 2 * n * 2.0 ** -149
+    got = attend(ops, c, q, scale).double()
+    for s in range(4):
+        beyond = float(((got[s] - want[s]).abs() - allowed[s]).max())
+        assert beyond <= 0, (s, float(got[s].abs().max()), beyond / float(allowed[s].max()))
