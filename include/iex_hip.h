@@ -496,8 +496,9 @@ int iex_paged_attention(const iex_paged_cache* cache, int heads, const void* q, 
 /* out: (seqs, kv_heads, count), the `count` pages of every sequence's table whose keys can score highest with the query heads of
  * a key head, in ascending order, -1 behind them where there are fewer: the first `first` and last `last` pages that the
  * sequence uses, then by score = sum over the group's heads and the features of max(q lo, q hi), summed in 64 bits and rounded
- * once to 32; ties go to the lower page, a NaN score comes first, pages outside the cache are not selected.  Reads cache->bounds, not
- * keys and values (may be null).  workspace: iex_select_pages_workspace_bytes, 256-byte aligned. */
+ * once to 32 (where none of the group's queries is positive, an infinite largest key adds nothing, and where none is negative, an infinite
+ * smallest one; keys of 65504 that e4m3 rows store as 65536 have an infinite bound in fp16); ties go to the lower page, a NaN score comes first,
+ * pages outside the cache are not selected.  Reads cache->bounds, not keys and values (may be null).  workspace: iex_select_pages_workspace_bytes, 256-byte aligned. */
 size_t iex_select_pages_workspace_bytes(const iex_paged_cache* cache);
 int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, int count, int first,
                      int last, int* out, void* workspace, size_t workspace_bytes, void* stream);
