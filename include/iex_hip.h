@@ -473,8 +473,8 @@ typedef struct iex_paged_cache {
  * can hold; the first `rotary` features (a multiple of 16, 0: none) turn in pairs (j, j + rotary / 2), or (2j, 2j + 1) where
  * interleaved.  A sequence longer than its table or shorter than its new tokens is passed over, tokens behind the last
  * sequence's too: nothing is written to the cache, their rows of q_out are zeros.  Two sequences that append to the same page
- * in one call leave one of the two in it.  In an 8-bit cache infinities become NaN.  Bounds begin anew with a page's first token:
- * tokens that are taken back (a shorter length) and written again widen them at most. */
+ * in one call leave one of the two in it.  In an 8-bit cache infinities become NaN; a row's exponent is that of its finite values.  Bounds begin
+ * anew with a page's first token: tokens that are taken back (a shorter length) and written again widen them at most. */
 int iex_kv_append(const iex_paged_cache* cache, int tokens, const int* offsets, int heads, const void* k, const long long* k_strides,
                   const void* v, const long long* v_strides, const void* q, const long long* q_strides, void* q_out,
                   const long long* q_out_strides, const float* rotation, int positions, int rotary, int interleaved, void* stream);

@@ -159,6 +159,16 @@ __device__ __forceinline__ void store_unit(const AppendParams& p, bool is_k, int
 #pragma unroll
     for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
     top = group_max<D / 16>(top);
+    const bool finite = top < 0x7F800000u;
+    if (__ballot(!finite)) {   // an infinity or NaN in some row: the exponent is of the largest finite magnitude, so that the others are kept
+      unsigned rest = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const unsigned magnitude = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+        rest = max(rest, magnitude < 0x7F800000u ? magnitude : 0u);
+      }
+      top = group_max<D / 16>(rest);
+    }
     const int e = e4m3_exponent(top);
     const float down = power_of_two(254 - e), up = power_of_two(e);
     unsigned code[4];
@@ -167,7 +177,7 @@ __device__ __forceinline__ void store_unit(const AppendParams& p, bool is_k, int
       code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * down, x[4 * j + 1] * down, 0, false);
       code[j] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * down, x[4 * j + 3] * down, code[j], true);
     }
-    if (top >= 0x7F800000u) {   // an infinity or NaN in the row: e4m3 has no infinity, both become its NaN
+    if (!finite) {   // e4m3 has no infinity: it becomes NaN too
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if ((__float_as_uint(x[j]) & 0x7FFFFFFFu) >= 0x7F800000u) code[j / 4] |= 0x7Fu << (j % 4 * 8);

@@ -90,7 +90,7 @@ IEX_HD long long append_most_spans(long long tokens, long long seqs, int span) {
 
 // ---- e4m3 -------------------------------------------------------------------------------------------------------------
 // The exponent of a row whose largest magnitude has these bits (as fp32): the least power of two, biased by 127, that brings it
-// to 448, e4m3's largest value.  An infinity or NaN gives one that leaves them what they are.
+// to 448, e4m3's largest value.  (Of a row's finite values: its infinities and NaN become NaN.)
 IEX_HD int e4m3_exponent(unsigned magnitude_bits) {
   const int e = (int)((magnitude_bits + 0x1FFFFFu) >> 23) - 8;   // (mantissas above 1.75 round up)
   return e < 1 ? 1 : e > 254 ? 254 : e;

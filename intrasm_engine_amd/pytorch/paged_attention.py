@@ -34,7 +34,7 @@ class KVCache:
     """``pages`` pages of ``page_size`` (16 .. 256, a power of two) tokens for ``kv_heads`` heads of ``head_dim`` (64, 128 or 256).
 
     ``eight_bits``: e4m3 codes and, per token and head, the least power of two as their scale that brings the largest magnitude to
-    448 (one byte), in place of ``dtype``: half the memory, and half the time of reading it.  ``bounds``: also keep the smallest and
+    448 (one byte; infinities become NaN and do not count), in place of ``dtype``: half the memory, and half the time of reading it.  ``bounds``: also keep the smallest and
     largest key of every page, head and feature, which :meth:`select` reads (they begin anew with a page's first token; tokens that are
     taken back, by a shorter length, and written again widen them at most).  Who has which page is the caller's business: two
     sequences may share pages that neither appends to (a common prefix)."""

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from _paged import E4M3, HALF_STEP, Cache, power
+from _paged import E4M3, HALF_STEP, Cache, feature_major, power
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -90,3 +90,35 @@ def test_values_at_the_ends_of_the_range(ops, dev, dim, e8, n):
     for s in range(4):
         beyond = float(((got[s] - want[s]).abs() - allowed[s]).max())
         assert beyond <= 0, (s, float(got[s].abs().max()), beyond / float(allowed[s].max()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout,single", [("tokens", True), ("features", True), ("tokens", False), ("features", False)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_eight_bit_rows_keep_what_is_finite(ops, dev, dtype, layout, single, dim):
+    """Infinities and NaN of a row become NaN; its other features are stored by the least power of two that brings the largest finite one to
+    448, as in a row without them."""
+    n = 6 if single else 70
+    gen = torch.Generator(device=dev).manual_seed(4)
+    c = Cache(dev, [1] * n if single else [n], 2, dim, 16, dtype, e8=True, bounds=True, poison=False)
+    x = torch.randn(n, 2, dim, generator=gen, device=dev).to(dtype)
+    bad = torch.zeros(n, 2, dim, dtype=torch.bool, device=dev)
+    for i, value in enumerate((math.inf, -math.inf, math.nan)):
+        bad[i, 0, 5 + i] = True
+        x[i, 0, 5 + i] = value
+    bad[3, 1], bad[4, 0, 1:] = True, True
+    x[3, 1], x[4, 0, 1:] = math.inf, math.nan
+    shape = feature_major if layout == "features" else lambda t: t
+    offsets = None if single else torch.tensor([0, n], dtype=torch.int32, device=dev)
+    ops.kv_append_(shape(x), shape(x), c.keys, c.values, c.table, c.lengths, offsets, None, None, False, c.bounds, *c.exponents())
+    finite = torch.where(bad, 0.0, x.double())
+    top = finite.abs().amax(-1)
+    mantissa, exponent = torch.frexp(top)
+    exponent = torch.where(top == 0, 1, (exponent + 118 + (mantissa > 0.875)).clamp(1, 254))
+    step = torch.maximum(finite.abs() * HALF_STEP[E4M3], 2.0 ** -10 * power(exponent)[..., None])
+    for name, exponents in (("keys", c.key_exponents), ("values", c.value_exponents)):
+        for i in range(n):
+            page, slot = (int(c.table[i, 0]), 0) if single else (int(c.table[0, i // 16]), i % 16)
+            got = c.stored(name, page)[:, slot]
+            assert torch.equal(got.isnan(), bad[i]) and torch.equal(exponents[page, :, slot].long(), exponent[i])
+            assert ((got - finite[i]).abs()[~bad[i]] <= step[i][~bad[i]]).all()
