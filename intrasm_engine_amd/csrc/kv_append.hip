@@ -58,6 +58,7 @@ extern "C" int iex_kv_append(const iex_paged_cache* cache, int tokens, const int
   if (tokens == 0) return 0;
   IEX_REQUIRE(k && v && k_strides && v_strides, IEX_ERR_BAD_ARGUMENT, "kv_append: null pointer argument");
   IEX_REQUIRE(heads == 0 || (q && q_out && q_strides && q_out_strides), IEX_ERR_BAD_ARGUMENT, "kv_append: null pointer argument");
+  IEX_REQUIRE(cache->seqs == 0 || cache->lengths, IEX_ERR_BAD_ARGUMENT, "kv_append: null pointer argument");   // (without key heads too: queries turn by them)
   IEX_REQUIRE(rotary == 0 || (rotation && aligned(rotation, 16)), IEX_ERR_BAD_ARGUMENT, "kv_append: the rotation must be a 16-byte aligned array");
   IEX_REQUIRE(rotary >= 0 && rotary % 16 == 0 && rotary <= cache->head_dim, IEX_ERR_UNSUPPORTED,
               "kv_append: rotated features must be a multiple of 16 of the head's (%d of %d)", rotary, cache->head_dim);
