@@ -27,6 +27,8 @@ constexpr int kTwoRounds = 256;
 // 16.8 and 19.3); 32 rows of 3000, the other side, 18.9, 17.3 and 20.1.
 constexpr int kFew = 512;
 
+constexpr long long kMostListed = 1ll << 30;   // tokens of a list of pages
+
 struct Split {
   long long blocks, slots, workgroups;   // blocks of up to 16 heads of a key head; parts beyond one per sequence; workgroups of the launch
   int few, fixed, pitch;                 // (PagedAttentionParams); parts of every row (0: by the lengths)
@@ -105,7 +107,9 @@ int check_heads(const iex_paged_cache* c, int heads, const char* what) {
 
 extern "C" size_t iex_paged_attention_workspace_bytes(const iex_paged_cache* cache, int heads, int count) {
   using namespace iex;
-  if (check_paged_cache(cache, "paged_attention", false) || check_heads(cache, heads, "paged_attention") || heads == 0 || cache->seqs == 0 || count < 0) return 0;
+  if (check_paged_cache(cache, "paged_attention", false) || check_heads(cache, heads, "paged_attention") || heads == 0 || cache->seqs == 0 || count < 0 ||
+      (long long)count * cache->page_size >= kMostListed)
+    return 0;
   const Split s = split_of(*cache, heads, count);
   if (s.fixed == 1) return 0;
   return partial_floats(*cache, s) * 4 + (size_t)s.workgroups * s.pitch * 8;
@@ -119,7 +123,7 @@ extern "C" int iex_paged_attention(const iex_paged_cache* cache, int heads, cons
   if (int rc = check_heads(cache, heads, "paged_attention")) return rc;
   IEX_REQUIRE(count >= 0 && (!listed || count > 0), IEX_ERR_BAD_ARGUMENT, "paged_attention: a list of pages must have entries");
   IEX_REQUIRE(listed || count == 0, IEX_ERR_BAD_ARGUMENT, "paged_attention: null pointer argument");
-  IEX_REQUIRE((long long)count * cache->page_size < (1ll << 30), IEX_ERR_TOO_LARGE, "paged_attention: up to 2^30 tokens in a list of pages");
+  IEX_REQUIRE((long long)count * cache->page_size < kMostListed, IEX_ERR_TOO_LARGE, "paged_attention: up to 2^30 tokens in a list of pages");
   if (cache->seqs == 0 || heads == 0) return 0;
   IEX_REQUIRE(cache->pages > 0, IEX_ERR_BAD_ARGUMENT, "paged_attention: a cache without pages");
   IEX_REQUIRE(q && q_strides && out && out_strides, IEX_ERR_BAD_ARGUMENT, "paged_attention: null pointer argument");
