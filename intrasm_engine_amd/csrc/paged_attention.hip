@@ -23,10 +23,9 @@ constexpr int kNarrow = 64;
 // lengths come anyway (512 rows of 4000 .. 16384, e4m3: 221 one, 205.7 two, 206.3 three, 207.7 four; 2048 of 1 .. 4096, heads of 64: 65.7,
 // 62.4, 62.6, 63.2).
 constexpr int kTwoRounds = 256;
-// Tiles have a workgroup each, if that makes at most this many: 8 rows of 4000 tokens 13.8 us, by two tiles 15.6, by four 18.6 (8192: 15.4,
-// 16.8 and 19.3); 32 rows of 3000, the other side, 18.9, 17.3 and 20.1.
-constexpr int kFew = 512;
-
+// Tiles have a workgroup each, if that makes at most this many, one on each CU: a sequence of 4000 tokens, 8 key heads of 64 (256 workgroups)
+// 12.0 us, by two tiles 13.6; 64 listed pages of 64 (256) 10.3 and 11.9; 8192 tokens (512), the other side, 16.4 and 14.8.
+constexpr int kFew = 256;
 constexpr long long kMostListed = 1ll << 30;   // tokens of a list of pages
 
 struct Split {
@@ -50,7 +49,7 @@ Split split_of(const iex_paged_cache& c, int heads, int count) {
   if (count && !whole) {   // (every row is as long)
     const long long all = (long long)c.seqs * most;
     const int total = all < INT_MAX ? (int)all : INT_MAX;
-    s.fixed = paged_parts(most, paged_part_most(total, (int)s.slots, paged_least(total, s.few)));
+    s.fixed = paged_parts(most, paged_part_most(total - c.seqs, (int)s.slots, paged_least(total, s.few)));
   }
   s.workgroups = s.blocks * (s.fixed ? (long long)c.seqs * s.fixed : c.seqs + s.slots);
   return s;

@@ -75,7 +75,7 @@ __device__ __forceinline__ bool find_part(const PagedAttentionParams& p, LaneLen
     total += lane_tiles(p, lengths);
   }
   total = bcast_i(wave_scan(total), kWave - 1);
-  const int most = paged_part_most(total, p.slots, paged_least(total, p.few));
+  const int most = paged_part_most(total - p.cache.seqs, p.slots, paged_least(total, p.few));
   int before = 0;
   for (int s0 = 0; s0 < p.cache.seqs; s0 += kWave) {
     if (p.cache.seqs > kWave) lengths.load(p.cache, s0);

@@ -23,14 +23,14 @@ constexpr int kPagedTile = 128;   // tokens
 
 IEX_HD int paged_tiles(int tokens) { return tokens <= kPagedTile ? 1 : tokens / kPagedTile + (tokens % kPagedTile != 0); }
 
-// Tiles that a part has at most, where `total` tiles (of all sequences, one block of heads) go to about `slots` workgroups.  The
-// parts of all sequences are at most `slots` more than there are sequences: one has one more than whole parts fit into it.
-IEX_HD int paged_part_most(int total, int slots, int least) {
+// Tiles that a part has at most, where `beyond` tiles (of all sequences, one block of heads, beyond the first of each) go to `slots`
+// workgroups.  The parts of all sequences are at most `slots` more than there are sequences: t tiles are 1 + (t - 1) / most parts at most.
+IEX_HD int paged_part_most(int beyond, int slots, int least) {
   if (slots == 0) return 1 << 30;
-  const int even = total / slots + (total % slots != 0);
+  const int even = beyond / slots + (beyond % slots != 0);
   return even > least ? even : least;
 }
-// The `least` above: one tile where all of them (at most `few`) can have a workgroup each, else two.
+// The `least` above, of all tiles: one where each (at most `few`) can have a workgroup, else two.
 IEX_HD int paged_least(int total, int few) { return total <= few ? 1 : 2; }
 IEX_HD int paged_parts(int tiles, int most) { return tiles <= most ? 1 : tiles / most + (tiles % most != 0); }
 // The first tile of a part (of part number `parts`: the end).
