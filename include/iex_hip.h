@@ -498,7 +498,8 @@ int iex_paged_attention(const iex_paged_cache* cache, int heads, const void* q, 
  * sequence uses, then by score = sum over the group's heads and the features of max(q lo, q hi), summed in 64 bits and rounded
  * once to 32 (where none of the group's queries is positive, an infinite largest key adds nothing, and where none is negative, an infinite
  * smallest one; keys of 65504 that e4m3 rows store as 65536 have an infinite bound in fp16); ties go to the lower page, a NaN score comes first,
- * pages outside the cache are not selected.  Reads cache->bounds, not keys and values (may be null).  workspace: iex_select_pages_workspace_bytes, 256-byte aligned. */
+ * pages outside the cache are not selected.  Reads cache->bounds, not keys and values (may be null).  seqs * kv_heads
+ * below 2^22, in tables of more than 12288 pages below 65536.  workspace: iex_select_pages_workspace_bytes, 256-byte aligned. */
 size_t iex_select_pages_workspace_bytes(const iex_paged_cache* cache);
 int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, int count, int first,
                      int last, int* out, void* workspace, size_t workspace_bytes, void* stream);

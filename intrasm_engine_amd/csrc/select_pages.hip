@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
 // One launch where the scores are few (a row's pages on one CU: 256 9.1 us against 10.3, 512 11.1 against 9.9, 2048 31 against 13) or rows
 // enough for the chip (256 of 1024 28.1 against 31.8, 128 of 1024 21.3 against 20.1).
 bool one_launch(const iex_paged_cache& c) {
-  return c.table_width <= kSelectKept && (c.table_width <= 256 || c.seqs * c.kv_heads >= 256);
+  return c.table_width <= kSelectKept && (c.table_width <= 256 || (long long)c.seqs * c.kv_heads >= 256);
 }
 
 template <bool BF16, int D>
@@ -347,7 +347,8 @@ extern "C" int iex_select_pages(const iex_paged_cache* cache, int heads, const v
   if (cache->seqs == 0 || cache->kv_heads == 0) return 0;
   IEX_REQUIRE((heads == 0 || (q && q_strides)) && out && (cache->bounds || cache->pages == 0), IEX_ERR_BAD_ARGUMENT, "select_pages: null pointer argument");
   IEX_REQUIRE(aligned(q, 2) && aligned(out, 4) && aligned(cache->bounds, 16), IEX_ERR_UNSUPPORTED, "select_pages: operands must be aligned");
-  IEX_REQUIRE((long long)cache->seqs * cache->kv_heads < 65536, IEX_ERR_TOO_LARGE, "select_pages: too many sequences or heads");
+  // (2^32 threads a launch; scores in a launch of their own have a row in the grid's second dimension)
+  IEX_REQUIRE((long long)cache->seqs * cache->kv_heads < (one_launch(*cache) ? 1 << 22 : 65536), IEX_ERR_TOO_LARGE, "select_pages: too many sequences or heads");
   const size_t need = iex_select_pages_workspace_bytes(cache);
   IEX_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), IEX_ERR_BAD_ARGUMENT,
               "select_pages: needs a 256-byte aligned workspace of %zu bytes", need);

@@ -82,3 +82,24 @@ def test_a_key_that_eight_bits_round_past_fp16(dev):
         assert torch.equal(cache.select(q, table, lengths, 4, 0, 0).cpu(), by_definition(plain, q, 4, 0, 0))
     q[:, :, 9] = -0.001
     assert not (cache.select(q, table, lengths, 4, 0, 0) == 5).any()
+
+
+def test_many_rows(dev):
+    """More sequences and key heads than a launch has in its second dimension, where a workgroup selects a row."""
+    seqs, kv_heads, dim, page = 4100, 16, 64, 16
+    pages = 50
+    gen = torch.Generator(device=dev).manual_seed(3)
+    bounds = torch.randn(pages, kv_heads, 2, dim, generator=gen, device=dev).sort(2)[0].half()
+    table = torch.randint(0, pages, (seqs, 6), generator=gen, device=dev, dtype=torch.int32)
+    lengths = torch.randint(0, 6 * page + 1, (seqs,), generator=gen, device=dev, dtype=torch.int32)
+    q = torch.randn(seqs, kv_heads, dim, generator=gen, device=dev).half()
+    got = torch.ops.iex_ops.select_pages(q, bounds, table, lengths, page, 2, 0, 1)
+    assert _lib.last_kernels().startswith("page_select_kernel<f16, 64>")
+    b = bounds[table.long()].double()                                               # (seqs, 6, kv_heads, 2, dim)
+    score = torch.maximum(q.double()[:, None] * b[:, :, :, 0], q.double()[:, None] * b[:, :, :, 1]).sum(-1).float().transpose(1, 2)
+    used = (-(-lengths // page)).long()[:, None, None]
+    number = torch.arange(6, device=dev)
+    score = torch.where(number < used, torch.where(number == used - 1, math.inf, score), -math.inf)
+    best = torch.sort(score, dim=-1, descending=True, stable=True)[1][..., :2]
+    best = torch.where(best < used, best, 6).sort(-1)[0]
+    assert torch.equal(got.long(), torch.where(best < 6, best, -1))
