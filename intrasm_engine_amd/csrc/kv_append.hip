@@ -25,7 +25,7 @@ int launch(const AppendParams& p, bool rows, hipStream_t s) {
   const dim3 grid((unsigned)append_most_spans(p.tokens, p.cache.seqs, append_span(1 << p.cache.page_shift)),
                   (p.bounds ? kv_heads : kv_groups) + kv_groups + ceil_div(p.heads, p.per_group));
   const int lds = (rows ? 0 : kColumnTokens * D * 2) + (p.bounds ? per_step * D * 4 : 0);
-  note_kernel("%s<%s, %d, %s>", rows ? "kv_append_kernel" : "kv_append_columns_kernel", type, D, stored);
+  note_kernel("%s<%s, %d, %s> (%d heads a workgroup)", rows ? "kv_append_kernel" : "kv_append_columns_kernel", type, D, stored, p.per_group);
   if (!rows) hipLaunchKernelGGL((kv_append_columns_kernel<BF16, D, E8, INTERLEAVED>), grid, dim3(256), lds, s, p);
   else if (p.per_group == 1) hipLaunchKernelGGL((kv_append_kernel<BF16, D, E8, INTERLEAVED, 1>), grid, dim3(256), lds, s, p);
   else hipLaunchKernelGGL((kv_append_kernel<BF16, D, E8, INTERLEAVED, 4>), grid, dim3(256), lds, s, p);
