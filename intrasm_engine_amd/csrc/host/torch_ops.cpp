@@ -156,12 +156,18 @@ void set_mask_tables(const Tensor& q, const Tensor& row_offsets, const Tensor& c
 }
 
 std::optional<Known> note_of(const Tensor& row_offsets, const Tensor& column_indices, int64_t k) {
-  std::shared_lock lock(notes_mutex);
-  const Note* found = find_note(row_offsets, column_indices, k);
-  if (!found) return {};
-  const Note& n = *found;
-  Known known{n.status, n.has_histogram, n.histogram, n.dense_share, Tensor(), n.tables_stream};
-  if (auto alive = n.tables.lock()) known.tables = Tensor(std::move(alive));
+  std::optional<Known> known;
+  Weak tables = weak_of({});
+  {
+    std::shared_lock lock(notes_mutex);
+    const Note* n = find_note(row_offsets, column_indices, k);
+    if (!n) return {};
+    known = Known{n->status, n->has_histogram, n->histogram, n->dense_share, Tensor(), n->tables_stream};
+    tables = n->tables;
+  }
+  // (a tensor that only Python holds is taken with the interpreter's lock, and those who have that lock wait for notes_mutex: never the one
+  // with the other in hand)
+  if (auto alive = tables.lock()) known->tables = Tensor(std::move(alive));
   return known;
 }
 
