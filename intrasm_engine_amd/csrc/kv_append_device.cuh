@@ -12,9 +12,9 @@
 // by the one workgroup that has a page's new tokens, from LDS; a page that had tokens before keeps theirs.
 //
 // What bounds it: prompts by memory (each feature is read and written once), a step of generation by latency: lengths -> table
-// -> store is the longest chain of loads.  Measured: 16 prompts of 512 tokens, 3 x 32 heads of 128, feature-major 81 us = 5.0 TB/s read
-// and written; 23 of 3 .. 5001 tokens, 32 + 2 x 8 heads, into e4m3 with bounds 97 - 100 us = 4.0 (waiting for a row's maximum, vector
-// units 36 %); a step of one sequence of 3 x 32 heads 3.0 us, of 64 of 32 + 2 x 8 heads with bounds 4.5.
+// -> store is the longest chain of loads.  Measured: 16 prompts of 512 tokens, 3 x 32 heads of 128, feature-major 79 us = 5.1 TB/s read
+// and written; 23 of 3 .. 5001 tokens, 32 + 2 x 8 heads, into e4m3 with bounds 96 us = 4.2 (waiting for a row's maximum, vector
+// units 36 %); a step of one sequence of 3 x 32 heads 3.0 us, of 64 of 32 + 2 x 8 heads with bounds 4.2.
 #pragma once
 #include "paged_cache_device.cuh"
 

@@ -10,18 +10,19 @@ namespace {
 // Workgroups of four wavefronts that are resident at once: by their registers two to four on each of the 256 CUs.
 int resident(int head_dim) { return 256 * paged_simd_waves(head_dim); }
 
-// Rows of up to this many tiles stay whole, and there is no second launch: 32 x 700 tokens of 128 12.8 us, cut 14.5; 16 x 32 rows of
-// 600 .. 1023 39.7 and 44; 32 x 2000, the other side, 16 cut and 24 whole.
+// Rows of up to this many tiles stay whole, and there is no second launch: 128 rows of 700 tokens of 128 12.0 us, cut 17.0; 512 of 600 .. 1023
+// 37.4 and 43; 32 of 2000, the other side, 13.2 cut and 22.8 whole.  (Where all tiles of shorter rows could have a workgroup each, cutting would be
+// the faster, which the rule leaves: 32 of 700 11.1 whole and 10.0 cut.)
 constexpr int kWholeTiles = 8;
-// Whole rows go to eight wavefronts each where four would leave CUs without work: 128 rows of 700 13.1 us by eight, 17.5 by four; 512 of
-// 500 30.5 and 24.8.
+// Whole rows go to eight wavefronts each where four would leave CUs without work: 128 rows of 700 12.0 us by eight, 16.0 by four; 512 of
+// 500 28.1 and 23.7.
 constexpr int kWideRows = 512;
 // Rows of up to this many tokens have a wavefront each: 4096 rows of 12 tokens in tables of 64 28.6 us by four, 14.3 by one; of 64 33.3 and
 // 24.9; of 128, the other side, 47.5 and 51.5.
 constexpr int kNarrow = 64;
-// Parts: one round of resident workgroups where rows are few (131071 tokens, 8 rows: 92.8 us, two rounds 99.8), two where rows of unequal
-// lengths come anyway (512 rows of 4000 .. 16384, e4m3: 221 one, 205.7 two, 206.3 three, 207.7 four; 2048 of 1 .. 4096, heads of 64: 65.7,
-// 62.4, 62.6, 63.2).
+// Parts: one round of resident workgroups where rows are few (131071 tokens, 8 rows: 92.5 us, two rounds 101.6), two where rows of unequal
+// lengths come anyway (512 rows of 4000 .. 16384, e4m3: 236 one, 206.5 two; 2048 of 1 .. 4096, heads of 64: 65.5 and 61.9; three and four rounds
+// as two).
 constexpr int kTwoRounds = 256;
 // Tiles have a workgroup each, if that makes at most this many, one on each CU: a sequence of 4000 tokens, 8 key heads of 64 (256 workgroups)
 // 12.0 us, by two tiles 13.6; 64 listed pages of 64 (256) 10.3 and 11.9; 8192 tokens (512), the other side, 16.4 and 14.8.

@@ -16,9 +16,9 @@
 // so a replayed graph follows them); one, four or eight wavefronts take its tiles in turn and meet in LDS, parts meet in a second launch.
 // An 8-bit cache (e4m3) widens to 16 bits in registers; its powers of two go to the scores and the probabilities.
 //
-// Measured: 131071 tokens, 8 key heads of 128, 64 query heads, bf16 87 us = 6.3 TB/s, its join 6; 64 sequences of 4000 .. 16384 in e4m3
-// 201 us = 6.0 TB/s; 16 x 600 .. 1023, 32 heads 40 us = 5.3; 128 x 1 .. 4096, 16 heads of 64, pages of 16 55 us = 4.9 (vector units busy
-// 10 - 32 %, matrix cores 4 - 11 %; profiles/paged_cache_kernel_trace_and_counters.txt).
+// Measured: 131071 tokens, 8 key heads of 128, 64 query heads, bf16 88 us = 6.2 TB/s, its join 6; 64 sequences of 4000 .. 16384 in e4m3
+// 200 us = 6.0 TB/s; 16 x 600 .. 1023, 32 heads 40 us = 5.3; 16 x 1007 .. 1693, 16 heads of 256 63.5 us = 5.7; 128 x 1 .. 4096, 16 heads of 64,
+// pages of 16 55 us = 4.9 (vector units busy 9 - 37 %, matrix cores 4 - 14 %; profiles/paged_cache_kernel_trace_and_counters.txt).
 #pragma once
 #include "paged_cache_device.cuh"
 

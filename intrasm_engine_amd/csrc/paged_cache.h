@@ -1,7 +1,7 @@
 // Which tokens, pages and rows the kernels of the paged cache (kv_append, paged_attention, select_pages) touch: how new
 // tokens are dealt to workgroups, how a cache's length is split, where a page lies.  Plain C++, so that a program on the host
-// can walk every access of a launch (tests/paged_cache_check.cpp).  Lengths, offsets, tables and lists are device data that
-// nobody has checked: everything here keeps inside the arrays whatever they hold.
+// can walk what it gives (tests/paged_cache_check.cpp, tests/paged_parts_check.cpp); the addresses that kernels make of it are theirs.  Lengths,
+// offsets, tables and lists are device data that nobody has checked: everything here keeps inside the arrays whatever they hold.
 #pragma once
 #include <cstddef>
 

@@ -11,8 +11,9 @@
 // does both for a sequence and key head, its scores in LDS, where that keeps the chip busy or the scores are few; else the scores
 // come from a launch of their own.
 //
-// Measured (heads of 128): scores of 8 x 90000 .. 131072 tokens in pages of 32, 8 key heads 25 us = 4.5 TB/s (64-bit conversions, 16 clocks
-// each, would allow 10), selection 10.6; 32 x up to 1024 pages, 8 key heads, in one launch 19 us = 1.9 TB/s, 68 % of it waiting.
+// Measured (heads of 128): scores of 8 x 90000 .. 131072 tokens in pages of 32, 8 key heads 25 us = 4.5 TB/s (46 % waiting, 44 % for issue: 64-bit
+// conversions take 16 clocks each, which alone would allow 10), selection 10.4; 32 x up to 1024 pages, 8 key heads, in one launch 19 us = 1.9 TB/s,
+// 68 % of it waiting (a workgroup a row: the longest set the time).
 #include "paged_cache_host.h"
 
 namespace iex {
