@@ -51,6 +51,7 @@ class CUDAGraphCaptureNotifier:
     def __init__(self):
         self._device = None
         self._pool = None
+        self._begun: dict[tuple, int] = {}      # captures into each pool: the allocator counts them, and wants as many releases
         self._capture_stream = None
         self._active = False
 
@@ -70,6 +71,7 @@ class CUDAGraphCaptureNotifier:
         self._capture_stream = stream
         # before the capture starts, as in the reference (pybind.cu:221-237)
         torch._C._cuda_beginAllocateCurrentStreamToPool(self._device, self._pool)
+        self._begun[self._pool] = self._begun.get(self._pool, 0) + 1
         self._active = True
 
     def assert_capture_has_begun(self):
@@ -97,10 +99,11 @@ class CUDAGraphCaptureNotifier:
         return self._pool
 
     def release_pool(self):
-        """Let the allocator reclaim the capture's pool once its tensors are gone."""
-        if self._pool is not None and self._device is not None:
-            torch._C._cuda_releasePool(self._device, self._pool)
-            self._pool = None
+        """Let the allocator reclaim the captures' pools once their tensors are gone."""
+        begun, self._begun, self._pool = self._begun, {}, None
+        for pool, captures in begun.items():
+            for _ in range(captures):
+                torch._C._cuda_releasePool(self._device, pool)
 
     def __del__(self):
         try:
