@@ -10,7 +10,7 @@
 //                  if group g's share of the sum over tokens is those very tokens.  A lane loads 16 bytes (features c * 8 ..) of
 //                  each of them; one byte permute per dword pairs tokens, and operand j has features c * 8 + j as its rows.
 // The running maximum and sum are per query; sums follow a new maximum only where some score has passed it.  Probabilities go
-// in as 16-bit parts, three of bf16 or two of fp16, so that nothing is lost: matrix cores idle otherwise.
+// in as 16-bit parts, three of bf16 (all of their 24 bits) or two of fp16 (22): matrix cores idle otherwise.
 //
 // A sequence is split over its length into parts, a workgroup each (paged_cache.h: parts are cut from the lengths on the device,
 // so a replayed graph follows them); one, four or eight wavefronts take its tiles in turn and meet in LDS, parts meet in a second launch.
