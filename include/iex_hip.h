@@ -493,6 +493,16 @@ int iex_paged_attention(const iex_paged_cache* cache, int heads, const void* q, 
                         const int* listed, int count, void* out, const long long* out_strides, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* iex_paged_attention over every page, and weights[s, g, t] (seqs, kv_heads, table_width * page_size; fp32, 16-byte aligned) grows by what token t got:
+ * the sum over the query heads of key head g of their softmax weights, each exp(scale * (score - maximum)) / sum in 32 bits, added up in the order
+ * of the heads and then to what is there (no atomics: the same call gives the same bits).  Tokens behind a sequence's length and in pages given back
+ * keep what they have.  Needs its workspace always: it holds a score in 32 bits for every query head and token of the table.
+ * Up to 4096 query heads of a key head. */
+size_t iex_paged_attention_accumulate_workspace_bytes(const iex_paged_cache* cache, int heads);
+int iex_paged_attention_accumulate(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, float scale,
+                                   float* weights, void* out, const long long* out_strides, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
 /* out: (seqs, kv_heads, count), the `count` pages of every sequence's table whose keys can score highest with the query heads of
  * a key head, in ascending order, -1 behind them where there are fewer: the first `first` and last `last` pages that the
  * sequence uses, then by score = sum over the group's heads and the features of max(q lo, q hi), summed in 64 bits and rounded

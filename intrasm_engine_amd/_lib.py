@@ -92,6 +92,8 @@ SIGNATURES = {
     "iex_kv_append": (_i, [_cache, _i, _vp, _i, _vp, _strides, _vp, _strides, _vp, _strides, _vp, _strides, _vp, _i, _i, _i, _vp]),
     "iex_paged_attention_workspace_bytes": (_c.c_size_t, [_cache, _i, _i]),
     "iex_paged_attention": (_i, [_cache, _i, _vp, _strides, _f, _vp, _i, _vp, _strides, _vp, _c.c_size_t, _vp]),
+    "iex_paged_attention_accumulate_workspace_bytes": (_c.c_size_t, [_cache, _i]),
+    "iex_paged_attention_accumulate": (_i, [_cache, _i, _vp, _strides, _f, _vp, _vp, _strides, _vp, _c.c_size_t, _vp]),
     "iex_select_pages_workspace_bytes": (_c.c_size_t, [_cache]),
     "iex_select_pages": (_i, [_cache, _i, _vp, _strides, _i, _i, _i, _vp, _vp, _c.c_size_t, _vp]),
     "iex_csr_softmax": (_i, [_i, _i, _i, _vp, _vp, _vp, _f, _vp, _i]),

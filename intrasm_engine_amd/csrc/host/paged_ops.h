@@ -151,6 +151,37 @@ Tensor paged_attention(const Tensor& q, const Tensor& keys, const Tensor& values
   return out;
 }
 
+// What the tokens of every sequence and key head got of attention: (sequences, kv_heads, tokens of a table).
+void check_weights(const Tensor& weights, const Tensor& with, const iex_paged_cache& c, const char* op) {
+  check_tensor(weights, with, 3, op, "weights");
+  check_no_gradient(weights, op);
+  TORCH_CHECK(weights.scalar_type() == at::kFloat && weights.is_contiguous() && weights.size(0) == c.seqs && weights.size(1) == c.kv_heads &&
+                  weights.size(2) == (int64_t)c.table_width * c.page_size,
+              op, ": weights must be contiguous float32 (sequences, kv_heads, tokens of a table)");
+}
+
+Tensor paged_attention_accumulate(const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& page_table, const Tensor& lengths, const Tensor& weights,
+                                  std::optional<double> scale, const std::optional<Tensor>& key_exponents, const std::optional<Tensor>& value_exponents) {
+  constexpr const char* op = "paged_attention_accumulate_";
+  check_tensor(q, q, 3, op, "q");
+  check_no_gradient(q, op);
+  const iex_paged_cache c = paged_cache(op, q, keys, values, page_table, lengths, {}, key_exponents, value_exponents);
+  TORCH_CHECK(q.size(0) == c.seqs, op, ": one token per sequence (", q.size(0), ", ", c.seqs, ")");
+  check_weights(weights, q, c, op);
+  const c10::DeviceGuard guard(q.device());
+  if (c.pages == 0) return at::zeros_like(q);   // nothing to attend to
+  const Tensor out = at::empty_like(q);
+  const int heads = as_int(q.size(1), op);
+  const Strides qs(q), os(out);
+  const size_t bytes = iex_paged_attention_accumulate_workspace_bytes(&c, heads);
+  const Tensor ws = workspace(bytes, q);
+  check(iex_paged_attention_accumulate(&c, heads, q.const_data_ptr(), qs.of, (float)scale.value_or(1.0 / std::sqrt((double)q.size(2))),
+                                       const_cast<float*>(weights.const_data_ptr<float>()), out.data_ptr(), os.of, ws.defined() ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+        op);
+  changed(weights);
+  return out;
+}
+
 Tensor select_pages(const Tensor& q, const Tensor& bounds, const Tensor& page_table, const Tensor& lengths, int64_t page_size, int64_t count, int64_t first,
                     int64_t last) {
   constexpr const char* op = "select_pages";

@@ -741,6 +741,9 @@ TORCH_LIBRARY(iex_ops, lib) {
   define("paged_attention", "(Tensor q, Tensor keys, Tensor values, Tensor page_table, Tensor lengths, float? scale=None, Tensor? pages=None, "
          "Tensor? key_exponents=None, Tensor? value_exponents=None) -> Tensor",
          TORCH_FN(paged_attention));
+  define("paged_attention_accumulate_", "(Tensor q, Tensor keys, Tensor values, Tensor page_table, Tensor lengths, Tensor(a!) weights, float? scale=None, "
+         "Tensor? key_exponents=None, Tensor? value_exponents=None) -> Tensor",
+         TORCH_FN(paged_attention_accumulate));
   define("select_pages", "(Tensor q, Tensor bounds, Tensor page_table, Tensor lengths, int page_size, int count, int first=1, int last=1) -> Tensor",
          TORCH_FN(select_pages));
 }

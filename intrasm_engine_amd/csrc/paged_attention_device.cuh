@@ -39,7 +39,43 @@ struct PagedAttentionParams {
   float scale_log2;
   float* partial;   // per part: group_rows x D sums, then per part group_rows maxima and sums
   float* stats;
+  // attention that keeps account (WEIGH below)
+  float* weights;     // (seqs, kv_heads, tokens of a table)
+  float* scores;      // (seqs, heads, tokens of a table)
+  float* row_stats;   // per sequence and query head maximum and sum, of rows of one part
+  int at_once;        // rows are whole and their queries together: no second launch
 };
+
+__device__ __forceinline__ size_t table_tokens(const PagedParams& c) { return (size_t)c.table_width << c.page_shift; }
+
+// What stands in the place of the score of a token that is not attended to: a NaN that no product of 16-bit or 8-bit operands has, so that a row whose
+// scores are NaN or infinite leaves no trace in what it does not attend to.
+constexpr unsigned kNoScore = 0xFFFFFFFFu;
+
+// Four tokens' scores of one query as weights: exp2((score - maximum) * scale) / sum.
+struct QueryWeights {
+  float shift, share;
+  __device__ __forceinline__ QueryWeights(float top, float sum, float scale_log2) : shift(sum == -1.f ? 0.f : -top * scale_log2), share(sum == -1.f ? 0.f : 1.f / sum) {}
+  __device__ __forceinline__ QueryWeights(float2 both) : shift(both.x), share(both.y) {}
+  __device__ __forceinline__ void add(f32x4& to, const f32x4& score, float scale_log2) const {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float more = fmaf(__builtin_amdgcn_exp2f(fmaf(score[r], scale_log2, shift)), share, to[r]);
+      to[r] = __float_as_uint(score[r]) == kNoScore ? to[r] : more;
+    }
+  }
+};
+// `got` more for tokens t .. t + 3 of a row of `length` (the others are not touched).
+__device__ __forceinline__ void add_weights(float* weights, int t, int length, const f32x4& got) {
+  if (t + 4 <= length) {
+    f32x4 now = *reinterpret_cast<f32x4*>(weights + t);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) now[r] += got[r];
+    *reinterpret_cast<f32x4*>(weights + t) = now;
+  } else {
+    for (int r = 0; t + r < length; ++r) weights[t + r] += got[r];
+  }
+}
 
 // Tokens that a sequence of `length` tokens attends to at most.
 __device__ __forceinline__ int row_tokens(const PagedAttentionParams& p, int length) { return p.count && length ? p.count << p.cache.page_shift : length; }
@@ -140,7 +176,9 @@ constexpr int paged_simd_waves(int head_dim) { return head_dim == 256 ? 2 : head
 constexpr int paged_sum_gap(int head_dim) { return head_dim == 64 ? 0 : 16; }
 constexpr int paged_sum_pitch(int head_dim) { return head_dim + 3 * paged_sum_gap(head_dim) + 1; }
 
-template <bool BF16, int D, bool E8, int WAVES>
+// WEIGH: scores are left behind too, 4 bytes a token and query head, and become weights when the row's maximum and sum are known: here, by the
+// one workgroup that has the row, or in paged_account_kernel.
+template <bool BF16, int D, bool E8, int WAVES, bool WEIGH>
 __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attention_kernel(PagedAttentionParams p) {
   typedef unsigned short u16;
   constexpr int ES = E8 ? 1 : 2;               // bytes of an element
@@ -330,7 +368,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
   };
   constexpr int PARTS = kWeightParts<PV_BF16>;
   u32x4 weight[SUB / 2][PARTS];
-  auto weights = [&](const Where& w) {
+  auto weights = [&](const Where& w, int t) {
     int valid = 0;
 #pragma unroll
     for (int a = 0; a < SUB; ++a) valid += w.valid[a];
@@ -346,6 +384,21 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
             for (int h = 0; h < VWORDS; ++h) value[a][r][h] = VWord{};
             if constexpr (E8) ve[a] = (ve[a] & ~(0xFFu << (r * 8))) | 0x7Fu << (r * 8);
           }
+    }
+    if constexpr (WEIGH) {
+      if (col < rows) {
+        float* to = p.scores + ((size_t)seq * p.heads + kv_head * p.group + group_tile * 16 + col) * table_tokens(cache) + t + g * 4;
+#pragma unroll
+        for (int a = 0; a < SUB; ++a)
+          if (t + a * 16 < end) {
+            f32x4 left = s[a];
+            if (w.valid[a] != 16) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) left[r] = g * 4 + r >= w.valid[a] ? __uint_as_float(kNoScore) : left[r];
+            }
+            *reinterpret_cast<f32x4*>(to + a * 16) = left;
+          }
+      }
     }
     float m = s[0][0];
 #pragma unroll
@@ -418,13 +471,13 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
       const Where next = find(t + STEP);
       scores();
       load_keys(next);
-      weights(now);
+      weights(now, t);
       weigh_values();
       now = next;
     }
     load_values(now);
     scores();
-    weights(now);
+    weights(now, t);
     weigh_values();
   }
 
@@ -436,6 +489,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
   constexpr int PITCH = paged_sum_pitch(D), GAP = paged_sum_gap(D);
   float* sums = smem;                              // [wave][row][PITCH]
   float* tops = smem + WAVES * rows * PITCH;       // [wave][row] (maximum, sum)
+  float2* shares = reinterpret_cast<float2*>(smem + (WAVES * rows * (PITCH + 2) + 1) / 2 * 2);   // WEIGH: [row]
   if (col < rows) {
     float* mine = sums + (wave * rows + col) * PITCH + g * (D / 4 + GAP);
 #pragma unroll
@@ -467,10 +521,27 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
     if (parts == 1) {
       const int head = kv_head * p.group + group_tile * 16 + row;
       p.out[seq * p.out_strides[0] + head * p.out_strides[1] + d * p.out_strides[2]] = f32_to_16(any ? acc / (all * up) : 0.f, BF16);
+      if (WEIGH && d == 0 && !p.at_once) *reinterpret_cast<float2*>(p.row_stats + ((size_t)seq * p.heads + head) * 2) = float2{m, any ? all : -1.f};
+      if (WEIGH && d == 0 && p.at_once) {
+        const QueryWeights mine(m, any ? all : -1.f, p.scale_log2);
+        shares[row] = float2{mine.shift, mine.share};
+      }
     } else {
       const size_t to = (size_t)blockIdx.x * p.pitch + row;
       p.partial[to * D + d] = acc;
       if (d == 0) p.stats[to * 2] = m, p.stats[to * 2 + 1] = any ? all : -1.f;
+    }
+  }
+  if constexpr (WEIGH) {
+    if (!p.at_once) return;
+    __syncthreads();   // (the wavefronts' scores are there too)
+    const float* from = p.scores + ((size_t)seq * p.heads + kv_head * p.group) * table_tokens(cache);
+    float* to = p.weights + ((size_t)seq * cache.kv_heads + kv_head) * table_tokens(cache);
+    for (int t = threadIdx.x * 4; t < length; t += WAVES * 256) {
+      f32x4 got = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int row = 0; row < rows; ++row) QueryWeights(shares[row]).add(got, *reinterpret_cast<const f32x4*>(from + row * table_tokens(cache) + t), p.scale_log2);
+      add_weights(to, t, length, got);
     }
   }
 }
@@ -478,11 +549,11 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
 // Parts of a row into its result, a workgroup per sequence and query head: the parts' weights first, 256 at a time, then
 // 256 / (D / 4) parts side by side, a thread four features; they meet in LDS.
 template <bool BF16, int D, bool E8>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p) {
+__device__ __forceinline__ void join_parts(const PagedAttentionParams& p, int seq, int head) {
   constexpr int LANES = D / 4, SIDE = 256 / LANES;   // threads of a row; parts side by side
   __shared__ float4 accs[SIDE][LANES];
   __shared__ float weights[256], tops[4], sums[4];
-  const int seq = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+  const int tid = threadIdx.x;
   const int kv_head = head / p.group, in_group = head % p.group;
   LaneLengths lengths;
   int found, first = seq * p.fixed, number = p.fixed, tiles;
@@ -542,6 +613,62 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p)
 #pragma unroll
   for (int i = 0; i < SIDE; ++i) x += reinterpret_cast<const float*>(accs[i])[tid];
   p.out[seq * p.out_strides[0] + head * p.out_strides[1] + tid * p.out_strides[2]] = f32_to_16(any ? x / (total * up) : 0.f, BF16);
+}
+template <bool BF16, int D, bool E8>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p) {
+  join_parts<BF16, D, E8>(p, blockIdx.x, blockIdx.y);
+}
+
+// The second launch of attention that keeps account: workgroups `joins` and on add the weights of 1024 tokens at a time of a sequence and key
+// head, `side` workgroups taking turns; those before join parts (of rows that were cut: with the weights in one launch, since neither waits for the
+// other; each works out the rows' maxima and sums from the parts').
+constexpr int kAccountTokens = 1024;
+template <bool BF16, int D, bool E8>
+__global__ __launch_bounds__(256) void paged_account_kernel(PagedAttentionParams p, int joins, int side) {
+  extern __shared__ __align__(16) float2 shares[];   // of the group's queries
+  if ((int)blockIdx.x < joins) {
+    join_parts<BF16, D, E8>(p, blockIdx.x / p.heads, blockIdx.x % p.heads);
+    return;
+  }
+  const PagedParams& cache = p.cache;
+  const int item = blockIdx.x - joins, row = item / side, seq = row / cache.kv_heads, kv_head = row % cache.kv_heads, wave = uniform(threadIdx.x >> 6), lane = lane_id();
+  const int length = cached_length(cache.lengths[seq], cache.table_width, 1 << cache.page_shift);
+  int t = item % side * kAccountTokens + threadIdx.x * 4;
+  if (item % side * kAccountTokens >= length) return;
+  LaneLengths lengths;
+  int found, first = seq, number = 1, tiles;
+  if (!p.fixed) find_part(p, lengths, [&](int s, int, int) { return s == seq; }, found, first, number, tiles);
+  for (int i = wave; i < p.group; i += 4) {
+    const int head = kv_head * p.group + i;
+    float top = -INFINITY, sum = -1.f;
+    if (number == 1) {
+      const float2 both = *reinterpret_cast<const float2*>(p.row_stats + ((size_t)seq * p.heads + head) * 2);
+      top = both.x, sum = both.y;
+    } else {
+      const int block = kv_head * p.group_tiles + i / 16;
+      auto part = [&](int n) { return *reinterpret_cast<const float2*>(p.stats + (((size_t)(first + n) * p.blocks + block) * p.pitch + i % 16) * 2); };
+      bool counts = false;
+      for (int n = lane; n < number; n += kWave)
+        if (const float2 both = part(n); both.y != -1.f) counts = true, top = fmaxf(top, both.x);   // (NaN is a sum)
+      top = wave_max(top);
+      float mine = 0.f;
+      for (int n = lane; n < number; n += kWave)
+        if (const float2 both = part(n); both.y != -1.f) mine += both.x == top ? both.y : __builtin_amdgcn_exp2f((both.x - top) * p.scale_log2) * both.y;
+      sum = wave_sum(mine);
+      if (!__ballot(counts)) sum = -1.f;
+    }
+    const QueryWeights its(top, sum, p.scale_log2);
+    if (lane == 0) shares[i] = float2{its.shift, its.share};
+  }
+  __syncthreads();
+  const float* from = p.scores + ((size_t)seq * p.heads + kv_head * p.group) * table_tokens(cache);
+  float* to = p.weights + ((size_t)seq * cache.kv_heads + kv_head) * table_tokens(cache);
+  for (; t < length; t += side * kAccountTokens) {
+    f32x4 got = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int i = 0; i < p.group; ++i) QueryWeights(shares[i]).add(got, *reinterpret_cast<const f32x4*>(from + i * table_tokens(cache) + t), p.scale_log2);
+    add_weights(to, t, length, got);
+  }
 }
 
 }  // namespace iex
