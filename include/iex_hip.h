@@ -514,6 +514,19 @@ size_t iex_select_pages_workspace_bytes(const iex_paged_cache* cache);
 int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, const long long* q_strides, int count, int first,
                      int last, int* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Tokens that got least attention leave the cache.  A sequence of more than `keep` tokens (lengths[s], cut to what the table holds; lengths is
+ * cache->lengths) has `keep` of them afterwards, for every key head its own: the first `first`, the last `recent` and, of those between, the ones
+ * with the largest weights[s, g, t] (seqs, kv_heads, table_width * page_size; ties: the earlier token; a NaN is larger than all).  Their rows move, in order,
+ * to the sequence's first `keep` places, their weights with them; the weights of places behind are 0 then, lengths[s] is `keep`, bounds (if the
+ * cache has them) are those of the tokens that the pages then hold.  kept: (seqs, kv_heads, keep), where the tokens were, ascending.
+ * Other sequences stay as they are, kept has their tokens 0 .. lengths[s] - 1 and -1 behind them.  A sequence of more than `keep` tokens with pages
+ * given back among those it uses is passed over: nothing changes, kept is -1.  Rows move in place: a sequence that loses tokens must have its
+ * pages for itself (no other one reads right what it shares with it, and a page that two such sequences, or one twice, have holds what either wrote).
+ * workspace: iex_evict_tokens_workspace_bytes, 256-byte aligned. */
+size_t iex_evict_tokens_workspace_bytes(const iex_paged_cache* cache, int keep);
+int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, float* weights, int keep, int recent, int first, int* kept,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* In-place row-wise softmax over the stored entries of a CSR matrix:
  * values[z, j] = exp(scale*values[z, j] - max_row) / sum_row.  values is (batch, nnz).
  * The middle step of sparse attention between SDDMM and SpMM (no reference

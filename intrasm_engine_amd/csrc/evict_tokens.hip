@@ -1,0 +1,280 @@
+// Tokens of a paged cache that got least attention leave it.  Of a sequence of n > keep tokens every key head keeps the first `first`, the last `recent` and,
+// of those between, the ones with the largest accumulated weight (paged_account.hip), the earlier of two that are equal; they move, in order, to places
+// 0 .. keep - 1 of the sequence's own pages, their weights with them, and the sequence has `keep` tokens.
+//
+// Two launches.  The first, a workgroup a sequence and key head, finds the keep largest weights (select_device.cuh) and leaves the list of kept tokens, ascending.
+// The second moves rows, in place: chunk c of a list, up to `chunk` tokens, reads rows that others may be about to write.  The i-th kept token is
+// at place i or behind it, so what chunk c writes, places c * chunk and on, is only ever read by itself and by chunks before it (the list's stretch
+// with tokens there ends before its own); all of a chunk's rows are in registers before its first write, and it writes when the chunks before it that
+// read there, two at most, have said that theirs are too.  Chunks are drawn by ticket: the one that is waited for has been drawn before, by a workgroup that is
+// running and that waits for nobody before it has read, so every wait ends.
+//
+// What bounds it: memory, kept rows read and written once.
+#include "paged_cache_host.h"
+#include "select_device.cuh"
+
+namespace iex {
+namespace {
+
+struct EvictParams {
+  PagedParams cache;
+  int keep, first, recent, chunks;   // chunks of a list
+  int* lengths;
+  float* weights;      // (seqs, kv_heads, tokens of a table)
+  int* kept;           // (seqs, kv_heads, keep)
+  unsigned short* bounds;
+  // the workspace; rows are a sequence's key heads
+  int* tokens;         // (rows) tokens of a row that is cut, else 0
+  int* tickets;        // (rows) chunks drawn
+  int* flags;          // (rows, chunks) 1: read
+  int* before;         // (rows, chunks + 1) how many tokens before place i * chunk are kept
+  float* kept_weights; // (rows, keep)
+};
+
+constexpr int kEvictThreads = 1024, kEvictKept = 12288;   // ... whose weights fit in LDS
+
+// KEPT: the row's keys stay in LDS, else every round reads its weights again.
+template <bool KEPT>
+__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p, int chunk) {
+  extern __shared__ unsigned keys[];
+  const PagedParams& c = p.cache;
+  const int row = blockIdx.x, seq = row / c.kv_heads, tid = threadIdx.x;
+  const int length = cached_length(c.lengths[seq], c.table_width, 1 << c.page_shift);
+  int* const kept = p.kept + (size_t)row * p.keep;
+  if (length <= p.keep) {
+    for (int i = tid; i < p.keep; i += kEvictThreads) kept[i] = i < length ? i : -1;
+    if (tid == 0) p.tokens[row] = 0;
+    return;
+  }
+  // a sequence with pages given back has no place for what it keeps: passed over
+  bool gone = false;
+  for (int i = tid; i << c.page_shift < length; i += kEvictThreads) gone |= (unsigned)c.table[(size_t)seq * c.table_row + i] >= (unsigned)c.pages;
+  if (__syncthreads_or(gone)) {
+    for (int i = tid; i < p.keep; i += kEvictThreads) kept[i] = -1;
+    if (tid == 0) p.tokens[row] = 0;
+    return;
+  }
+  for (int i = tid; i < p.chunks; i += kEvictThreads) p.flags[(size_t)row * p.chunks + i] = 0;
+  if (tid == 0) p.tokens[row] = length, p.tickets[row] = 0;
+  const float* const weights = p.weights + (size_t)row * ((size_t)c.table_width << c.page_shift);
+  auto key_at = [&](int i) { return i < p.first || i >= length - p.recent ? kSelectAlways : select_key(__float_as_uint(weights[i])); };
+  if constexpr (KEPT) {
+    for (int i = tid; i < length; i += kEvictThreads) keys[i] = key_at(i);
+    __syncthreads();
+  }
+  int* const before = p.before + (size_t)row * (p.chunks + 1);
+  float* const moved = p.kept_weights + (size_t)row * p.keep;
+  select_largest<kEvictThreads>(
+      length, p.keep, [&](int i) { return KEPT ? keys[i] : key_at(i); },
+      [&](int to, int i) {
+        kept[to] = i;
+        moved[to] = weights[i];
+      },
+      [&](int i0, int taken) {
+        if (i0 % chunk == 0 && i0 / chunk <= p.chunks && lane_id() == 0) before[i0 / chunk] = taken;
+      });
+}
+
+// Tokens of a chunk: eight 16-byte loads of 256 threads, of keys and values.
+constexpr int evict_chunk(int row_bytes) { return 8 * 256 * 16 / (2 * row_bytes) < 64 ? 64 : 8 * 256 * 16 / (2 * row_bytes); }
+
+// ROW: bytes of a token's key or value of one head.
+template <int ROW, bool E8>
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
+  constexpr int T = evict_chunk(ROW), LANES = ROW / 16, LOADS = T * LANES / 256;   // tokens; 16-byte pieces of a row; loads of a thread, of keys and of values
+  const PagedParams& c = p.cache;
+  const int rows = c.seqs * c.kv_heads, row = blockIdx.x % rows, seq = row / c.kv_heads, head = row % c.kv_heads, tid = threadIdx.x;
+  const int length = p.tokens[row];
+  if (length == 0) return;
+  __shared__ int drawn;
+  __shared__ int from[T], to[T];   // rows before a token's in the cache, page by page: page << page_shift | slot
+  if (tid == 0) drawn = atomicAdd(p.tickets + row, 1);
+  __syncthreads();
+  const int chunk = drawn, first = chunk * T, count = min(T, p.keep - first);
+  const int* const kept = p.kept + (size_t)row * p.keep;
+  float* const weights = p.weights + (size_t)row * ((size_t)c.table_width << c.page_shift);
+  // the weights, which nobody reads here: those of the chunk's tokens, and this chunk's share of the zeros behind the kept ones
+  for (int i = tid; i < count; i += 256) weights[first + i] = p.kept_weights[(size_t)row * p.keep + first + i];
+  const int share = (length - p.keep + p.chunks - 1) / p.chunks;
+  for (int i = p.keep + chunk * share + tid; i < min(length, p.keep + (chunk + 1) * share); i += 256) weights[i] = 0.f;
+  if (head == 0 && chunk == 0 && tid == 0) p.lengths[seq] = p.keep;
+  if (kept[first + count - 1] == first + count - 1) return;   // all of them are where they belong
+
+  const int* const table = c.table + (size_t)seq * c.table_row;
+  for (int i = tid; i < T; i += 256) {   // (behind the last one: that one again)
+    const int t = first + min(i, count - 1), source = kept[t];
+    from[i] = table[source >> c.page_shift] << c.page_shift | (source & ((1 << c.page_shift) - 1));
+    to[i] = table[t >> c.page_shift] << c.page_shift | (t & ((1 << c.page_shift) - 1));
+  }
+  __syncthreads();
+  auto row_at = [&](int place, long long page_stride) {   // elements are bytes where E8, else two
+    const int page = place >> c.page_shift, slot = place & ((1 << c.page_shift) - 1);
+    return (page * page_stride) * (E8 ? 1 : 2) + ((long long)(head << c.page_shift) + slot) * ROW;
+  };
+  auto exponent_at = [&](int place) {
+    const int page = place >> c.page_shift, slot = place & ((1 << c.page_shift) - 1);
+    return (((size_t)page * c.kv_heads + head) << c.page_shift) + slot;
+  };
+  unsigned char* const keys = static_cast<unsigned char*>(const_cast<void*>(c.keys));
+  unsigned char* const values = static_cast<unsigned char*>(const_cast<void*>(c.values));
+  unsigned char* const key_exponents = const_cast<unsigned char*>(c.key_exponents);
+  unsigned char* const value_exponents = const_cast<unsigned char*>(c.value_exponents);
+  const int piece = tid % LANES * 16, line = tid / LANES;
+  u32x4 k[LOADS], v[LOADS];
+  unsigned char ke = 0, ve = 0;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int place = from[line + i * (256 / LANES)];
+    k[i] = *reinterpret_cast<const u32x4*>(keys + row_at(place, c.key_page) + piece);
+    v[i] = *reinterpret_cast<const u32x4*>(values + row_at(place, c.value_page) + piece);
+  }
+  if constexpr (E8) {
+    static_assert(T <= 256, "a thread has a token's exponents");
+    if (tid < T) ke = key_exponents[exponent_at(from[tid])], ve = value_exponents[exponent_at(from[tid])];
+  }
+  // who reads what this chunk writes: tokens before it that are kept from places low .. high of the list
+  const int* const before = p.before + (size_t)row * (p.chunks + 1);
+  const int low = before[chunk], high = first + T >= length ? first : min(before[chunk + 1], first);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int* const flags = p.flags + (size_t)row * p.chunks;
+  if (tid == 0) __hip_atomic_store(flags + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (low < high && tid <= (high - 1) / T - low / T) {
+    while (__hip_atomic_load(flags + low / T + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(2);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int at = line + i * (256 / LANES);
+    if (at >= count) break;
+    const int place = to[at];
+    *reinterpret_cast<u32x4*>(keys + row_at(place, c.key_page) + piece) = k[i];
+    *reinterpret_cast<u32x4*>(values + row_at(place, c.value_page) + piece) = v[i];
+  }
+  if constexpr (E8) {
+    if (tid < count) key_exponents[exponent_at(to[tid])] = ke, value_exponents[exponent_at(to[tid])] = ve;
+  }
+}
+
+// Bounds of the pages that a cut row's tokens are in now, a workgroup each: a thread has a feature and tokens SIDE apart; they meet in LDS.
+template <bool BF16, int D, bool E8>
+__global__ __launch_bounds__(256) void evict_bounds_kernel(EvictParams p) {
+  constexpr int SIDE = 256 / D;
+  __shared__ float low[256], high[256];
+  const PagedParams& c = p.cache;
+  const int rows = c.seqs * c.kv_heads, row = blockIdx.x % rows, number = blockIdx.x / rows, seq = row / c.kv_heads, head = row % c.kv_heads;
+  if (p.tokens[row] == 0) return;
+  const int page = c.table[(size_t)seq * c.table_row + number], count = min(1 << c.page_shift, p.keep - (number << c.page_shift));
+  const int f = threadIdx.x % D;
+  const size_t first = (size_t)head << c.page_shift;
+  float lo = INFINITY, hi = -INFINITY;
+  for (int i = threadIdx.x / D; i < count; i += SIDE) {
+    float x;
+    if constexpr (E8) {
+      const unsigned code = static_cast<const unsigned char*>(c.keys)[page * c.key_page + (long long)(first + i) * D + f];
+      const float up = power_of_two(c.key_exponents[(((size_t)page * c.kv_heads) << c.page_shift) + first + i]);
+      x = f32_of_16<BF16>((unsigned short)pack_pair<BF16>(__builtin_amdgcn_cvt_f32_fp8(code, 0) * up, 0.f));
+    } else {
+      x = f32_of_16<BF16>(static_cast<const unsigned short*>(c.keys)[page * c.key_page + (long long)(first + i) * D + f]);
+    }
+    lo = smaller(lo, x), hi = larger(hi, x);
+  }
+  low[threadIdx.x] = lo, high[threadIdx.x] = hi;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+#pragma unroll
+  for (int i = 1; i < SIDE; ++i) lo = smaller(lo, low[f + i * D]), hi = larger(hi, high[f + i * D]);
+  unsigned short* const to = p.bounds + ((size_t)page * c.kv_heads + head) * (2 * D) + f;
+  to[0] = (unsigned short)pack_pair<BF16>(lo, 0.f), to[D] = (unsigned short)pack_pair<BF16>(hi, 0.f);
+}
+
+int row_bytes(const iex_paged_cache& c) { return c.head_dim * (c.eight_bits ? 1 : 2); }
+int chunk_of(const iex_paged_cache& c) { return evict_chunk(row_bytes(c)); }
+
+template <int D, bool E8>
+void launch_move(const EvictParams& p, unsigned grid, hipStream_t s) {
+  note_kernel("evict_move_kernel<%d, %s>", D, E8 ? "e4m3" : "16");
+  hipLaunchKernelGGL((evict_move_kernel<D * (E8 ? 1 : 2), E8>), dim3(grid), dim3(256), 0, s, p);
+}
+template <bool E8>
+void launch_move(const EvictParams& p, int head_dim, unsigned grid, hipStream_t s) {
+  if (head_dim == 64) launch_move<64, E8>(p, grid, s);
+  else if (head_dim == 128) launch_move<128, E8>(p, grid, s);
+  else launch_move<256, E8>(p, grid, s);
+}
+
+template <bool BF16, bool E8>
+void launch_bounds(const EvictParams& p, int head_dim, unsigned grid, hipStream_t s) {
+  note_kernel("evict_bounds_kernel<%s, %d, %s>", BF16 ? "bf16" : "f16", head_dim, E8 ? "e4m3" : "16");
+  if (head_dim == 64) hipLaunchKernelGGL((evict_bounds_kernel<BF16, 64, E8>), dim3(grid), dim3(256), 0, s, p);
+  else if (head_dim == 128) hipLaunchKernelGGL((evict_bounds_kernel<BF16, 128, E8>), dim3(grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((evict_bounds_kernel<BF16, 256, E8>), dim3(grid), dim3(256), 0, s, p);
+}
+
+struct Layout {
+  long long rows, chunks;
+  size_t tickets, flags, before, kept_weights, bytes;   // where they begin, behind the rows' tokens
+};
+Layout layout_of(const iex_paged_cache& c, int keep) {
+  Layout l;
+  l.rows = (long long)c.seqs * c.kv_heads, l.chunks = ceil_div(keep, chunk_of(c));
+  l.tickets = (size_t)l.rows * 4;
+  l.flags = l.tickets + (size_t)l.rows * 4;
+  l.before = l.flags + (size_t)l.rows * l.chunks * 4;
+  l.kept_weights = l.before + (size_t)l.rows * (l.chunks + 1) * 4;
+  l.bytes = l.kept_weights + (size_t)l.rows * keep * 4;
+  return l;
+}
+// A table that holds no more than is kept: nothing ever moves.
+bool never(const iex_paged_cache& c, int keep) { return (long long)c.table_width * c.page_size <= keep; }
+
+}  // namespace
+}  // namespace iex
+
+extern "C" size_t iex_evict_tokens_workspace_bytes(const iex_paged_cache* cache, int keep) {
+  using namespace iex;
+  if (check_paged_cache(cache, "evict_tokens", false) || keep < 1) return 0;
+  return layout_of(*cache, keep).bytes;
+}
+
+extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, float* weights, int keep, int recent, int first, int* kept, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  using namespace iex;
+  trail_reset();
+  if (int rc = check_paged_cache(cache, "evict_tokens", true)) return rc;
+  IEX_REQUIRE(keep > 0 && first >= 0 && recent >= 0 && (long long)first + recent <= keep, IEX_ERR_BAD_ARGUMENT,
+              "evict_tokens: at least one token, the first and recent ones that are always kept among them (keep=%d first=%d recent=%d)", keep, first, recent);
+  if (cache->seqs == 0 || cache->kv_heads == 0) return 0;
+  IEX_REQUIRE(lengths == cache->lengths && kept && (weights || cache->table_width == 0), IEX_ERR_BAD_ARGUMENT, "evict_tokens: null pointer argument");
+  IEX_REQUIRE(aligned(weights, 4) && aligned(kept, 4), IEX_ERR_UNSUPPORTED, "evict_tokens: operands must be aligned to their elements");
+  IEX_REQUIRE((long long)cache->pages * cache->page_size < (1ll << 31), IEX_ERR_TOO_LARGE, "evict_tokens: up to 2^31 tokens in a cache");
+  const Layout l = layout_of(*cache, keep);
+  const long long pages = ceil_div(keep, cache->page_size);
+  IEX_REQUIRE(l.rows < (1ll << 22) && l.rows * l.chunks < (1ll << 24) && (!cache->bounds || l.rows * pages < (1ll << 24)), IEX_ERR_TOO_LARGE,
+              "evict_tokens: too many sequences, heads or tokens to keep");
+  IEX_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= l.bytes, IEX_ERR_BAD_ARGUMENT, "evict_tokens: needs a 256-byte aligned workspace of %zu bytes", l.bytes);
+  EvictParams p{};
+  p.cache = paged_params(*cache);
+  p.keep = keep, p.first = first, p.recent = recent, p.chunks = (int)l.chunks;
+  p.lengths = lengths, p.weights = weights, p.kept = kept, p.bounds = static_cast<unsigned short*>(cache->bounds);
+  char* const ws = static_cast<char*>(workspace);
+  p.tokens = reinterpret_cast<int*>(ws), p.tickets = reinterpret_cast<int*>(ws + l.tickets), p.flags = reinterpret_cast<int*>(ws + l.flags);
+  p.before = reinterpret_cast<int*>(ws + l.before), p.kept_weights = reinterpret_cast<float*>(ws + l.kept_weights);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const long long room = (long long)cache->table_width * cache->page_size;
+  const int chunk = chunk_of(*cache);
+  note_kernel("evict_select_kernel<%s>", room <= kEvictKept ? "kept" : "read again");
+  if (room <= kEvictKept) hipLaunchKernelGGL((evict_select_kernel<true>), dim3((unsigned)l.rows), dim3(kEvictThreads), room * 4, s, p, chunk);
+  else hipLaunchKernelGGL((evict_select_kernel<false>), dim3((unsigned)l.rows), dim3(kEvictThreads), 0, s, p, chunk);
+  if (int rc = check_hip(hipGetLastError(), "evict_tokens launch")) return rc;
+  if (never(*cache, keep) || cache->pages == 0) return 0;
+  const unsigned grid = (unsigned)(l.rows * l.chunks);
+  if (cache->eight_bits) launch_move<true>(p, cache->head_dim, grid, s);
+  else launch_move<false>(p, cache->head_dim, grid, s);
+  if (int rc = check_hip(hipGetLastError(), "evict_tokens launch")) return rc;
+  if (!cache->bounds) return 0;
+  const unsigned page_grid = (unsigned)(l.rows * pages);
+  if (cache->dtype == IEX_BF16) cache->eight_bits ? launch_bounds<true, true>(p, cache->head_dim, page_grid, s) : launch_bounds<true, false>(p, cache->head_dim, page_grid, s);
+  else cache->eight_bits ? launch_bounds<false, true>(p, cache->head_dim, page_grid, s) : launch_bounds<false, false>(p, cache->head_dim, page_grid, s);
+  return check_hip(hipGetLastError(), "evict_tokens launch");
+}

@@ -31,11 +31,11 @@ struct Strides {
   explicit Strides(const Tensor& t) : of{t.size(0) == 1 ? 0 : t.stride(0), t.size(1) == 1 ? 0 : t.stride(1), t.stride(2)} {}
 };
 
-// The cache as the C entry points take it; q is (rows, heads, head_dim).  keys / values undefined: bounds only.
-iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths,
+// The cache as the C entry points take it, for operands like q, heads of `dim` of `type`.  keys / values undefined: bounds only.
+iex_paged_cache paged_cache(const char* op, const Tensor& q, at::ScalarType type, int64_t dim, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths,
                             const std::optional<Tensor>& bounds, const std::optional<Tensor>& key_exponents, const std::optional<Tensor>& value_exponents) {
   iex_paged_cache c{};
-  c.dtype = dtype_code(q.scalar_type());
+  c.dtype = dtype_code(type);
   TORCH_CHECK(c.dtype == IEX_F16 || c.dtype == IEX_BF16, op, ": fp16 or bf16");
   check_ints(table, q, 2, op, "page_table");
   check_ints(lengths, q, 1, op, "lengths");
@@ -46,7 +46,7 @@ iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys,
     check_tensor(keys, q, 4, op, "keys");
     check_tensor(values, q, 4, op, "values");
     TORCH_CHECK(values.sizes() == keys.sizes() && values.scalar_type() == keys.scalar_type(), op, ": keys and values must be alike");
-    TORCH_CHECK(keys.size(3) == q.size(2), op, ": heads of ", q.size(2), " over a cache of heads of ", keys.size(3));
+    TORCH_CHECK(keys.size(3) == dim, op, ": heads of ", dim, " over a cache of heads of ", keys.size(3));
     for (const Tensor* t : {&keys, &values}) {
       check_no_gradient(*t, op);
       TORCH_CHECK(t->numel() == 0 || t->select(0, 0).is_contiguous(), op, ": a page of keys or values must be contiguous");
@@ -55,7 +55,7 @@ iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys,
     c.key_page_stride = keys.stride(0), c.value_page_stride = values.stride(0);
     c.keys = const_cast<void*>(keys.const_data_ptr()), c.values = const_cast<void*>(values.const_data_ptr());
     c.eight_bits = keys.scalar_type() == at::kFloat8_e4m3fn;
-    TORCH_CHECK(c.eight_bits || keys.scalar_type() == q.scalar_type(), op, ": the cache must hold the operands' type or float8_e4m3fn");
+    TORCH_CHECK(c.eight_bits || keys.scalar_type() == type, op, ": the cache must hold the operands' type or float8_e4m3fn");
     TORCH_CHECK(key_exponents.has_value() == (bool)c.eight_bits && value_exponents.has_value() == (bool)c.eight_bits, op,
                 ": a float8_e4m3fn cache has exponents of keys and of values, another none");
     if (c.eight_bits) {
@@ -72,12 +72,18 @@ iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys,
     check_tensor(*bounds, q, 4, op, "bounds");
     check_no_gradient(*bounds, op);
     if (!keys.defined()) c.pages = as_int(bounds->size(0), op), c.kv_heads = as_int(bounds->size(1), op), c.head_dim = as_int(bounds->size(3), op);
-    TORCH_CHECK(bounds->scalar_type() == q.scalar_type() && bounds->is_contiguous() && bounds->size(0) == c.pages && bounds->size(1) == c.kv_heads &&
-                    bounds->size(2) == 2 && bounds->size(3) == c.head_dim && c.head_dim == q.size(2),
+    TORCH_CHECK(bounds->scalar_type() == type && bounds->is_contiguous() && bounds->size(0) == c.pages && bounds->size(1) == c.kv_heads &&
+                    bounds->size(2) == 2 && bounds->size(3) == c.head_dim && c.head_dim == dim,
                 op, ": bounds must be contiguous (pages, kv_heads, 2, head_dim) of the operands' type");
     c.bounds = const_cast<void*>(bounds->const_data_ptr());
   }
   return c;
+}
+
+// ... for q (rows, heads, head_dim).
+iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths,
+                            const std::optional<Tensor>& bounds, const std::optional<Tensor>& key_exponents, const std::optional<Tensor>& value_exponents) {
+  return paged_cache(op, q, q.scalar_type(), q.size(2), keys, values, table, lengths, bounds, key_exponents, value_exponents);
 }
 
 void changed(const Tensor& t) {
@@ -200,4 +206,27 @@ Tensor select_pages(const Tensor& q, const Tensor& bounds, const Tensor& page_ta
                          ws.defined() ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
         op);
   return out;
+}
+
+Tensor evict_tokens(const Tensor& keys, const Tensor& values, const Tensor& page_table, const Tensor& lengths, const Tensor& weights, int64_t keep, int64_t recent,
+                    int64_t first, const std::optional<Tensor>& bounds, const std::optional<Tensor>& key_exponents, const std::optional<Tensor>& value_exponents) {
+  constexpr const char* op = "evict_tokens_";
+  check_tensor(keys, keys, 4, op, "keys");
+  // (an 8-bit cache's tokens are moved as they are; only its bounds have a type)
+  const at::ScalarType type = keys.scalar_type() != at::kFloat8_e4m3fn ? keys.scalar_type() : bounds ? bounds->scalar_type() : at::kHalf;
+  const iex_paged_cache c = paged_cache(op, keys, type, keys.size(3), keys, values, page_table, lengths, bounds, key_exponents, value_exponents);
+  check_weights(weights, keys, c, op);
+  TORCH_CHECK(keep > 0, op, ": at least one token");
+  const c10::DeviceGuard guard(keys.device());
+  const Tensor kept = at::empty({c.seqs, c.kv_heads, keep}, page_table.options());
+  const int most = as_int(keep, op);
+  const size_t bytes = iex_evict_tokens_workspace_bytes(&c, most);
+  const Tensor ws = workspace(bytes, keys);
+  check(iex_evict_tokens(&c, const_cast<int*>(c.lengths), const_cast<float*>(weights.const_data_ptr<float>()), most, as_int(recent, op), as_int(first, op), kept.data_ptr<int>(),
+                         ws.defined() ? ws.data_ptr() : nullptr, bytes, stream_of(keys)),
+        op);
+  for (const Tensor* t : {&keys, &values, &lengths, &weights}) changed(*t);
+  for (const std::optional<Tensor>* t : {&bounds, &key_exponents, &value_exponents})
+    if (*t) changed(**t);
+  return kept;
 }

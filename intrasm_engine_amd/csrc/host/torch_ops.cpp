@@ -746,6 +746,9 @@ TORCH_LIBRARY(iex_ops, lib) {
          TORCH_FN(paged_attention_accumulate));
   define("select_pages", "(Tensor q, Tensor bounds, Tensor page_table, Tensor lengths, int page_size, int count, int first=1, int last=1) -> Tensor",
          TORCH_FN(select_pages));
+  define("evict_tokens_", "(Tensor(a!) keys, Tensor(b!) values, Tensor page_table, Tensor(c!) lengths, Tensor(d!) weights, int keep, int recent, int first=0, "
+         "Tensor(e!)? bounds=None, Tensor(f!)? key_exponents=None, Tensor(g!)? value_exponents=None) -> Tensor",
+         TORCH_FN(evict_tokens));
 }
 
 PYBIND11_MODULE(_iex_host, module) {

@@ -15,6 +15,7 @@
 // conversions take 16 clocks each, which alone would allow 10), selection 10.4; 32 x up to 1024 pages, 8 key heads, in one launch 19 us = 1.9 TB/s,
 // 68 % of it waiting (a workgroup a row: the longest set the time).
 #include "paged_cache_host.h"
+#include "select_device.cuh"
 
 namespace iex {
 namespace {
@@ -195,10 +196,8 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
   constexpr int WAVES = kSelectThreads / kWave;
   extern __shared__ unsigned kept[];
   __shared__ double weights[SCORED ? 2 : 2 * D];
-  __shared__ unsigned histogram[256];
-  __shared__ int chosen[3], totals[2][WAVES];
   const PagedParams& c = p.cache;
-  const int row = blockIdx.x, seq = row / c.kv_heads, tid = threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
+  const int row = blockIdx.x, seq = row / c.kv_heads, tid = threadIdx.x, wave = uniform(tid >> 6);
   const int used = used_pages(c, seq);
   const unsigned* keys = SCORED ? p.keys + (size_t)row * c.table_width : nullptr;
   int* out = p.out + (size_t)row * p.count;
@@ -212,81 +211,7 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
   __syncthreads();
   auto key_of = [&](int i) { return KEPT ? kept[i] : keys[i]; };
 
-  // ---- the count-th largest key ----
-  unsigned threshold = 0;
-  int need = p.count;   // of the keys that agree with it in the bits found so far, the need-th largest
-  if (used > p.count) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) histogram[tid] = 0;
-      __syncthreads();
-      for (int i0 = wave * kWave; i0 < used; i0 += kSelectThreads) {
-        const int i = i0 + lane;
-        const unsigned key = i < used ? key_of(i) : 0u;
-        const bool mine = i < used && (shift == 24 || key >> (shift + 8) == threshold >> (shift + 8));
-        const int bin = key >> shift & 255;
-        // scores of a row share their leading bits: the lanes that agree with the first one are counted at once
-        const unsigned long long some = __ballot(mine);
-        if (some) {
-          const int leader = __ffsll(some) - 1, its = __builtin_amdgcn_readlane(bin, leader);
-          const unsigned long long same = __ballot(mine && bin == its);
-          if (lane == leader) atomicAdd(&histogram[its], (unsigned)__popcll(same));
-          else if (mine && bin != its) atomicAdd(&histogram[bin], 1u);
-        }
-      }
-      __syncthreads();
-      if (wave == 0) {   // four bins a lane, from the largest down
-        unsigned four[4], mine = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mine += four[j] = histogram[255 - (lane * 4 + j)];
-        unsigned above = (unsigned)wave_scan((int)mine) - mine;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (above < (unsigned)need && above + four[j] >= (unsigned)need)
-            chosen[0] = 255 - (lane * 4 + j), chosen[1] = need - (int)above, chosen[2] = above + four[j] == (unsigned)need;
-          above += four[j];
-        }
-      }
-      __syncthreads();
-      threshold |= (unsigned)chosen[0] << shift;
-      need = chosen[1];
-      if (chosen[2] && threshold != 0) {   // all that agree so far are wanted: whatever follows (and nothing below)
-        --threshold, need = 0;
-        break;
-      }
-    }
-  }
-
-  // ---- pages above it, and the first `need` that equal it, in ascending order: a wavefront has a stretch of pages ----
-  const int stretch = (used + kSelectThreads - 1) / kSelectThreads * kWave, begin = min(used, wave * stretch), end = min(used, begin + stretch);
-  int above = 0, equal = 0;
-  for (int i0 = begin; i0 < end; i0 += kWave) {
-    const unsigned key = i0 + lane < end ? key_of(i0 + lane) : 0u;
-    above += __popcll(__ballot(key > threshold));
-    equal += __popcll(__ballot(key == threshold && key != 0));
-  }
-  if (lane == 0) totals[0][wave] = above, totals[1][wave] = equal;
-  __syncthreads();
-  int written = 0, equals = 0, all = 0;   // before this wavefront's stretch; all pages that are taken
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const int taken = min(totals[1][w], max(0, need - equals));
-    if (w < wave) written += totals[0][w] + taken;
-    all += totals[0][w] + taken;
-    equals += totals[1][w];
-  }
-  equals = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) equals += w < wave ? totals[1][w] : 0;
-  for (int i0 = begin; i0 < end; i0 += kWave) {
-    const unsigned key = i0 + lane < end ? key_of(i0 + lane) : 0u;
-    const bool same = key == threshold && key != 0;
-    const unsigned long long sames = __ballot(same), below = (1ull << lane) - 1;
-    const bool take = key > threshold || (same && equals + __popcll(sames & below) < need);
-    const unsigned long long takes = __ballot(take);
-    const int to = written + __popcll(takes & below);
-    if (take && to < p.count) out[to] = i0 + lane;
-    written += __popcll(takes), equals += __popcll(sames);
-  }
+  const int all = select_largest<kSelectThreads>(used, p.count, key_of, [&](int to, int i) { out[to] = i; }, [](int, int) {});
   for (int i = all + tid; i < p.count; i += kSelectThreads) out[i] = -1;
 }
 
