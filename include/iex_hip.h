@@ -479,6 +479,34 @@ int iex_kv_append(const iex_paged_cache* cache, int tokens, const int* offsets, 
                   const void* v, const long long* v_strides, const void* q, const long long* q_strides, void* q_out,
                   const long long* q_out_strides, const float* rotation, int positions, int rotary, int interleaved, void* stream);
 
+/* A rotation of features by position.  table: (rows, features) fp32, features / 2 cosines and as many sines of a position; the first `features`
+ * features of a head turn in pairs (j, j + features / 2), or (2j, 2j + 1) where interleaved: y0 = x0 cos - x1 sin, y1 = x1 cos + x0 sin, each product
+ * and sum rounded to 32 bits, rounded once more to the operand's type.  at: (axes, tokens) int32, rows `axis_stride` apart, the position of
+ * every token on one to four axes; sections (host memory; may be null for one axis): how many of the features / 2 planes go by each axis, stretches of
+ * planes one behind the other or, in_turn, planes dealt to the axes in turn as long as an axis has some left.  Read on the device when the kernels
+ * run: a position below 0 counts as 0, the planes of one at or behind `rows` come out as NaN. */
+typedef struct iex_rotation {
+  const float* table;
+  int rows, features;
+  const int* at;
+  long long axis_stride;
+  int axes;
+  const int* sections;
+  int in_turn, interleaved;
+} iex_rotation;
+
+/* iex_kv_append with positions that are given (rotation->at: of the call's tokens) and not the tokens' places in their sequences.  rotation null or of no
+ * features: nothing turns; rotation->at null: as iex_kv_append. */
+int iex_kv_append_at(const iex_paged_cache* cache, int tokens, const int* offsets, int heads, const void* k, const long long* k_strides,
+                     const void* v, const long long* v_strides, const void* q, const long long* q_strides, void* q_out,
+                     const long long* q_out_strides, const iex_rotation* rotation, void* stream);
+
+/* out = x rotated: (tokens, heads, head_dim) of fp32, fp16 or bf16, any strides (token, head, feature; elements; of out no two elements in one
+ * place), not in place.  Features behind the rotated ones are copied.  back: by the same angles the other way (the gradient).  rotation->at is
+ * needed, rotation->features even. */
+int iex_rotate(int dtype, int tokens, int heads, int head_dim, const void* x, const long long* x_strides, void* out,
+               const long long* out_strides, const iex_rotation* rotation, int back, void* stream);
+
 /* out[s, h] = softmax over the tokens of sequence s (scale * q[s, h] . key) value; heads / kv_heads query heads share a key
  * head.  q, out: (seqs, heads, head_dim), any strides (sequence, head, feature).  listed (null: every page): (seqs, kv_heads,
  * count), the pages of the sequence's table to attend to; entries outside the table (-1) are passed over, one that comes twice

@@ -41,7 +41,12 @@ class PagedCache(_c.Structure):
                 ("value_exponents", _vp), ("bounds", _vp), ("table", _vp), ("seqs", _i), ("table_width", _i), ("table_stride", _ll), ("lengths", _vp)]
 
 
-_cache, _strides = _c.POINTER(PagedCache), _c.POINTER(_ll)
+class Rotation(_c.Structure):
+    """``iex_rotation``: cosines and sines by position, and the tokens' positions."""
+    _fields_ = [("table", _vp), ("rows", _i), ("features", _i), ("at", _vp), ("axis_stride", _ll), ("axes", _i), ("sections", _c.POINTER(_i)), ("in_turn", _i), ("interleaved", _i)]
+
+
+_cache, _strides, _rotation = _c.POINTER(PagedCache), _c.POINTER(_ll), _c.POINTER(Rotation)
 
 # name -> (restype, argtypes).  Kept in one table so that the symbol-export test can
 # walk it against the header.
@@ -90,6 +95,8 @@ SIGNATURES = {
     "iex_sparse_attention_fits": (_i, [_i, _i, _i]),
     "iex_sparse_attention": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f, _vp, _vp, _c.c_size_t, _vp]),
     "iex_kv_append": (_i, [_cache, _i, _vp, _i, _vp, _strides, _vp, _strides, _vp, _strides, _vp, _strides, _vp, _i, _i, _i, _vp]),
+    "iex_kv_append_at": (_i, [_cache, _i, _vp, _i, _vp, _strides, _vp, _strides, _vp, _strides, _vp, _strides, _rotation, _vp]),
+    "iex_rotate": (_i, [_i, _i, _i, _i, _vp, _strides, _vp, _strides, _rotation, _i, _vp]),
     "iex_paged_attention_workspace_bytes": (_c.c_size_t, [_cache, _i, _i]),
     "iex_paged_attention": (_i, [_cache, _i, _vp, _strides, _f, _vp, _i, _vp, _strides, _vp, _c.c_size_t, _vp]),
     "iex_paged_attention_accumulate_workspace_bytes": (_c.c_size_t, [_cache, _i]),

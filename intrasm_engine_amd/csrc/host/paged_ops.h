@@ -86,13 +86,45 @@ iex_paged_cache paged_cache(const char* op, const Tensor& q, const Tensor& keys,
   return paged_cache(op, q, q.scalar_type(), q.size(2), keys, values, table, lengths, bounds, key_exponents, value_exponents);
 }
 
+// A rotation as the C entry points take it: the table, and where given the positions of `tokens` tokens and their axes' sections.
+struct RotationArguments {
+  iex_rotation rotation{};
+  std::array<int, 4> sections{};
+  RotationArguments(const char* op, const Tensor& with, const std::optional<Tensor>& table, const std::optional<Tensor>& positions, at::OptionalIntArrayRef by, bool in_turn,
+                    bool interleaved) {
+    rotation.axes = 1;
+    rotation.in_turn = in_turn, rotation.interleaved = interleaved;
+    TORCH_CHECK(table || !positions, op, ": positions without a rotation");
+    TORCH_CHECK(positions || !by, op, ": sections without positions");
+    if (!table) return;
+    check_tensor(*table, with, 2, op, "rotation");
+    check_no_gradient(*table, op);
+    TORCH_CHECK(table->scalar_type() == at::kFloat && table->is_contiguous(), op, ": rotation must be contiguous float32 (positions, rotated features)");
+    rotation.table = table->const_data_ptr<float>();
+    rotation.rows = as_int(table->size(0), op), rotation.features = as_int(table->size(1), op);
+    if (!positions) return;
+    TORCH_CHECK(rotation.features > 0, op, ": positions without a rotation");
+    check_ints(*positions, with, positions->dim() == 2 ? 2 : 1, op, "positions");
+    TORCH_CHECK(positions->size(-1) == with.size(0), op, ": positions must be (tokens) or (axes, tokens) (", positions->size(-1), ", ", with.size(0), " tokens)");
+    rotation.axes = positions->dim() == 2 ? as_int(positions->size(0), op) : 1;
+    rotation.axis_stride = positions->dim() == 2 ? positions->stride(0) : 0;
+    rotation.at = positions->const_data_ptr<int>();
+    if (!by) return;
+    TORCH_CHECK((int64_t)by->size() == rotation.axes && rotation.axes <= 4, op, ": a section for each of one to four axes (", by->size(), " sections, ", rotation.axes, " axes)");
+    for (size_t i = 0; i < by->size(); ++i) sections[i] = as_int((*by)[i], op);
+    rotation.sections = sections.data();
+  }
+  RotationArguments(const RotationArguments&) = delete;   // (the C argument points into it)
+};
+
 void changed(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values, const Tensor& page_table, const Tensor& lengths,
                  const std::optional<Tensor>& offsets, const std::optional<Tensor>& q, const std::optional<Tensor>& rotation, bool interleaved,
-                 const std::optional<Tensor>& bounds, const std::optional<Tensor>& key_exponents, const std::optional<Tensor>& value_exponents) {
+                 const std::optional<Tensor>& bounds, const std::optional<Tensor>& key_exponents, const std::optional<Tensor>& value_exponents,
+                 const std::optional<Tensor>& positions, at::OptionalIntArrayRef sections, bool in_turn) {
   constexpr const char* op = "kv_append_";
   check_tensor(k, k, 3, op, "k");
   check_tensor(v, k, 3, op, "v");
@@ -111,23 +143,33 @@ Tensor kv_append(const Tensor& k, const Tensor& v, const Tensor& keys, const Ten
     check_no_gradient(*q, op);
     TORCH_CHECK(q->scalar_type() == k.scalar_type() && q->size(0) == k.size(0) && q->size(2) == k.size(2), op, ": q must be (tokens, heads, head_dim) like k");
   }
-  int rotary = 0, positions = 0;
-  if (rotation) {
-    check_tensor(*rotation, k, 2, op, "rotation");
-    check_no_gradient(*rotation, op);
-    TORCH_CHECK(rotation->scalar_type() == at::kFloat && rotation->is_contiguous(), op, ": rotation must be contiguous float32 (positions, rotated features)");
-    positions = as_int(rotation->size(0), op), rotary = as_int(rotation->size(1), op);
-  }
+  const RotationArguments turn(op, k, rotation, positions, sections, in_turn, interleaved);
   const c10::DeviceGuard guard(k.device());
   const Tensor out = q ? at::empty_like(*q) : Tensor();
   const Strides ks(k), vs(v), qs(q ? *q : k), os(q ? out : k);
-  check(iex_kv_append(&c, as_int(k.size(0), op), offsets ? offsets->const_data_ptr<int>() : nullptr, q ? as_int(q->size(1), op) : 0, k.const_data_ptr(), ks.of,
+  check(iex_kv_append_at(&c, as_int(k.size(0), op), offsets ? offsets->const_data_ptr<int>() : nullptr, q ? as_int(q->size(1), op) : 0, k.const_data_ptr(), ks.of,
                       v.const_data_ptr(), vs.of, q ? q->const_data_ptr() : nullptr, qs.of, q ? out.data_ptr() : nullptr, os.of,
-                      rotation ? rotation->const_data_ptr<float>() : nullptr, positions, rotary, interleaved, stream_of(k)),
+                         &turn.rotation, stream_of(k)),
         op);
   for (const Tensor* t : {&keys, &values}) changed(*t);
   for (const std::optional<Tensor>* t : {&bounds, &key_exponents, &value_exponents})
     if (*t) changed(**t);
+  return out;
+}
+
+// x (tokens, heads, head_dim) turned by its tokens' positions; as x lies.
+Tensor rotated(const Tensor& x, const Tensor& rotation, const Tensor& positions, at::OptionalIntArrayRef sections, bool in_turn, bool interleaved, bool back) {
+  constexpr const char* op = "rotate";
+  check_tensor(x, x, 3, op, "x");
+  const int dtype = dtype_code(x.scalar_type());
+  TORCH_CHECK(dtype >= 0, op, ": fp32, fp16 or bf16");
+  const RotationArguments turn(op, x, rotation, positions, sections, in_turn, interleaved);
+  const c10::DeviceGuard guard(x.device());
+  const Tensor out = at::empty_like(x);
+  const Strides xs(x), os(out);
+  check(iex_rotate(dtype, as_int(x.size(0), op), as_int(x.size(1), op), as_int(x.size(2), op), x.const_data_ptr(), xs.of, out.data_ptr(), os.of, &turn.rotation, back,
+                   stream_of(x)),
+        op);
   return out;
 }
 

@@ -717,6 +717,34 @@ Tensor trainable_linear(const Tensor& input, const Tensor& weight) {
   return TrainableLinear::apply(input, weight);
 }
 
+// The gradient of a rotation is the rotation back (of its gradient the rotation itself).
+struct TrainableRotate : torch::autograd::Function<TrainableRotate> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& rotation, const Tensor& positions, at::OptionalIntArrayRef sections, bool in_turn, bool interleaved,
+                        bool back) {
+    ctx->save_for_backward({rotation, positions});
+    ctx->saved_data["sections"] = sections ? c10::IValue(sections->vec()) : c10::IValue();
+    ctx->saved_data["in_turn"] = in_turn, ctx->saved_data["interleaved"] = interleaved, ctx->saved_data["back"] = back;
+    return rotated(x, rotation, positions, sections, in_turn, interleaved, back);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
+
+Tensor trainable_rotate(const Tensor& x, const Tensor& rotation, const Tensor& positions, at::OptionalIntArrayRef sections, bool in_turn, bool interleaved, bool back) {
+  if (!at::GradMode::is_enabled() || !x.requires_grad()) return rotated(x, rotation, positions, sections, in_turn, interleaved, back);
+  return TrainableRotate::apply(x, rotation, positions, sections, in_turn, interleaved, back);
+}
+
+variable_list TrainableRotate::backward(AutogradContext* ctx, variable_list grads) {
+  const auto saved = ctx->get_saved_variables();
+  variable_list out(7);
+  if (!ctx->needs_input_grad(0) || !grads[0].defined()) return out;
+  const c10::IValue& sections = ctx->saved_data["sections"];
+  const std::vector<int64_t> by = sections.isNone() ? std::vector<int64_t>() : sections.toIntVector();
+  out[0] = trainable_rotate(grads[0], saved[0], saved[1], sections.isNone() ? at::OptionalIntArrayRef() : at::OptionalIntArrayRef(by), ctx->saved_data["in_turn"].toBool(),
+                            ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["back"].toBool());
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(iex_ops, lib) {
@@ -736,8 +764,12 @@ TORCH_LIBRARY(iex_ops, lib) {
   define("csr_softmax_", "(Tensor(a!) values, Tensor row_indices, Tensor row_offsets, float scale) -> Tensor(a!)", TORCH_FN(csr_softmax));
   define("gemm_mfma", "(Tensor a, Tensor b, bool trans_b=False) -> Tensor", TORCH_FN(gemm));
   define("kv_append_", "(Tensor k, Tensor v, Tensor(a!) keys, Tensor(b!) values, Tensor page_table, Tensor lengths, Tensor? offsets=None, Tensor? q=None, "
-         "Tensor? rotation=None, bool interleaved=False, Tensor(c!)? bounds=None, Tensor(d!)? key_exponents=None, Tensor(e!)? value_exponents=None) -> Tensor",
+         "Tensor? rotation=None, bool interleaved=False, Tensor(c!)? bounds=None, Tensor(d!)? key_exponents=None, Tensor(e!)? value_exponents=None, "
+         "Tensor? positions=None, int[]? sections=None, bool in_turn=False) -> Tensor",
          TORCH_FN(kv_append));
+  define("rotate", "(Tensor x, Tensor rotation, Tensor positions, int[]? sections=None, bool in_turn=False, bool interleaved=False, bool back=False) -> Tensor",
+         TORCH_FN(rotated));
+  lib.impl("rotate", torch::dispatch(c10::DispatchKey::Autograd, TORCH_FN(trainable_rotate)));
   define("paged_attention", "(Tensor q, Tensor keys, Tensor values, Tensor page_table, Tensor lengths, float? scale=None, Tensor? pages=None, "
          "Tensor? key_exponents=None, Tensor? value_exponents=None) -> Tensor",
          TORCH_FN(paged_attention));

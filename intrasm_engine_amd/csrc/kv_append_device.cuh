@@ -1,9 +1,6 @@
 // New tokens' keys and values into a paged cache, with the position rotation of keys and queries on the way.
 //
-// A token at position t has its features rotated in r / 2 planes, plane j by the angle a(t, j) whose cosine and sine are given:
-//   y0 = x0 cos - x1 sin,   y1 = x1 cos + x0 sin
-// where (x0, x1) are features (j, j + r/2) or, interleaved, (2j, 2j + 1).  Products and sums are rounded one by one in 32 bits (no
-// fused multiply-add), so that anybody's plain formula gives the same bits before the one rounding to the cache's type.
+// (Rotation: rotation_device.cuh.  A token's position is its place in the sequence, or given: behind tokens that have been dropped, on several axes.)
 //
 // A workgroup has the new tokens of one sequence in one span of positions (whole pages) for a few heads of one kind: keys,
 // queries or values.  A thread has a unit of 16 features of a token: both halves of eight planes, so a rotation needs nobody
@@ -16,7 +13,7 @@
 // and written; 23 of 3 .. 5001 tokens, 32 + 2 x 8 heads, into e4m3 with bounds 96 us = 4.2 (waiting for a row's maximum, vector
 // units 36 %); a step of one sequence of 3 x 32 heads 3.0 us, of 64 of 32 + 2 x 8 heads with bounds 4.2.
 #pragma once
-#include "paged_cache_device.cuh"
+#include "rotation_device.cuh"
 
 namespace iex {
 
@@ -27,12 +24,12 @@ struct AppendOperand {
 
 struct AppendParams {
   PagedParams cache;
-  int tokens, heads, rotary, columns, per_group;   // heads of a workgroup (keys: one, where there are bounds)
+  int tokens, heads, columns, per_group;   // heads of a workgroup (keys: one, where there are bounds)
   const int* offsets;                     // null: one token per sequence (kv_append_step_kernel)
   AppendOperand k, q, v;
   unsigned short* q_out;
   long long out_token, out_head, out_feature;   // strides
-  const float* rotation;
+  Rotation rotation;
   unsigned short* bounds;
 };
 
@@ -45,14 +42,6 @@ __device__ __forceinline__ unsigned group_max(unsigned v) {
   if (LANES >= 8) with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
   if (LANES >= 16) with((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
   return v;
-}
-
-// One plane.
-__device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
-#pragma clang fp contract(off)
-  const float ac = a * c, bs = b * s, bc = b * c, as = a * s;
-  a = ac - bs;
-  b = bc + as;
 }
 
 // What a workgroup has: rows low .. high of the span of positions from `begin` on, token `first_token` + row of the call; heads
@@ -117,15 +106,8 @@ struct UnitPlace {
   bool turned;
   int c0, c1;
   __device__ __forceinline__ UnitPlace(const AppendParams& p, const AppendWork& w, int u, bool interleaved) {
-    turned = (w.is_k || w.is_q) && u < p.rotary / 16 && w.a.sound;
-    c0 = !interleaved && turned ? u : 2 * u, c1 = !interleaved && turned ? u + p.rotary / 16 : 2 * u + 1;
-  }
-};
-struct Planes {
-  float4 c[2], s[2];
-  __device__ __forceinline__ void load(const AppendParams& p, int position, int u) {
-    const float4* t = reinterpret_cast<const float4*>(p.rotation + (size_t)position * p.rotary + 8 * u);
-    c[0] = t[0], c[1] = t[1], s[0] = t[p.rotary / 8], s[1] = t[p.rotary / 8 + 1];
+    turned = (w.is_k || w.is_q) && u < p.rotation.features / 16 && w.a.sound;
+    c0 = !interleaved && turned ? u : 2 * u, c1 = !interleaved && turned ? u + p.rotation.features / 16 : 2 * u + 1;
   }
 };
 // The unit's 16 features in 32 bits and, turned, in 16.
@@ -137,10 +119,8 @@ __device__ __forceinline__ void turn_unit(bool turned, const Planes& t, u32x4& r
     unpack_pair<BF16>(raw1[j], x[8 + 2 * j], x[9 + 2 * j]);
   }
   if (!turned) return;
-  const float c[8] = {t.c[0].x, t.c[0].y, t.c[0].z, t.c[0].w, t.c[1].x, t.c[1].y, t.c[1].z, t.c[1].w};
-  const float s[8] = {t.s[0].x, t.s[0].y, t.s[0].z, t.s[0].w, t.s[1].x, t.s[1].y, t.s[1].z, t.s[1].w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) rotate(x[INTERLEAVED ? 2 * i : i], x[INTERLEAVED ? 2 * i + 1 : 8 + i], c[i], s[i]);
+  for (int i = 0; i < 8; ++i) rotate(x[INTERLEAVED ? 2 * i : i], x[INTERLEAVED ? 2 * i + 1 : 8 + i], t.c[i], t.s[i]);
 #pragma unroll
   for (int j = 0; j < 4; ++j) raw0[j] = pack_pair<BF16>(x[2 * j], x[2 * j + 1]), raw1[j] = pack_pair<BF16>(x[8 + 2 * j], x[9 + 2 * j]);
 }
@@ -261,7 +241,7 @@ __device__ __forceinline__ void stored_unit(float* row, const UnitPlace& at, con
 
 // One token per sequence, a step of generation: rows are sequences, each with a place of its own, so a page's bounds are its row's
 // business.  STAGED: operands of any strides, lanes along the sequences, through LDS.
-template <bool BF16, int D, bool E8, bool INTERLEAVED, bool STAGED>
+template <bool BF16, int D, bool E8, bool INTERLEAVED, bool AT, bool STAGED>
 __global__ __launch_bounds__(256, 4) void kv_append_step_kernel(AppendParams p) {
   typedef unsigned short u16;
   constexpr int U = D / 16, R = 256 / U;
@@ -298,7 +278,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_step_kernel(AppendParams p) 
     raw1 = *reinterpret_cast<const u32x4*>(from + at.c1 * 8);
   }
   Planes planes;
-  if (at.turned) planes.load(p, w.a.position, u);   // (of a sound row)
+  if (at.turned) planes.load<AT>(p.rotation, seq, w.a.position, u);   // (of a sound row)
   const int slot = w.a.position & ((1 << cache.page_shift) - 1);
   int page = -1;
   if (!w.is_q && w.a.sound) page = cache.table[(size_t)seq * cache.table_row + (w.a.position >> cache.page_shift)];
@@ -364,7 +344,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_step_kernel(AppendParams p) 
 }
 
 // Operands whose rows are whole aligned 16-byte chunks.  HEADS: heads whose loads are in flight at once.
-template <bool BF16, int D, bool E8, bool INTERLEAVED, int HEADS>
+template <bool BF16, int D, bool E8, bool INTERLEAVED, bool AT, int HEADS>
 __global__ __launch_bounds__(256, 4) void kv_append_kernel(AppendParams p) {
   constexpr int U = D / 16, R = 256 / U;   // units of a row, rows of a step
   extern __shared__ __align__(16) unsigned char smem[];
@@ -381,7 +361,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_kernel(AppendParams p) {
     const int row = block + r, position = w.begin + row;
     const bool mine = row >= w.low && row < w.high;
     Planes planes;
-    if (at.turned && mine) planes.load(p, position, u);
+    if (at.turned && mine) planes.load<AT>(p.rotation, w.first_token + row, position, u);
     int page = -1;
     if (!w.is_q && mine) page = p.cache.table[(size_t)w.seq * p.cache.table_row + (position >> p.cache.page_shift)];
     for (int head1 = w.head0; head1 < w.head_end; head1 += HEADS) {
@@ -426,7 +406,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_kernel(AppendParams p) {
 // written 16 bytes at a time, eight tokens of a feature, and turned around two bytes at a time in LDS; else two bytes at a time in memory.
 constexpr int kColumnTokens = 64;
 typedef u32x4 AnyChunk __attribute__((aligned(2)));
-template <bool BF16, int D, bool E8, bool INTERLEAVED>
+template <bool BF16, int D, bool E8, bool INTERLEAVED, bool AT>
 __global__ __launch_bounds__(256, 4) void kv_append_columns_kernel(AppendParams p) {
   typedef unsigned short u16;
   constexpr int U = D / 16, R = 256 / U, T = kColumnTokens;
@@ -502,7 +482,7 @@ __global__ __launch_bounds__(256, 4) void kv_append_columns_kernel(AppendParams 
         const int t = sub + r, position = w.begin + block + t;
         const bool mine = t >= low && t < high;
         Planes planes;
-        if (at.turned && mine) planes.load(p, position, u);
+        if (at.turned && mine) planes.load<AT>(p.rotation, token0 + t, position, u);
         int page = -1;
         if (!w.is_q && mine) page = p.cache.table[(size_t)w.seq * p.cache.table_row + (position >> p.cache.page_shift)];
         u32x4 raw0 = {0u, 0u, 0u, 0u}, raw1 = raw0;
