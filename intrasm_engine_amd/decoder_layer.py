@@ -179,24 +179,32 @@ class SparseDecoderLayer:
         """(hidden, tokens) as (tokens, heads, head_dim), where it lies."""
         return t.view(self.heads, self.head_dim, t.shape[1]).permute(2, 0, 1)
 
-    def prompt(self, x: torch.Tensor, cache: KVCache, page_table, lengths, offsets, rotation=None) -> None:
+    def prompt(self, x: torch.Tensor, cache: KVCache, page_table, lengths, offsets, rotation=None, positions=None, sections=None, in_turn: bool = False) -> None:
         """Keys and values of prompts into the cache: columns ``offsets[s] .. offsets[s + 1]`` of x (hidden, tokens) are sequence s's
-        newest, ``lengths`` counts them.  For this layer's cache only: new tokens do not attend to each other here, so there is no result to
+        newest, ``lengths`` counts them; ``positions`` as :meth:`KVCache.append_` takes them.  For this layer's cache only: new tokens do not attend to each other here, so there is no result to
         hand on to a next layer, whose prompts go through :meth:`decode` token by token."""
-        cache.append_(self._tokens(self.proj("k", x)), self._tokens(self.proj("v", x)), page_table, lengths, offsets, None, rotation)
+        cache.append_(self._tokens(self.proj("k", x)), self._tokens(self.proj("v", x)), page_table, lengths, offsets, None, rotation,
+                      positions=positions, sections=sections, in_turn=in_turn)
 
-    def decode(self, x: torch.Tensor, cache: KVCache, page_table, lengths, rotation=None, pages: int = 0) -> torch.Tensor:
+    def decode(self, x: torch.Tensor, cache: KVCache, page_table, lengths, rotation=None, pages: int = 0, positions=None, sections=None, in_turn: bool = False,
+               weights=None) -> torch.Tensor:
         """One new token of every sequence: x (hidden, sequences) fp16 -> same shape.  Its key and value go into the cache (``lengths``
         counts it) and it attends to all of its sequence, or to the ``pages`` pages that its query can score highest with (a cache
-        with bounds; the page with the new token is always among them, and the first one if there are more).  Capturable: a graph follows
-        ``page_table`` and ``lengths``."""
+        with bounds; the page with the new token is always among them, and the first one if there are more).  ``weights`` (:meth:`KVCache.new_weights`): what
+        tokens get of attention is added to them, for :meth:`KVCache.evict_` between steps, behind which new tokens need ``positions``.  Capturable: a graph
+        follows ``page_table``, ``lengths`` and ``positions``."""
         if pages < 0:
             raise ValueError("decode: pages must not be negative")
+        if pages and weights is not None:
+            raise ValueError("decode: an account is kept over all pages, not over selected ones")
+        if weights is not None and not cache.fits(weights, page_table):
+            raise ValueError("decode: weights must be contiguous float32 (sequences, kv_heads, tokens of a table)")
         if pages and cache.bounds is None:      # (before anything is written)
             raise RuntimeError("decode: the cache keeps no bounds")
-        q = cache.append_(self._tokens(self.proj("k", x)), self._tokens(self.proj("v", x)), page_table, lengths, None, self._tokens(self.proj("q", x)), rotation)
+        q = cache.append_(self._tokens(self.proj("k", x)), self._tokens(self.proj("v", x)), page_table, lengths, None, self._tokens(self.proj("q", x)), rotation,
+                          positions=positions, sections=sections, in_turn=in_turn)
         selected = cache.select(q, page_table, lengths, pages, first=min(1, pages - 1)) if pages else None
-        attended = cache.attend(q, page_table, lengths, None, selected)
+        attended = cache.attend(q, page_table, lengths, None, selected, weights)
         h = self._proj_with("o", attended.permute(1, 2, 0).reshape(self.hidden, x.shape[1]), x, 1)
         return self.mlp_block(h)
 
