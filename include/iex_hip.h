@@ -544,7 +544,7 @@ int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, con
 
 /* Tokens that got least attention leave the cache.  A sequence of more than `keep` tokens (lengths[s], cut to what the table holds; lengths is
  * cache->lengths) has `keep` of them afterwards, for every key head its own: the first `first`, the last `recent` and, of those between, the ones
- * with the largest weights[s, g, t] (seqs, kv_heads, table_width * page_size; ties: the earlier token; a NaN is larger than all).  Their rows move, in order,
+ * with the largest weights[s, g, t] (seqs, kv_heads, table_width * page_size; 16-byte aligned; ties: the earlier token; a NaN is larger than all).  Their rows move, in order,
  * to the sequence's first `keep` places, their weights with them; the weights of places behind are 0 then, lengths[s] is `keep`, bounds (if the
  * cache has them) are those of the tokens that the pages then hold.  kept: (seqs, kv_heads, keep), where the tokens were, ascending.
  * Other sequences stay as they are, kept has their tokens 0 .. lengths[s] - 1 and -1 behind them.  A sequence of more than `keep` tokens with pages

@@ -2,8 +2,9 @@
 // of those between, the ones with the largest accumulated weight (paged_account.hip), the earlier of two that are equal; they move, in order, to places
 // 0 .. keep - 1 of the sequence's own pages, their weights with them, and the sequence has `keep` tokens.
 //
-// Two launches.  The first, a workgroup a sequence and key head, finds the keep largest weights (select_device.cuh) and leaves the list of kept tokens, ascending.
-// The second moves rows, in place: chunk c of a list, up to `chunk` tokens, reads rows that others may be about to write.  The i-th kept token is
+// First the list of kept tokens, ascending: by a workgroup a sequence and key head whose keys are in LDS (select_device.cuh), for tables of more than 32768
+// tokens by slices of 8192, in a launch for each eight bits of the keys and one that takes what is above.
+// Then a launch that moves rows, in place: chunk c of a list, up to `chunk` tokens, reads rows that others may be about to write.  The i-th kept token is
 // at place i or behind it, so what chunk c writes, places c * chunk and on, is only ever read by itself and by chunks before it (the list's stretch
 // with tokens there ends before its own); all of a chunk's rows are in registers before its first write, and it writes when the chunks before it that
 // read there, two at most, have said that theirs are too.  Chunks are drawn by ticket: the one that is waited for has been drawn before, by a workgroup that is
@@ -29,50 +30,150 @@ struct EvictParams {
   int* flags;          // (rows, chunks) 1: read
   int* before;         // (rows, chunks + 1) how many tokens before place i * chunk are kept
   float* kept_weights; // (rows, keep)
+  unsigned* histograms;   // slices: two of (rows, slices, 256)
+  int4* found;            // ... (rows, slices) what of the threshold is known, how many that agree with it are wanted, how many before the slice are above it
+  int slices;
 };
 
-constexpr int kEvictThreads = 1024, kEvictKept = 12288;   // ... whose weights fit in LDS
+constexpr int kEvictThreads = 1024, kEvictKept = 32768;   // ... whose weights fit in LDS
+constexpr int kEvictSlice = 8192;                         // tokens
 
-// KEPT: the row's keys stay in LDS, else every round reads its weights again.
-template <bool KEPT>
-__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p, int chunk) {
-  extern __shared__ unsigned keys[];
+// Whether a row is to be cut.  One that is not gets its list here (all of a sequence that is short enough, or nothing: a sequence with pages given back has no
+// place for what it keeps), by the workgroups that are `one`; all of a row's workgroups see the same.
+__device__ __forceinline__ bool evict_begin(const EvictParams& p, int row, int length, bool one) {
   const PagedParams& c = p.cache;
-  const int row = blockIdx.x, seq = row / c.kv_heads, tid = threadIdx.x;
-  const int length = cached_length(c.lengths[seq], c.table_width, 1 << c.page_shift);
-  int* const kept = p.kept + (size_t)row * p.keep;
-  if (length <= p.keep) {
-    for (int i = tid; i < p.keep; i += kEvictThreads) kept[i] = i < length ? i : -1;
-    if (tid == 0) p.tokens[row] = 0;
-    return;
-  }
-  // a sequence with pages given back has no place for what it keeps: passed over
+  const int seq = row / c.kv_heads, tid = threadIdx.x;
   bool gone = false;
-  for (int i = tid; i << c.page_shift < length; i += kEvictThreads) gone |= (unsigned)c.table[(size_t)seq * c.table_row + i] >= (unsigned)c.pages;
-  if (__syncthreads_or(gone)) {
-    for (int i = tid; i < p.keep; i += kEvictThreads) kept[i] = -1;
-    if (tid == 0) p.tokens[row] = 0;
-    return;
+  if (length > p.keep)
+    for (int i = tid; i << c.page_shift < length; i += kEvictThreads) gone |= (unsigned)c.table[(size_t)seq * c.table_row + i] >= (unsigned)c.pages;
+  const bool cut = !__syncthreads_or(gone) && length > p.keep;
+  if (!one) return cut;
+  if (!cut) {
+    int* const kept = p.kept + (size_t)row * p.keep;
+    for (int i = tid; i < p.keep; i += kEvictThreads) kept[i] = length <= p.keep && i < length ? i : -1;
+  } else {
+    for (int i = tid; i < p.chunks; i += kEvictThreads) p.flags[(size_t)row * p.chunks + i] = 0;
   }
-  for (int i = tid; i < p.chunks; i += kEvictThreads) p.flags[(size_t)row * p.chunks + i] = 0;
-  if (tid == 0) p.tokens[row] = length, p.tickets[row] = 0;
-  const float* const weights = p.weights + (size_t)row * ((size_t)c.table_width << c.page_shift);
-  auto key_at = [&](int i) { return i < p.first || i >= length - p.recent ? kSelectAlways : select_key(__float_as_uint(weights[i])); };
-  if constexpr (KEPT) {
-    for (int i = tid; i < length; i += kEvictThreads) keys[i] = key_at(i);
-    __syncthreads();
+  if (tid == 0) p.tokens[row] = cut ? length : 0, p.tickets[row] = 0;
+  return cut;
+}
+
+// Keys of a row's weights, and what becomes of those that are taken.
+struct EvictRow {
+  const EvictParams& p;
+  int length, chunk_shift;
+  const unsigned* weights;
+  int *kept, *before;
+  unsigned* moved;
+  __device__ __forceinline__ EvictRow(const EvictParams& params, int row, int tokens, int shift) : p(params), length(tokens), chunk_shift(shift) {
+    weights = reinterpret_cast<const unsigned*>(p.weights) + (size_t)row * ((size_t)p.cache.table_width << p.cache.page_shift);
+    kept = p.kept + (size_t)row * p.keep, before = p.before + (size_t)row * (p.chunks + 1);
+    moved = reinterpret_cast<unsigned*>(p.kept_weights) + (size_t)row * p.keep;
   }
-  int* const before = p.before + (size_t)row * (p.chunks + 1);
-  float* const moved = p.kept_weights + (size_t)row * p.keep;
+  __device__ __forceinline__ u32x4 weights_at(int i) const { return four_of<true>(weights, i, length); }
+  __device__ __forceinline__ u32x4 keys_at(int i) const {
+    u32x4 four = weights_at(i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) four[j] = i + j >= length ? 0u : i + j < p.first || i + j >= length - p.recent ? kSelectAlways : select_key(four[j]);
+    return four;
+  }
+  __device__ __forceinline__ void take(int to, int i, unsigned weight) const { kept[to] = i, moved[to] = weight; }
+  __device__ __forceinline__ void place(int i, int taken) const {
+    if ((i & ((1 << chunk_shift) - 1)) == 0 && i >> chunk_shift <= p.chunks) before[i >> chunk_shift] = taken;
+  }
+};
+
+__device__ __forceinline__ int evict_length(const PagedParams& c, int row) { return cached_length(c.lengths[row / c.kv_heads], c.table_width, 1 << c.page_shift); }
+
+__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p, int chunk_shift) {
+  extern __shared__ __align__(16) unsigned keys[];
+  const int row = blockIdx.x, length = evict_length(p.cache, row);
+  if (!evict_begin(p, row, length, true)) return;
+  const EvictRow its(p, row, length, chunk_shift);
+#pragma unroll 4
+  for (int i = threadIdx.x * 4; i < length; i += kEvictThreads * 4) *reinterpret_cast<u32x4*>(keys + i) = its.keys_at(i);   // (a table's tokens are a multiple of 16)
+  __syncthreads();
   select_largest<kEvictThreads>(
-      length, p.keep, [&](int i) { return KEPT ? keys[i] : key_at(i); },
-      [&](int to, int i) {
-        kept[to] = i;
-        moved[to] = weights[i];
-      },
-      [&](int i0, int taken) {
-        if (i0 % chunk == 0 && i0 / chunk <= p.chunks && lane_id() == 0) before[i0 / chunk] = taken;
-      });
+      length, p.keep, [&](int i) { return i < length ? *reinterpret_cast<const u32x4*>(keys + i) : u32x4{}; }, [&](int i) { return its.weights_at(i); },
+      [&](int to, int i, unsigned weight) { its.take(to, i, weight); }, [&](int i, int taken) { its.place(i, taken); });
+}
+
+// Slices: launch STAGE 0 .. 3 counts the keys that agree with what is known of the threshold by their next eight bits, a histogram a slice; the next
+// launch's workgroups each add up all of their row's histograms and know eight bits more, how many of those that agree are wanted, and how many keys
+// in slices before theirs are above the threshold.  Launch 4 takes what is above it.  Nobody waits for another workgroup, and no sum depends on an order.
+template <int STAGE>
+__global__ __launch_bounds__(kEvictThreads) void evict_slice_kernel(EvictParams p, int chunk_shift) {
+  __shared__ unsigned histogram[256], total[4][256], earlier[4][256];
+  __shared__ int chosen[4];   // bin, still wanted, above it in earlier slices, equal to it there
+  const PagedParams& c = p.cache;
+  const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices, tid = threadIdx.x, lane = lane_id();
+  int length;
+  if constexpr (STAGE == 0) {
+    length = evict_length(c, row);
+    if (slice != 0 && slice * kEvictSlice >= length) return;
+    if (!evict_begin(p, row, length, slice == 0)) return;
+  } else {
+    length = p.tokens[row];
+    if (slice * kEvictSlice >= length) return;   // (0 where a row is not cut)
+  }
+  const EvictRow its(p, row, length, chunk_shift);
+  const int first = slice * kEvictSlice, used = min(length, first + kEvictSlice), slices = (length + kEvictSlice - 1) / kEvictSlice;
+  const size_t all = (size_t)c.seqs * c.kv_heads * p.slices;   // histograms of a launch
+  int4 found{0, p.keep, 0, 0};
+  if constexpr (STAGE > 0) {
+    if (STAGE > 1) found = p.found[(size_t)row * p.slices + slice];
+    const unsigned* from = p.histograms + ((STAGE - 1) % 2 * all + (size_t)row * p.slices) * 256;
+    unsigned sum = 0, mine = 0;
+    for (int s = tid >> 8; s < slices; s += 4) {
+      const unsigned n = from[s * 256 + (tid & 255)];
+      sum += n, mine += s < slice ? n : 0u;
+    }
+    total[tid >> 8][tid & 255] = sum, earlier[tid >> 8][tid & 255] = mine;
+    __syncthreads();
+    if (tid < kWave) {   // four bins a lane, from the largest down
+      unsigned four[4], before[4], in_lane = 0, before_in_lane = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int bin = 255 - (lane * 4 + j);
+        four[j] = total[0][bin] + total[1][bin] + total[2][bin] + total[3][bin];
+        before[j] = earlier[0][bin] + earlier[1][bin] + earlier[2][bin] + earlier[3][bin];
+        in_lane += four[j], before_in_lane += before[j];
+      }
+      unsigned above = (unsigned)wave_scan((int)in_lane) - in_lane, above_before = (unsigned)wave_scan((int)before_in_lane) - before_in_lane;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (above < (unsigned)found.y && above + four[j] >= (unsigned)found.y)
+          chosen[0] = 255 - (lane * 4 + j), chosen[1] = found.y - (int)above, chosen[2] = (int)above_before, chosen[3] = (int)before[j];
+        above += four[j], above_before += before[j];
+      }
+    }
+    __syncthreads();
+    found.x |= chosen[0] << (32 - 8 * STAGE), found.y = chosen[1], found.z += chosen[2], found.w = chosen[3];
+    if (STAGE < 4 && tid == 0) p.found[(size_t)row * p.slices + slice] = found;
+  }
+  if constexpr (STAGE < 4) {
+    constexpr int shift = 24 - 8 * STAGE;
+    for (int i = tid; i < 256; i += kEvictThreads) histogram[i] = 0;
+    __syncthreads();
+    u32x4 k[kEvictSlice / (kEvictThreads * 4)];
+#pragma unroll
+    for (int a = 0; a < kEvictSlice / (kEvictThreads * 4); ++a) k[a] = its.keys_at(first + (a * kEvictThreads + tid) * 4);
+#pragma unroll
+    for (int a = 0; a < kEvictSlice / (kEvictThreads * 4); ++a)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bool counts = first + (a * kEvictThreads + tid) * 4 + j < used;
+        if constexpr (STAGE > 0) counts = counts && (k[a][j] ^ (unsigned)found.x) >> (shift + 8) == 0;
+        if (counts) atomicAdd(&histogram[k[a][j] >> shift & 255], 1u);
+      }
+    __syncthreads();
+    unsigned* to = p.histograms + (STAGE % 2 * all + (size_t)row * p.slices + slice) * 256;
+    if (tid < 256) to[tid] = histogram[tid];
+  } else {
+    take_largest<kEvictThreads>(
+        first, used, p.keep, (unsigned)found.x, found.y, found.z, found.w, [&](int i) { return its.keys_at(i); }, [&](int i) { return its.weights_at(i); },
+        [&](int to, int i, unsigned weight) { its.take(to, i, weight); }, [&](int i, int taken) { its.place(i, taken); });
+  }
 }
 
 // Tokens of a chunk: eight 16-byte loads of 256 threads, of keys and values.
@@ -213,7 +314,8 @@ void launch_bounds(const EvictParams& p, int head_dim, unsigned grid, hipStream_
 
 struct Layout {
   long long rows, chunks;
-  size_t tickets, flags, before, kept_weights, bytes;   // where they begin, behind the rows' tokens
+  int slices;                                                              // of a row, 0: rows are in LDS
+  size_t tickets, flags, before, kept_weights, histograms, found, bytes;   // where they begin, behind the rows' tokens
 };
 Layout layout_of(const iex_paged_cache& c, int keep) {
   Layout l;
@@ -222,7 +324,11 @@ Layout layout_of(const iex_paged_cache& c, int keep) {
   l.flags = l.tickets + (size_t)l.rows * 4;
   l.before = l.flags + (size_t)l.rows * l.chunks * 4;
   l.kept_weights = l.before + (size_t)l.rows * (l.chunks + 1) * 4;
-  l.bytes = l.kept_weights + (size_t)l.rows * keep * 4;
+  const long long room = (long long)c.table_width * c.page_size;
+  l.slices = room <= kEvictKept ? 0 : ceil_div(room, kEvictSlice);
+  l.found = (l.kept_weights + (size_t)l.rows * keep * 4 + 15) / 16 * 16;
+  l.histograms = l.found + (size_t)l.rows * l.slices * 16;
+  l.bytes = l.histograms + (size_t)l.rows * l.slices * 2 * 256 * 4;
   return l;
 }
 // A table that holds no more than is kept: nothing ever moves.
@@ -246,11 +352,12 @@ extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, floa
               "evict_tokens: at least one token, the first and recent ones that are always kept among them (keep=%d first=%d recent=%d)", keep, first, recent);
   if (cache->seqs == 0 || cache->kv_heads == 0) return 0;
   IEX_REQUIRE(lengths == cache->lengths && kept && (weights || cache->table_width == 0), IEX_ERR_BAD_ARGUMENT, "evict_tokens: null pointer argument");
-  IEX_REQUIRE(aligned(weights, 4) && aligned(kept, 4), IEX_ERR_UNSUPPORTED, "evict_tokens: operands must be aligned to their elements");
+  IEX_REQUIRE(aligned(weights, 16), IEX_ERR_UNSUPPORTED, "evict_tokens: the weights must be 16-byte aligned");
+  IEX_REQUIRE(aligned(kept, 4), IEX_ERR_UNSUPPORTED, "evict_tokens: operands must be aligned to their elements");
   IEX_REQUIRE((long long)cache->pages * cache->page_size < (1ll << 31), IEX_ERR_TOO_LARGE, "evict_tokens: up to 2^31 tokens in a cache");
   const Layout l = layout_of(*cache, keep);
   const long long pages = ceil_div(keep, cache->page_size);
-  IEX_REQUIRE(l.rows < (1ll << 22) && l.rows * l.chunks < (1ll << 24) && (!cache->bounds || l.rows * pages < (1ll << 24)), IEX_ERR_TOO_LARGE,
+  IEX_REQUIRE(l.rows < (1ll << 22) && l.rows * l.slices < (1ll << 22) && l.rows * l.chunks < (1ll << 24) && (!cache->bounds || l.rows * pages < (1ll << 24)), IEX_ERR_TOO_LARGE,
               "evict_tokens: too many sequences, heads or tokens to keep");
   IEX_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= l.bytes, IEX_ERR_BAD_ARGUMENT, "evict_tokens: needs a 256-byte aligned workspace of %zu bytes", l.bytes);
   EvictParams p{};
@@ -261,11 +368,32 @@ extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, floa
   p.tokens = reinterpret_cast<int*>(ws), p.tickets = reinterpret_cast<int*>(ws + l.tickets), p.flags = reinterpret_cast<int*>(ws + l.flags);
   p.before = reinterpret_cast<int*>(ws + l.before), p.kept_weights = reinterpret_cast<float*>(ws + l.kept_weights);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const long long room = (long long)cache->table_width * cache->page_size;
-  const int chunk = chunk_of(*cache);
-  note_kernel("evict_select_kernel<%s>", room <= kEvictKept ? "kept" : "read again");
-  if (room <= kEvictKept) hipLaunchKernelGGL((evict_select_kernel<true>), dim3((unsigned)l.rows), dim3(kEvictThreads), room * 4, s, p, chunk);
-  else hipLaunchKernelGGL((evict_select_kernel<false>), dim3((unsigned)l.rows), dim3(kEvictThreads), 0, s, p, chunk);
+  p.found = reinterpret_cast<int4*>(ws + l.found), p.histograms = reinterpret_cast<unsigned*>(ws + l.histograms), p.slices = l.slices;
+  const size_t lds = (size_t)cache->table_width * cache->page_size * 4;
+  const int chunk_shift = log2_of(chunk_of(*cache));   // (a power of two)
+  if (l.slices) {
+    note_kernel("evict_slice_kernel x 5");
+    const dim3 slices((unsigned)(l.rows * l.slices)), threads(kEvictThreads);
+    hipLaunchKernelGGL((evict_slice_kernel<0>), slices, threads, 0, s, p, chunk_shift);
+    hipLaunchKernelGGL((evict_slice_kernel<1>), slices, threads, 0, s, p, chunk_shift);
+    hipLaunchKernelGGL((evict_slice_kernel<2>), slices, threads, 0, s, p, chunk_shift);
+    hipLaunchKernelGGL((evict_slice_kernel<3>), slices, threads, 0, s, p, chunk_shift);
+    hipLaunchKernelGGL((evict_slice_kernel<4>), slices, threads, 0, s, p, chunk_shift);
+  } else {
+    note_kernel("evict_select_kernel");
+    if (lds > 48 * 1024) {   // (beside what the selection has)
+      static thread_local unsigned long long raised = 0;   // on which devices
+      int device = 0;
+      if (int rc = check_hip(hipGetDevice(&device), "hipGetDevice")) return rc;
+      if (!(raised >> (device & 63) & 1)) {
+        if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(evict_select_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kEvictKept * 4),
+                               "hipFuncSetAttribute(LDS size)"))
+          return rc;
+        raised |= 1ull << (device & 63);
+      }
+    }
+    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)l.rows), dim3(kEvictThreads), lds, s, p, chunk_shift);
+  }
   if (int rc = check_hip(hipGetLastError(), "evict_tokens launch")) return rc;
   if (never(*cache, keep) || cache->pages == 0) return 0;
   const unsigned grid = (unsigned)(l.rows * l.chunks);

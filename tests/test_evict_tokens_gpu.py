@@ -107,6 +107,22 @@ def test_many_chunks(ops, dev, dtype, e8, dim):
         check(ops, c, weights, 1500, 100, 3)
 
 
+@pytest.mark.parametrize("keep,recent,first", [(1, 0, 0), (16383, 300, 2), (8192, 8192, 0), (20000, 0, 19000), (33000, 1, 1)])
+def test_rows_in_slices(ops, dev, keep, recent, first):
+    """Tables of more than 32768 tokens: lengths that end a slice, are short of one, fill the table; equal keys over slices' ends, and rows of nothing else."""
+    lengths = [34000, 8192, 8193, 16384, 0, 5, 33024, 1 << 30, 33001]
+    c = Cache(dev, [min(n, 34048) for n in lengths], 2, 64, 256, F16, poison=False, width=133, bounds=True)
+    c.lengths[7] = lengths[7]
+    weights = random_weights(c)
+    weights[2, 0] = 0.5
+    weights[3, :, 8000:8400] = 7e4
+    weights[3, 1, 8100:16300] = 7e4
+    weights[0, 0], weights[0, 0, 5000:30000:7] = -0.0, 1e-30
+    weights[7, 1, ::3] = math.nan
+    check(ops, c, weights, keep, recent, first, c.bounds)
+    assert "evict_slice_kernel" in _lib.last_kernels()
+
+
 def test_ties_and_values_that_are_not_numbers(ops, dev):
     """Equal weights: the earlier ones; negative ones, infinities, zeros of both signs; NaN is larger than everything."""
     c = Cache(dev, [200] * 6, 1, 64, 16, F16, poison=False)
@@ -227,7 +243,7 @@ def test_kernels_and_changes_are_noted(ops, dev):
     weights = random_weights(c)
     versions = [x._version for x in (c.keys, c.values, c.lengths, weights, c.bounds)]
     evict(ops, c, weights, 50, 10, 0, c.bounds)
-    for name in ("evict_select_kernel<kept>", "evict_move_kernel<64, 16>", "evict_bounds_kernel<f16, 64, 16>"):
+    for name in ("evict_select_kernel", "evict_move_kernel<64, 16>", "evict_bounds_kernel<f16, 64, 16>"):
         assert name in _lib.last_kernels()
     assert all(x._version > v for x, v in zip((c.keys, c.values, c.lengths, weights, c.bounds), versions))
 
