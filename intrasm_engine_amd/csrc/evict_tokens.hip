@@ -10,7 +10,9 @@
 // read there, two at most, have said that theirs are too.  Chunks are drawn by ticket: the one that is waited for has been drawn before, by a workgroup that is
 // running and that waits for nobody before it has read, so every wait ends.
 //
-// What bounds it: memory, kept rows read and written once.
+// What bounds it: memory, kept rows read and written once: 64 sequences of 1500 .. 4224 tokens to 2048, 8 key heads of 128 in 16 bits 149 us = 5.1 TB/s,
+// selection 16; 131071 tokens to 32768, every fourth row of 256 bytes, 66 us = 4.1 TB/s, selection 34 in five launches (by one workgroup a row, whose CU reads
+// the weights again in every round, 143); 700 tokens to 512, 32 key heads 6.7 and 7.1.
 #include "paged_cache_host.h"
 #include "select_device.cuh"
 
@@ -38,21 +40,92 @@ struct EvictParams {
 constexpr int kEvictThreads = 1024, kEvictKept = 32768;   // ... whose weights fit in LDS
 constexpr int kEvictSlice = 8192;                         // tokens
 
+// Four words from place i on of a 16-byte aligned row of `used`, 0 behind it.
+__device__ __forceinline__ u32x4 four_of(const unsigned* row, int i, int used) {
+  if (i + 4 <= used) return *reinterpret_cast<const u32x4*>(row + i);
+  return u32x4{i < used ? row[i] : 0u, i + 1 < used ? row[i + 1] : 0u, i + 2 < used ? row[i + 2] : 0u, 0u};
+}
+
+// The keys of places first .. used - 1 that are above a threshold, and those that equal it as long as fewer than `need` of the row's do before them, in
+// ascending order: emit(to, i, payload), to = how many are taken before i.  aboves, equals: how many of the row's keys before `first` are above it, and equal it.
+// place(i, before): at every fourth place how many are taken below it.  Returns how many are up to the end.
+template <int THREADS, typename KEYS, typename PAYLOADS, typename EMIT, typename PLACE>
+__device__ __forceinline__ int take_largest(int first, int used, int count, unsigned threshold, int need, int aboves, int equals, KEYS keys, PAYLOADS payloads, EMIT emit,
+                                            PLACE place) {
+  constexpr int WAVES = THREADS / kWave, AHEAD = 4, STEP = 4 * kWave;
+  __shared__ int totals[2][WAVES];
+  const int lane = lane_id(), wave = uniform(threadIdx.x >> 6);
+  const int stretch = (used - first + THREADS * 4 - 1) / (THREADS * 4) * STEP, begin = min(used, first + wave * stretch), end = min(used, begin + stretch);
+  auto marks = [&](const u32x4& k) {   // (those that equal it, 256 of a step at most) << 16 | those above
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n += (k[j] > threshold ? 1 : 0) + (k[j] == threshold && k[j] != 0 ? 1 << 16 : 0);
+    return n;
+  };
+  int above = 0, equal = 0;   // of this lane
+  for (int i0 = begin + lane * 4; i0 < end; i0 += AHEAD * STEP) {
+    u32x4 k[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) k[a] = i0 + a * STEP < end ? keys(i0 + a * STEP) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int n = marks(k[a]);
+      above += n & 0xFFFF, equal += n >> 16;
+    }
+  }
+  above = wave_scan(above), equal = wave_scan(equal);
+  if (lane == kWave - 1) totals[0][wave] = above, totals[1][wave] = equal;
+  __syncthreads();
+  int all_above = aboves, all_equal = equals;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) aboves += totals[0][w], equals += totals[1][w];   // before this wavefront's stretch
+    all_above += totals[0][w], all_equal += totals[1][w];
+  }
+  for (int i0 = begin; i0 < end; i0 += AHEAD * STEP) {
+    u32x4 k[AHEAD], what[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = i0 + a * STEP + lane * 4;
+      k[a] = what[a] = u32x4{0u, 0u, 0u, 0u};
+      if (i < end) k[a] = keys(i), what[a] = payloads(i);
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (i0 + a * STEP >= end) break;
+      const int i = i0 + a * STEP + lane * 4, mine = marks(k[a]), upto = wave_scan(mine);
+      int above_before = aboves + ((upto - mine) & 0xFFFF), equal_before = equals + ((upto - mine) >> 16);
+      if (i < end) place(i, above_before + min(equal_before, need));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool more = k[a][j] > threshold, same = k[a][j] == threshold && k[a][j] != 0;
+        const int to = above_before + min(equal_before, need);
+        if ((more || (same && equal_before < need)) && to < count) emit(to, i + j, what[a][j]);
+        above_before += more, equal_before += same;
+      }
+      const int step = bcast_i(upto, kWave - 1);
+      aboves += step & 0xFFFF, equals += step >> 16;
+    }
+  }
+  return min(count, all_above + min(all_equal, need));
+}
+
 // Whether a row is to be cut.  One that is not gets its list here (all of a sequence that is short enough, or nothing: a sequence with pages given back has no
 // place for what it keeps), by the workgroups that are `one`; all of a row's workgroups see the same.
+template <int THREADS>
 __device__ __forceinline__ bool evict_begin(const EvictParams& p, int row, int length, bool one) {
   const PagedParams& c = p.cache;
   const int seq = row / c.kv_heads, tid = threadIdx.x;
   bool gone = false;
   if (length > p.keep)
-    for (int i = tid; i << c.page_shift < length; i += kEvictThreads) gone |= (unsigned)c.table[(size_t)seq * c.table_row + i] >= (unsigned)c.pages;
+    for (int i = tid; i << c.page_shift < length; i += THREADS) gone |= (unsigned)c.table[(size_t)seq * c.table_row + i] >= (unsigned)c.pages;
   const bool cut = !__syncthreads_or(gone) && length > p.keep;
   if (!one) return cut;
   if (!cut) {
     int* const kept = p.kept + (size_t)row * p.keep;
-    for (int i = tid; i < p.keep; i += kEvictThreads) kept[i] = length <= p.keep && i < length ? i : -1;
+    for (int i = tid; i < p.keep; i += THREADS) kept[i] = length <= p.keep && i < length ? i : -1;
   } else {
-    for (int i = tid; i < p.chunks; i += kEvictThreads) p.flags[(size_t)row * p.chunks + i] = 0;
+    for (int i = tid; i < p.chunks; i += THREADS) p.flags[(size_t)row * p.chunks + i] = 0;
   }
   if (tid == 0) p.tokens[row] = cut ? length : 0, p.tickets[row] = 0;
   return cut;
@@ -70,7 +143,7 @@ struct EvictRow {
     kept = p.kept + (size_t)row * p.keep, before = p.before + (size_t)row * (p.chunks + 1);
     moved = reinterpret_cast<unsigned*>(p.kept_weights) + (size_t)row * p.keep;
   }
-  __device__ __forceinline__ u32x4 weights_at(int i) const { return four_of<true>(weights, i, length); }
+  __device__ __forceinline__ u32x4 weights_at(int i) const { return four_of(weights, i, length); }
   __device__ __forceinline__ u32x4 keys_at(int i) const {
     u32x4 four = weights_at(i);
 #pragma unroll
@@ -85,17 +158,21 @@ struct EvictRow {
 
 __device__ __forceinline__ int evict_length(const PagedParams& c, int row) { return cached_length(c.lengths[row / c.kv_heads], c.table_width, 1 << c.page_shift); }
 
-__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p, int chunk_shift) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictParams p, int chunk_shift) {
   extern __shared__ __align__(16) unsigned keys[];
   const int row = blockIdx.x, length = evict_length(p.cache, row);
-  if (!evict_begin(p, row, length, true)) return;
   const EvictRow its(p, row, length, chunk_shift);
+  if (length > p.keep) {   // (beside the look at the pages)
 #pragma unroll 4
-  for (int i = threadIdx.x * 4; i < length; i += kEvictThreads * 4) *reinterpret_cast<u32x4*>(keys + i) = its.keys_at(i);   // (a table's tokens are a multiple of 16)
-  __syncthreads();
-  select_largest<kEvictThreads>(
-      length, p.keep, [&](int i) { return i < length ? *reinterpret_cast<const u32x4*>(keys + i) : u32x4{}; }, [&](int i) { return its.weights_at(i); },
-      [&](int to, int i, unsigned weight) { its.take(to, i, weight); }, [&](int i, int taken) { its.place(i, taken); });
+    for (int i = threadIdx.x * 4; i < length; i += THREADS * 4) *reinterpret_cast<u32x4*>(keys + i) = its.keys_at(i);   // (a table's tokens are a multiple of 16)
+  }
+  if (!evict_begin<THREADS>(p, row, length, true)) return;
+  select_largest<THREADS>(
+      length, p.keep, [&](int i) { return keys[i]; }, [&](int to, int i) { its.take(to, i, its.weights[i]); },
+      [&](int i, int taken) {
+        if (lane_id() == 0) its.place(i, taken);
+      });
 }
 
 // Slices: launch STAGE 0 .. 3 counts the keys that agree with what is known of the threshold by their next eight bits, a histogram a slice; the next
@@ -111,7 +188,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_slice_kernel(EvictParams 
   if constexpr (STAGE == 0) {
     length = evict_length(c, row);
     if (slice != 0 && slice * kEvictSlice >= length) return;
-    if (!evict_begin(p, row, length, slice == 0)) return;
+    if (!evict_begin<kEvictThreads>(p, row, length, slice == 0)) return;
   } else {
     length = p.tokens[row];
     if (slice * kEvictSlice >= length) return;   // (0 where a row is not cut)
@@ -176,8 +253,9 @@ __global__ __launch_bounds__(kEvictThreads) void evict_slice_kernel(EvictParams 
   }
 }
 
-// Tokens of a chunk: eight 16-byte loads of 256 threads, of keys and values.
-constexpr int evict_chunk(int row_bytes) { return 8 * 256 * 16 / (2 * row_bytes) < 64 ? 64 : 8 * 256 * 16 / (2 * row_bytes); }
+// Tokens of a chunk: sixteen 16-byte loads of 256 threads, of keys and values (131071 -> 32768 tokens, 8 key heads of 128: 66 us, by eight loads 80), and no
+// more than there are threads.
+constexpr int evict_chunk(int row_bytes) { return 16 * 256 * 16 / (2 * row_bytes) > 256 ? 256 : 16 * 256 * 16 / (2 * row_bytes); }
 
 // ROW: bytes of a token's key or value of one head.
 template <int ROW, bool E8>
@@ -331,6 +409,9 @@ Layout layout_of(const iex_paged_cache& c, int keep) {
   l.bytes = l.histograms + (size_t)l.rows * l.slices * 2 * 256 * 4;
   return l;
 }
+// Workgroups of 512 threads where there are many more rows than CUs, which then have several at a time, or rows are short (both launches, 512 rows of 1024
+// tokens 15.9 us, 2048 of 8192 88; by 1024 threads 17.5 and 99); else of 1024 (8 rows of 4096 16.9, 512 of 8192 32.5; by 512 18.4 and 34.5).
+bool few_threads(long long rows, long long room) { return room <= 1024 || (room <= 12288 && rows * 10 > room); }
 // A table that holds no more than is kept: nothing ever moves.
 bool never(const iex_paged_cache& c, int keep) { return (long long)c.table_width * c.page_size <= keep; }
 
@@ -369,7 +450,8 @@ extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, floa
   p.before = reinterpret_cast<int*>(ws + l.before), p.kept_weights = reinterpret_cast<float*>(ws + l.kept_weights);
   hipStream_t s = static_cast<hipStream_t>(stream);
   p.found = reinterpret_cast<int4*>(ws + l.found), p.histograms = reinterpret_cast<unsigned*>(ws + l.histograms), p.slices = l.slices;
-  const size_t lds = (size_t)cache->table_width * cache->page_size * 4;
+  const long long room = (long long)cache->table_width * cache->page_size;
+  const size_t lds = room * 4;
   const int chunk_shift = log2_of(chunk_of(*cache));   // (a power of two)
   if (l.slices) {
     note_kernel("evict_slice_kernel x 5");
@@ -386,13 +468,14 @@ extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, floa
       int device = 0;
       if (int rc = check_hip(hipGetDevice(&device), "hipGetDevice")) return rc;
       if (!(raised >> (device & 63) & 1)) {
-        if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(evict_select_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kEvictKept * 4),
+        if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(evict_select_kernel<kEvictThreads>), hipFuncAttributeMaxDynamicSharedMemorySize, kEvictKept * 4),
                                "hipFuncSetAttribute(LDS size)"))
           return rc;
         raised |= 1ull << (device & 63);
       }
     }
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)l.rows), dim3(kEvictThreads), lds, s, p, chunk_shift);
+    if (few_threads(l.rows, room)) hipLaunchKernelGGL((evict_select_kernel<512>), dim3((unsigned)l.rows), dim3(512), lds, s, p, chunk_shift);
+    else hipLaunchKernelGGL((evict_select_kernel<kEvictThreads>), dim3((unsigned)l.rows), dim3(kEvictThreads), lds, s, p, chunk_shift);
   }
   if (int rc = check_hip(hipGetLastError(), "evict_tokens launch")) return rc;
   if (never(*cache, keep) || cache->pages == 0) return 0;

@@ -41,12 +41,17 @@ struct PagedAttentionParams {
   float* stats;
   // attention that keeps account (WEIGH below)
   float* weights;     // (seqs, kv_heads, tokens of a table)
-  float* scores;      // (seqs, heads, tokens of a table)
+  float* scores;      // (seqs, kv_heads, tokens of a table / 16, heads of a key head, 16): what a wavefront leaves of a tile lies together
   float* row_stats;   // per sequence and query head maximum and sum, of rows of one part
   int at_once;        // rows are whole and their queries together: no second launch
 };
 
 __device__ __forceinline__ size_t table_tokens(const PagedParams& c) { return (size_t)c.table_width << c.page_shift; }
+// The scores of a sequence and key head; query i's with four tokens from t on are at account_place(t, i).
+__device__ __forceinline__ float* account_scores(const PagedAttentionParams& p, int seq, int kv_head) {
+  return p.scores + ((size_t)seq * p.cache.kv_heads + kv_head) * table_tokens(p.cache) * p.group;
+}
+__device__ __forceinline__ size_t account_place(const PagedAttentionParams& p, int t, int i) { return (size_t)(t & ~15) * p.group + i * 16 + (t & 15); }
 
 // What stands in the place of the score of a token that is not attended to: a NaN that no product of 16-bit or 8-bit operands has, so that a row whose
 // scores are NaN or infinite leaves no trace in what it does not attend to.
@@ -177,7 +182,9 @@ constexpr int paged_sum_gap(int head_dim) { return head_dim == 64 ? 0 : 16; }
 constexpr int paged_sum_pitch(int head_dim) { return head_dim + 3 * paged_sum_gap(head_dim) + 1; }
 
 // WEIGH: scores are left behind too, 4 bytes a token and query head, and become weights when the row's maximum and sum are known: here, by the
-// one workgroup that has the row, or in paged_account_kernel.
+// one workgroup that has the row, or in paged_account_kernel.  (64 x 2049 .. 4224 tokens, 32 heads over 8: 166 us, 132 without these 25 MB of
+// stores; a row for every head instead of tiles 168, held back in LDS to the end of a part 162, and then 700 tokens 13.2 for 12.4, by buffer address without a
+// branch 168, past the caches 171.)
 template <bool BF16, int D, bool E8, int WAVES, bool WEIGH>
 __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attention_kernel(PagedAttentionParams p) {
   typedef unsigned short u16;
@@ -387,7 +394,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
     }
     if constexpr (WEIGH) {
       if (col < rows) {
-        float* to = p.scores + ((size_t)seq * p.heads + kv_head * p.group + group_tile * 16 + col) * table_tokens(cache) + t + g * 4;
+        float* const to = account_scores(p, seq, kv_head) + ((long long)t * p.group + (group_tile * 16 + col) * 16 + g * 4);
 #pragma unroll
         for (int a = 0; a < SUB; ++a)
           if (t + a * 16 < end) {
@@ -396,7 +403,7 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
 #pragma unroll
               for (int r = 0; r < 4; ++r) left[r] = g * 4 + r >= w.valid[a] ? __uint_as_float(kNoScore) : left[r];
             }
-            *reinterpret_cast<f32x4*>(to + a * 16) = left;
+            *reinterpret_cast<f32x4*>(to + (long long)a * 16 * p.group) = left;
           }
       }
     }
@@ -535,12 +542,12 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
   if constexpr (WEIGH) {
     if (!p.at_once) return;
     __syncthreads();   // (the wavefronts' scores are there too)
-    const float* from = p.scores + ((size_t)seq * p.heads + kv_head * p.group) * table_tokens(cache);
+    const float* from = account_scores(p, seq, kv_head);
     float* to = p.weights + ((size_t)seq * cache.kv_heads + kv_head) * table_tokens(cache);
     for (int t = threadIdx.x * 4; t < length; t += WAVES * 256) {
       f32x4 got = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-      for (int row = 0; row < rows; ++row) QueryWeights(shares[row]).add(got, *reinterpret_cast<const f32x4*>(from + row * table_tokens(cache) + t), p.scale_log2);
+      for (int row = 0; row < rows; ++row) QueryWeights(shares[row]).add(got, *reinterpret_cast<const f32x4*>(from + account_place(p, t, row)), p.scale_log2);
       add_weights(to, t, length, got);
     }
   }
@@ -661,12 +668,12 @@ __global__ __launch_bounds__(256) void paged_account_kernel(PagedAttentionParams
     if (lane == 0) shares[i] = float2{its.shift, its.share};
   }
   __syncthreads();
-  const float* from = p.scores + ((size_t)seq * p.heads + kv_head * p.group) * table_tokens(cache);
+  const float* from = account_scores(p, seq, kv_head);
   float* to = p.weights + ((size_t)seq * cache.kv_heads + kv_head) * table_tokens(cache);
   for (; t < length; t += side * kAccountTokens) {
     f32x4 got = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int i = 0; i < p.group; ++i) QueryWeights(shares[i]).add(got, *reinterpret_cast<const f32x4*>(from + i * table_tokens(cache) + t), p.scale_log2);
+    for (int i = 0; i < p.group; ++i) QueryWeights(shares[i]).add(got, *reinterpret_cast<const f32x4*>(from + account_place(p, t, i)), p.scale_log2);
     add_weights(to, t, length, got);
   }
 }

@@ -60,21 +60,19 @@ Split split_of(const iex_paged_cache& c, int heads, int count) {
 size_t partial_floats(const iex_paged_cache& c, const Split& s) { return (size_t)s.workgroups * s.pitch * c.head_dim; }
 
 // LDS: the wavefronts' sums, maxima and sums of weights; the shares of the queries.
-inline int attention_lds(const Split& s, int head_dim, int waves, bool weigh) {
-  return waves * s.pitch * (paged_sum_pitch(head_dim) + 2) * 4 + (weigh ? (2 * s.pitch + 1) * 4 : 0);
+inline int attention_lds(int pitch, int head_dim, int waves, bool weigh) {
+  return waves * pitch * (paged_sum_pitch(head_dim) + 2) * 4 + (weigh ? (2 * pitch + 1) * 4 : 0);
 }
 template <bool BF16, int D, bool E8, int WAVES, bool WEIGH>
 int launch_attention(const PagedAttentionParams& p, const Split& s, hipStream_t stream) {
-  const int lds = attention_lds(s, D, WAVES, WEIGH);
+  const int lds = attention_lds(s.pitch, D, WAVES, WEIGH);
   auto kern = paged_attention_kernel<BF16, D, E8, WAVES, WEIGH>;
   if (lds > 64 * 1024) {
     static thread_local unsigned long long raised = 0;   // per instantiation: on which devices
     int device = 0;
     if (int rc = check_hip(hipGetDevice(&device), "hipGetDevice")) return rc;
     if (!(raised >> (device & 63) & 1)) {
-      Split most = s;
-      most.pitch = 16;
-      if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, attention_lds(most, D, WAVES, WEIGH)),
+      if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, attention_lds(16, D, WAVES, WEIGH)),
                              "hipFuncSetAttribute(LDS size)"))
         return rc;
       raised |= 1ull << (device & 63);

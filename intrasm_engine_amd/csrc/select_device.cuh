@@ -4,135 +4,49 @@
 
 namespace iex {
 
-// Four words from place i on of a row of `used`, 0 behind it.  ALIGNED: 16-byte aligned rows.
-template <bool ALIGNED>
-__device__ __forceinline__ u32x4 four_of(const unsigned* row, int i, int used) {
-  typedef u32x4 AnyFour __attribute__((aligned(4)));
-  if (i + 4 <= used) {
-    if constexpr (ALIGNED) return *reinterpret_cast<const u32x4*>(row + i);
-    else return *reinterpret_cast<const AnyFour*>(row + i);
-  }
-  return u32x4{i < used ? row[i] : 0u, i + 1 < used ? row[i + 1] : 0u, i + 2 < used ? row[i + 2] : 0u, 0u};
-}
-
-// The keys of places first .. used - 1 that are above a threshold, and those that equal it as long as fewer than `need` of the row's do before them, in
-// ascending order: emit(to, i, payload), to = how many are taken before i.  aboves, equals: how many of the row's keys before `first` are above it, and equal it.
-// place(i, before): at every fourth place how many are taken below it.  Returns how many are up to the end.
-template <int THREADS, typename KEYS, typename PAYLOADS, typename EMIT, typename PLACE>
-__device__ __forceinline__ int take_largest(int first, int used, int count, unsigned threshold, int need, int aboves, int equals, KEYS keys, PAYLOADS payloads, EMIT emit,
-                                            PLACE place) {
-  constexpr int WAVES = THREADS / kWave, AHEAD = 4, STEP = 4 * kWave;
-  __shared__ int totals[2][WAVES];
-  const int lane = lane_id(), wave = uniform(threadIdx.x >> 6);
-  const int stretch = (used - first + THREADS * 4 - 1) / (THREADS * 4) * STEP, begin = min(used, first + wave * stretch), end = min(used, begin + stretch);
-  auto marks = [&](const u32x4& k) {   // (those that equal it, 256 of a step at most) << 16 | those above
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) n += (k[j] > threshold ? 1 : 0) + (k[j] == threshold && k[j] != 0 ? 1 << 16 : 0);
-    return n;
-  };
-  int above = 0, equal = 0;   // of this lane
-  for (int i0 = begin + lane * 4; i0 < end; i0 += AHEAD * STEP) {
-    u32x4 k[AHEAD];
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) k[a] = i0 + a * STEP < end ? keys(i0 + a * STEP) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int n = marks(k[a]);
-      above += n & 0xFFFF, equal += n >> 16;
-    }
-  }
-  above = wave_scan(above), equal = wave_scan(equal);
-  if (lane == kWave - 1) totals[0][wave] = above, totals[1][wave] = equal;
-  __syncthreads();
-  int all_above = aboves, all_equal = equals;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < wave) aboves += totals[0][w], equals += totals[1][w];   // before this wavefront's stretch
-    all_above += totals[0][w], all_equal += totals[1][w];
-  }
-  for (int i0 = begin; i0 < end; i0 += AHEAD * STEP) {
-    u32x4 k[AHEAD], what[AHEAD];
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int i = i0 + a * STEP + lane * 4;
-      k[a] = what[a] = u32x4{0u, 0u, 0u, 0u};
-      if (i < end) k[a] = keys(i), what[a] = payloads(i);
-    }
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      if (i0 + a * STEP >= end) break;
-      const int i = i0 + a * STEP + lane * 4, mine = marks(k[a]), upto = wave_scan(mine);
-      int above_before = aboves + ((upto - mine) & 0xFFFF), equal_before = equals + ((upto - mine) >> 16);
-      if (i < end) place(i, above_before + min(equal_before, need));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool more = k[a][j] > threshold, same = k[a][j] == threshold && k[a][j] != 0;
-        const int to = above_before + min(equal_before, need);
-        if ((more || (same && equal_before < need)) && to < count) emit(to, i + j, what[a][j]);
-        above_before += more, equal_before += same;
-      }
-      const int step = bcast_i(upto, kWave - 1);
-      aboves += step & 0xFFFF, equals += step >> 16;
-    }
-  }
-  return min(count, all_above + min(all_equal, need));
-}
-
-// The `count` largest of `used` keys (all that are not 0 where there are no more): emit(to, i, payload) for each, to = 0, 1 .. in ascending order of i, by any
-// thread; equal keys: the lower places.  keys(i) and payloads(i): four of them from place i on, a multiple of 4; keys behind the row are 0.
-// place(i, before): at every fourth place how many were taken below it.  Returns how many were taken.
-//
-// The count-th largest key by three rounds of histograms, of 11, 11 and 10 bits: the first tells exponents and two bits of the fraction, so that weights
-// and scores, which share their leading bits, spread over some bins (lanes that meet in one are added one after the other: 64 clocks where all do).
-template <int THREADS, typename KEYS, typename PAYLOADS, typename EMIT, typename PLACE>
-__device__ __forceinline__ int select_largest(int used, int count, KEYS keys, PAYLOADS payloads, EMIT emit, PLACE place) {
-  constexpr int WAVES = THREADS / kWave, BINS = 2048, EACH = BINS / THREADS, AHEAD = 4;
-  static_assert(BINS % THREADS == 0 && EACH >= 1, "bins of a thread");
-  __shared__ unsigned histogram[BINS];
-  __shared__ int chosen[3], sums[WAVES];
+// The `count` largest of `used` keys (all that are not 0 where there are no more): emit(to, i) for each, to = 0, 1 .. in ascending order of i, by any
+// thread; equal keys: the lower places.  window(i0, before): before each 64 places from i0 on how many were taken below them (all lanes of a wavefront, not
+// every workgroup's).  By four rounds of histograms of 8 bits.  Returns how many were taken.
+template <int THREADS, typename KEY, typename EMIT, typename WINDOW>
+__device__ __forceinline__ int select_largest(int used, int count, KEY key_of, EMIT emit, WINDOW window) {
+  constexpr int WAVES = THREADS / kWave;
+  __shared__ unsigned histogram[256];
+  __shared__ int chosen[3], totals[2][WAVES];
   const int tid = threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
 
   // ---- the count-th largest key ----
   unsigned threshold = 0;
   int need = count;   // of the keys that agree with it in the bits found so far, the need-th largest
   if (used > count) {
-    for (int i = tid; i < BINS; i += THREADS) histogram[i] = 0;
-    __syncthreads();
-#pragma unroll 1
-    for (int round = 0; round < 3; ++round) {
-      const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round == 2 ? BINS / 2 : BINS, known = round == 1 ? 21 : 10;
-      for (int i0 = tid * 4; i0 < used; i0 += AHEAD * THREADS * 4) {
-        u32x4 k[AHEAD];
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) k[a] = keys(i0 + a * THREADS * 4);
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)   // (what is behind the row counts as keys of 0, below all that are taken)
-            if (i0 + a * THREADS * 4 < used && (round == 0 || (k[a][j] ^ threshold) >> known == 0)) atomicAdd(&histogram[k[a][j] >> shift & (bins - 1)], 1u);
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) histogram[tid] = 0;
+      __syncthreads();
+      for (int i0 = wave * kWave; i0 < used; i0 += THREADS) {
+        const int i = i0 + lane;
+        const unsigned key = i < used ? key_of(i) : 0u;
+        const bool mine = i < used && (shift == 24 || key >> (shift + 8) == threshold >> (shift + 8));
+        const int bin = key >> shift & 255;
+        // scores of a row share their leading bits: the lanes that agree with the first one are counted at once
+        const unsigned long long some = __ballot(mine);
+        if (some) {
+          const int leader = __ffsll(some) - 1, its = __builtin_amdgcn_readlane(bin, leader);
+          const unsigned long long same = __ballot(mine && bin == its);
+          if (lane == leader) atomicAdd(&histogram[its], (unsigned)__popcll(same));
+          else if (mine && bin != its) atomicAdd(&histogram[bin], 1u);
+        }
       }
       __syncthreads();
-      // a thread's bins, from the largest down, and how many keys are in the ones above
-      unsigned its[EACH], sum = 0;
+      if (wave == 0) {   // four bins a lane, from the largest down
+        unsigned four[4], mine = 0;
 #pragma unroll
-      for (int j = 0; j < EACH; ++j) {
-        const int bin = bins - 1 - (tid * EACH + j);
-        its[j] = bin >= 0 ? histogram[bin] : 0u;
-        if (bin >= 0) histogram[bin] = 0;   // (for the next round)
-        sum += its[j];
-      }
-      const int upto = wave_scan((int)sum);
-      if (lane == kWave - 1) sums[wave] = upto;
-      __syncthreads();
-      unsigned above = (unsigned)upto - sum;
+        for (int j = 0; j < 4; ++j) mine += four[j] = histogram[255 - (lane * 4 + j)];
+        unsigned above = (unsigned)wave_scan((int)mine) - mine;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) above += w < wave ? (unsigned)sums[w] : 0u;
-#pragma unroll
-      for (int j = 0; j < EACH; ++j) {
-        if (above < (unsigned)need && above + its[j] >= (unsigned)need)
-          chosen[0] = bins - 1 - (tid * EACH + j), chosen[1] = need - (int)above, chosen[2] = above + its[j] == (unsigned)need;
-        above += its[j];
+        for (int j = 0; j < 4; ++j) {
+          if (above < (unsigned)need && above + four[j] >= (unsigned)need)
+            chosen[0] = 255 - (lane * 4 + j), chosen[1] = need - (int)above, chosen[2] = above + four[j] == (unsigned)need;
+          above += four[j];
+        }
       }
       __syncthreads();
       threshold |= (unsigned)chosen[0] << shift;
@@ -143,7 +57,40 @@ __device__ __forceinline__ int select_largest(int used, int count, KEYS keys, PA
       }
     }
   }
-  return take_largest<THREADS>(0, used, count, threshold, need, 0, 0, keys, payloads, emit, place);
+
+  // ---- what is above it, and the first `need` that equal it, in ascending order: a wavefront has a stretch ----
+  const int stretch = (used + THREADS - 1) / THREADS * kWave, begin = min(used, wave * stretch), end = min(used, begin + stretch);
+  int above = 0, equal = 0;
+  for (int i0 = begin; i0 < end; i0 += kWave) {
+    const unsigned key = i0 + lane < end ? key_of(i0 + lane) : 0u;
+    above += __popcll(__ballot(key > threshold));
+    equal += __popcll(__ballot(key == threshold && key != 0));
+  }
+  if (lane == 0) totals[0][wave] = above, totals[1][wave] = equal;
+  __syncthreads();
+  int written = 0, equals = 0, all = 0;   // before this wavefront's stretch; all pages that are taken
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int taken = min(totals[1][w], max(0, need - equals));
+    if (w < wave) written += totals[0][w] + taken;
+    all += totals[0][w] + taken;
+    equals += totals[1][w];
+  }
+  equals = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) equals += w < wave ? totals[1][w] : 0;
+  for (int i0 = begin; i0 < end; i0 += kWave) {
+    window(i0, min(written, count));
+    const unsigned key = i0 + lane < end ? key_of(i0 + lane) : 0u;
+    const bool same = key == threshold && key != 0;
+    const unsigned long long sames = __ballot(same), below = (1ull << lane) - 1;
+    const bool take = key > threshold || (same && equals + __popcll(sames & below) < need);
+    const unsigned long long takes = __ballot(take);
+    const int to = written + __popcll(takes & below);
+    if (take && to < count) emit(to, i0 + lane);
+    written += __popcll(takes), equals += __popcll(sames);
+  }
+  return all;
 }
 
 }  // namespace iex

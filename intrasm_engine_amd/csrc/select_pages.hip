@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void page_score_kernel(Selec
 template <bool KEPT, bool SCORED, bool BF16, int D>
 __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParams p) {
   constexpr int WAVES = kSelectThreads / kWave;
-  extern __shared__ __align__(16) unsigned kept[];
+  extern __shared__ unsigned kept[];
   __shared__ double weights[SCORED ? 2 : 2 * D];
   const PagedParams& c = p.cache;
   const int row = blockIdx.x, seq = row / c.kv_heads, tid = threadIdx.x, wave = uniform(tid >> 6);
@@ -209,9 +209,9 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
     for (int i = tid; i < used; i += kSelectThreads) kept[i] = keys[i];
   }
   __syncthreads();
-  const int all = select_largest<kSelectThreads>(
-      used, p.count, [&](int i) { return KEPT ? four_of<true>(kept, i, used) : four_of<false>(keys, i, used); }, [](int) { return u32x4{}; },
-      [&](int to, int i, unsigned) { out[to] = i; }, [](int, int) {});
+  auto key_of = [&](int i) { return KEPT ? kept[i] : keys[i]; };
+
+  const int all = select_largest<kSelectThreads>(used, p.count, key_of, [&](int to, int i) { out[to] = i; }, [](int, int) {});
   for (int i = all + tid; i < p.count; i += kSelectThreads) out[i] = -1;
 }
 
