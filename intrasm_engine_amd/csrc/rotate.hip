@@ -3,8 +3,11 @@
 // What bounds it: memory, every feature is read and written once, 2 r more words of the table a token.  So a thread keeps its planes' cosines and
 // sines in registers for several heads, and loads and stores are 16 bytes or more:
 //   rows      features next to each other: a thread has eight planes of a token, 16 features
-//   columns   tokens next to each other (features x tokens, as a projection W @ X leaves them): a thread has a plane of eight tokens
+//   columns   tokens next to each other (features x tokens, as a projection W @ X leaves them): a thread has a plane of eight tokens, or, where they
+//             are not 16-byte aligned, planes of a token
 //   single    everything else: a thread has a plane of a token
+// Measured: 30001 tokens of 32 heads of 128 in bf16, 64 features by three axes in turn, rows 114 us = 4.4 TB/s read and written (with streaming loads 123, with
+// streaming stores 133); 8192 tokens in fp16, columns 31 us = 4.4; 300 tokens of 16 heads of 64 4.1.
 #include "rotation_host.h"
 
 namespace iex {
@@ -12,13 +15,13 @@ namespace {
 
 struct RotateParams {
   Rotation rotation;
-  int tokens, heads, dim, back, per_thread;   // heads that a thread takes one after the other
+  int tokens, heads, dim, back, per_thread, planes;   // heads that a thread takes one after the other; planes of a workgroup (tokens)
   const void* x;
   void* out;
   long long x_strides[3], out_strides[3];   // token, head, feature
 };
 
-// Eight elements next to each other, in 32 bits.  ALIGNED: to 16 bytes, else to an element.
+// Eight elements next to each other, 16-byte aligned, and in 32 bits.
 template <int DTYPE> struct rotate_element { typedef unsigned short type; };
 template <> struct rotate_element<IEX_F32> { typedef float type; };
 template <int DTYPE>
@@ -31,22 +34,18 @@ __device__ __forceinline__ typename rotate_element<DTYPE>::type narrow(float x) 
   if constexpr (DTYPE == IEX_F32) return x;
   else return (unsigned short)pack_pair<DTYPE == IEX_BF16>(x, 0.f);
 }
-template <int BYTES> struct any_piece;
-template <> struct any_piece<2> { typedef u32x4 type __attribute__((aligned(2))); };
-template <> struct any_piece<4> { typedef u32x4 type __attribute__((aligned(4))); };
-template <int DTYPE, bool ALIGNED>
+template <int DTYPE>
 struct Eight {
   typedef typename rotate_element<DTYPE>::type T;
   static constexpr int N = DTYPE == IEX_F32 ? 2 : 1;
-  typedef std::conditional_t<ALIGNED, u32x4, typename any_piece<sizeof(T)>::type> Piece;
   u32x4 raw[N];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) raw[i] = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(p) + i);
+    for (int i = 0; i < N; ++i) raw[i] = *(reinterpret_cast<const u32x4*>(p) + i);
   }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i) *(reinterpret_cast<Piece*>(p) + i) = raw[i];
+    for (int i = 0; i < N; ++i) *(reinterpret_cast<u32x4*>(p) + i) = raw[i];
   }
   __device__ __forceinline__ void get(float (&x)[8]) const {
 #pragma unroll
@@ -64,12 +63,14 @@ struct Eight {
   }
 };
 
-constexpr int kAhead = 4;   // heads whose loads are in flight at once
+// Heads whose loads are in flight at once: of rows (eight: 300 tokens of 16 heads of 64 5.0 us, 4.1 by four), of columns (four: 8192 tokens of 32 heads of
+// 128 37.7, 34.0 by eight).
+constexpr int kRowsAhead = 4, kColumnsAhead = 8;
 
 template <int DTYPE, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotate_rows_kernel(RotateParams p) {
   typedef typename rotate_element<DTYPE>::type T;
-  typedef Eight<DTYPE, true> Chunk;
+  typedef Eight<DTYPE> Chunk;
   const int units = p.dim / 16, turned_units = p.rotation.features / 16;
   const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
   const int token = (int)(item / units), u = (int)(item % units);
@@ -87,16 +88,16 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(RotateParams p) {
   const T* x = static_cast<const T*>(p.x) + token * p.x_strides[0];
   T* out = static_cast<T*>(p.out) + token * p.out_strides[0];
   const int first = blockIdx.y * p.per_thread, end = min(p.heads, first + p.per_thread);
-  for (int head = first; head < end; head += kAhead) {
-    Chunk a[kAhead], b[kAhead];
+  for (int head = first; head < end; head += kRowsAhead) {
+    Chunk a[kRowsAhead], b[kRowsAhead];
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
+    for (int h = 0; h < kRowsAhead; ++h) {
       if (head + h >= end) break;
       a[h].load(x + (head + h) * p.x_strides[1] + c0 * 8);
       b[h].load(x + (head + h) * p.x_strides[1] + c1 * 8);
     }
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
+    for (int h = 0; h < kRowsAhead; ++h) {
       if (head + h >= end) break;
       if (turned) {
         float f[16];
@@ -120,10 +121,10 @@ __device__ __forceinline__ void pair_of(const RotateParams& p, int plane, bool i
 }
 
 // Workgroups of 64 tokens x 32 planes: lanes have eight tokens each, eight of them and then the planes next to each other.
-template <int DTYPE, bool ALIGNED>
+template <int DTYPE>
 __global__ __launch_bounds__(256) void rotate_columns_kernel(RotateParams p, int interleaved) {
   typedef typename rotate_element<DTYPE>::type T;
-  typedef Eight<DTYPE, ALIGNED> Chunk;
+  typedef Eight<DTYPE> Chunk;
   const int token = blockIdx.x * 64 + threadIdx.x % 8 * 8, plane = blockIdx.y * 32 + threadIdx.x / 8;
   if (token >= p.tokens || plane >= p.dim / 2) return;
   const bool turned = plane < p.rotation.features / 2;
@@ -158,16 +159,16 @@ __global__ __launch_bounds__(256) void rotate_columns_kernel(RotateParams p, int
       }
     return;
   }
-  for (int head = first; head < end; head += kAhead) {
-    Chunk a[kAhead], b[kAhead];
+  for (int head = first; head < end; head += kColumnsAhead) {
+    Chunk a[kColumnsAhead], b[kColumnsAhead];
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
+    for (int h = 0; h < kColumnsAhead; ++h) {
       if (head + h >= end) break;
       a[h].load(x + (head + h) * p.x_strides[1] + f0 * p.x_strides[2]);
       b[h].load(x + (head + h) * p.x_strides[1] + f1 * p.x_strides[2]);
     }
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
+    for (int h = 0; h < kColumnsAhead; ++h) {
       if (head + h >= end) break;
       if (turned) {
         float y0[8], y1[8];
@@ -178,6 +179,47 @@ __global__ __launch_bounds__(256) void rotate_columns_kernel(RotateParams p, int
       }
       a[h].store(out + (head + h) * p.out_strides[1] + f0 * p.out_strides[2]);
       b[h].store(out + (head + h) * p.out_strides[1] + f1 * p.out_strides[2]);
+    }
+  }
+}
+
+// Workgroups of 64 tokens, a lane each, x up to 32 planes, in turn: the table's rows come once from memory for all of them.  (16 bytes a lane at any alignment:
+// 8191 tokens of 32 heads of 128 in fp16 66 us, 44 so.)
+template <int DTYPE>
+__global__ __launch_bounds__(256) void rotate_tokens_kernel(RotateParams p, int interleaved) {
+  typedef typename rotate_element<DTYPE>::type T;
+  const int token = blockIdx.x * 64 + lane_id(), wave = uniform(threadIdx.x >> 6);
+  if (token >= p.tokens) return;
+  const RotationPlace place(p.rotation, token);
+  const int first = blockIdx.z * p.per_thread, end = min(p.heads, first + p.per_thread), planes = min(p.dim / 2, (int)(blockIdx.y + 1) * p.planes);
+  const T* x = static_cast<const T*>(p.x) + token;
+  T* out = static_cast<T*>(p.out) + token;
+  for (int plane = blockIdx.y * p.planes + wave; plane < planes; plane += 4) {
+    const bool turned = plane < p.rotation.features / 2;   // (uniform)
+    int f0, f1;
+    pair_of(p, plane, interleaved, f0, f1);
+    float c = 1.f, s = 0.f;
+    if (turned) load_plane(p.rotation, place, axis_of(p.rotation, plane), plane, c, s);
+    if (p.back) s = -s;
+    for (int head = first; head < end; head += kColumnsAhead) {
+      T a[kColumnsAhead], b[kColumnsAhead];
+#pragma unroll
+      for (int h = 0; h < kColumnsAhead; ++h) {
+        if (head + h >= end) break;
+        a[h] = x[(head + h) * p.x_strides[1] + f0 * p.x_strides[2]];
+        b[h] = x[(head + h) * p.x_strides[1] + f1 * p.x_strides[2]];
+      }
+#pragma unroll
+      for (int h = 0; h < kColumnsAhead; ++h) {
+        if (head + h >= end) break;
+        float y0 = widen<DTYPE>(a[h]), y1 = widen<DTYPE>(b[h]);
+        if (turned) {
+          rotate(y0, y1, c, s);
+          a[h] = narrow<DTYPE>(y0), b[h] = narrow<DTYPE>(y1);
+        }
+        out[(head + h) * p.out_strides[1] + f0 * p.out_strides[2]] = a[h];
+        out[(head + h) * p.out_strides[1] + f1 * p.out_strides[2]] = b[h];
+      }
     }
   }
 }
@@ -210,9 +252,9 @@ __global__ __launch_bounds__(256) void rotate_single_kernel(RotateParams p, int 
 const char* dtype_name(int dtype) { return dtype == IEX_F32 ? "f32" : dtype == IEX_BF16 ? "bf16" : "f16"; }
 
 // Heads of a thread: all of them, fewer as long as the launch has too few workgroups.
-int heads_of_a_thread(const RotateParams& p, long long workgroups) {
+int heads_of_a_thread(const RotateParams& p, long long workgroups, int ahead) {
   int per = p.heads;
-  while (per > kAhead && workgroups * ceil_div(p.heads, per) < 2048) per = (per / 2 + kAhead - 1) / kAhead * kAhead;
+  while (per > ahead && workgroups * ceil_div(p.heads, per) < 2048) per = (per / 2 + ahead - 1) / ahead * ahead;
   return per;
 }
 
@@ -225,19 +267,22 @@ int launch(RotateParams p, bool interleaved, hipStream_t s) {
   auto columns_aligned = [&](const void* x, const long long* strides) { return aligned(x, 16) && strides[1] % chunk == 0 && strides[2] % chunk == 0; };
   if (p.dim % 16 == 0 && p.rotation.features % 16 == 0 && rows(p.x, p.x_strides) && rows(p.out, p.out_strides)) {
     const long long grid = ceil_div((long long)p.tokens * (p.dim / 16), 256);
-    p.per_thread = heads_of_a_thread(p, grid);
+    p.per_thread = heads_of_a_thread(p, grid, kRowsAhead);
     const dim3 dims((unsigned)grid, ceil_div(p.heads, p.per_thread));
     note_kernel("rotate_rows_kernel<%s>", dtype_name(DTYPE));
     if (interleaved) hipLaunchKernelGGL((rotate_rows_kernel<DTYPE, true>), dims, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((rotate_rows_kernel<DTYPE, false>), dims, dim3(256), 0, s, p);
   } else if (p.dim % 2 == 0 && p.x_strides[0] == 1 && p.out_strides[0] == 1 && p.tokens >= 8) {
-    const long long grid = (long long)ceil_div(p.tokens, 64) * ceil_div(p.dim, 64);
-    p.per_thread = heads_of_a_thread(p, grid);
-    const dim3 dims(ceil_div(p.tokens, 64), ceil_div(p.dim, 64), ceil_div(p.heads, p.per_thread));
     const bool whole = columns_aligned(p.x, p.x_strides) && columns_aligned(p.out, p.out_strides);
-    note_kernel("rotate_columns_kernel<%s, %s>", dtype_name(DTYPE), whole ? "aligned" : "any");
-    if (whole) hipLaunchKernelGGL((rotate_columns_kernel<DTYPE, true>), dims, dim3(256), 0, s, p, interleaved);
-    else hipLaunchKernelGGL((rotate_columns_kernel<DTYPE, false>), dims, dim3(256), 0, s, p, interleaved);
+    auto grid = [&] { return (long long)ceil_div(p.tokens, 64) * ceil_div(p.dim, 2 * p.planes); };
+    p.planes = 32;
+    // (a wavefront's planes come one after the other: fewer of them where there are too few workgroups; 2001 tokens of 8 heads 17.3 us by 32)
+    while (!whole && p.planes > 4 && grid() * ceil_div(p.heads, kColumnsAhead) < 1024) p.planes /= 2;
+    p.per_thread = heads_of_a_thread(p, grid(), kColumnsAhead);
+    const dim3 dims(ceil_div(p.tokens, 64), ceil_div(p.dim, 2 * p.planes), ceil_div(p.heads, p.per_thread));
+    note_kernel("%s<%s>", whole ? "rotate_columns_kernel" : "rotate_tokens_kernel", dtype_name(DTYPE));
+    if (whole) hipLaunchKernelGGL((rotate_columns_kernel<DTYPE>), dims, dim3(256), 0, s, p, interleaved);
+    else hipLaunchKernelGGL((rotate_tokens_kernel<DTYPE>), dims, dim3(256), 0, s, p, interleaved);
   } else {
     const long long grid = ceil_div((long long)p.tokens * ((p.dim + 1) / 2), 256);
     note_kernel("rotate_single_kernel<%s>", dtype_name(DTYPE));

@@ -91,8 +91,8 @@ def test_rotate(ops, dev, dtype, layout, tokens, heads, dim, r, sections, in_tur
         assert torch.equal(got[..., r:], x[..., r:])
 
 
-@pytest.mark.parametrize("dtype,layout,tokens,heads,dim,kernel", [(F16, "tokens", 300, 4, 128, "rotate_rows_kernel<f16>"), (F32, "features", 64, 4, 128, "rotate_columns_kernel<f32, aligned>"),
-                                                                  (BF16, "features", 65, 4, 64, "rotate_columns_kernel<bf16, any>"), (BF16, "tokens", 65, 4, 66, "rotate_single_kernel<bf16>"),
+@pytest.mark.parametrize("dtype,layout,tokens,heads,dim,kernel", [(F16, "tokens", 300, 4, 128, "rotate_rows_kernel<f16>"), (F32, "features", 64, 4, 128, "rotate_columns_kernel<f32>"),
+                                                                  (BF16, "features", 65, 4, 64, "rotate_tokens_kernel<bf16>"), (BF16, "tokens", 65, 4, 66, "rotate_single_kernel<bf16>"),
                                                                   (F16, "features", 7, 4, 64, "rotate_single_kernel<f16>")])
 def test_kernels(ops, dev, dtype, layout, tokens, heads, dim, kernel):
     x, table, positions = inputs(dev, tokens, heads, dim, dim, 1, dtype)
@@ -138,7 +138,7 @@ def test_gradient(ops, dev, layout, interleaved):
     f = [(turned(x + e * d, table, positions, sections, True, interleaved)[0] * g.detach()).sum() for e in (1.0, -1.0)]
     # x + d is rounded (2^-24 of it), as is every element of the gradient (2^-24 and 2 * 2^-24 of the pair)
     allowed = 2.0 ** -23 * float(((x.abs() + d.abs()).sum() + (grad.detach().abs() * d.abs()).sum()) * 8)
-    assert abs(float((f[0] - f[1]) / 2 - (grad.double() * d).sum())) <= allowed
+    assert abs(float((f[0] - f[1]) / 2 - (grad.detach().double() * d).sum())) <= allowed
     again, = torch.autograd.grad(grad, g, d)
     want, slack = turned(d, table, positions, sections, True, interleaved)
     close(again, want, slack)
