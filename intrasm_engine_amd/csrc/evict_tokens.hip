@@ -11,7 +11,7 @@
 // running and that waits for nobody before it has read, so every wait ends.
 //
 // What bounds it: memory, kept rows read and written once: 64 sequences of 1500 .. 4224 tokens to 2048, 8 key heads of 128 in 16 bits 149 us = 5.1 TB/s,
-// selection 16; 131071 tokens to 32768, every fourth row of 256 bytes, 66 us = 4.1 TB/s, selection 34 in five launches (by one workgroup a row, whose CU reads
+// selection 16; 131071 tokens to 32768, every fourth row of 256 bytes, 66 us = 4.1 TB/s, selection 32 in five launches (by one workgroup a row, whose CU reads
 // the weights again in every round, 143); 700 tokens to 512, 32 key heads 6.7 and 7.1.
 #include "paged_cache_host.h"
 #include "select_device.cuh"
@@ -46,68 +46,53 @@ __device__ __forceinline__ u32x4 four_of(const unsigned* row, int i, int used) {
   return u32x4{i < used ? row[i] : 0u, i + 1 < used ? row[i + 1] : 0u, i + 2 < used ? row[i + 2] : 0u, 0u};
 }
 
-// The keys of places first .. used - 1 that are above a threshold, and those that equal it as long as fewer than `need` of the row's do before them, in
-// ascending order: emit(to, i, payload), to = how many are taken before i.  aboves, equals: how many of the row's keys before `first` are above it, and equal it.
-// place(i, before): at every fourth place how many are taken below it.  Returns how many are up to the end.
-template <int THREADS, typename KEYS, typename PAYLOADS, typename EMIT, typename PLACE>
-__device__ __forceinline__ int take_largest(int first, int used, int count, unsigned threshold, int need, int aboves, int equals, KEYS keys, PAYLOADS payloads, EMIT emit,
-                                            PLACE place) {
-  constexpr int WAVES = THREADS / kWave, AHEAD = 4, STEP = 4 * kWave;
+// The keys of a slice, places first .. used - 1 of a row, that are above a threshold, and those that equal it as long as fewer than `need` of the row's do
+// before them, in ascending order: emit(to, i, payload), to = how many are taken before i.  aboves, equals: how many of the row's keys before `first` are above
+// it, and equal it.  place(i, before): at every fourth place how many are taken below it.  A wavefront has a stretch of 64 x 4 x STEPS places.
+template <int THREADS, int STEPS, typename KEYS, typename PAYLOADS, typename EMIT, typename PLACE>
+__device__ __forceinline__ void take_largest(int first, int used, int count, unsigned threshold, int need, int aboves, int equals, KEYS keys, PAYLOADS payloads, EMIT emit,
+                                             PLACE place) {
+  constexpr int WAVES = THREADS / kWave, STEP = 4 * kWave;
   __shared__ int totals[2][WAVES];
-  const int lane = lane_id(), wave = uniform(threadIdx.x >> 6);
-  const int stretch = (used - first + THREADS * 4 - 1) / (THREADS * 4) * STEP, begin = min(used, first + wave * stretch), end = min(used, begin + stretch);
-  auto marks = [&](const u32x4& k) {   // (those that equal it, 256 of a step at most) << 16 | those above
+  const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), begin = first + wave * (STEPS * STEP);
+  u32x4 k[STEPS], what[STEPS];
+#pragma unroll
+  for (int a = 0; a < STEPS; ++a) k[a] = keys(begin + a * STEP + lane * 4);   // (0 behind the row)
+#pragma unroll
+  for (int a = 0; a < STEPS; ++a) what[a] = payloads(begin + a * STEP + lane * 4);
+  auto marks = [&](const u32x4& key) {   // (those that equal it, 256 of a step at most) << 16 | those above
     int n = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) n += (k[j] > threshold ? 1 : 0) + (k[j] == threshold && k[j] != 0 ? 1 << 16 : 0);
+    for (int j = 0; j < 4; ++j) n += (key[j] > threshold ? 1 : 0) + (key[j] == threshold && key[j] != 0 ? 1 << 16 : 0);
     return n;
   };
-  int above = 0, equal = 0;   // of this lane
-  for (int i0 = begin + lane * 4; i0 < end; i0 += AHEAD * STEP) {
-    u32x4 k[AHEAD];
+  int mine[STEPS], upto[STEPS], above = 0, equal = 0;   // a step's own marks, with the lanes before; the wavefront's
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) k[a] = i0 + a * STEP < end ? keys(i0 + a * STEP) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int n = marks(k[a]);
-      above += n & 0xFFFF, equal += n >> 16;
-    }
+  for (int a = 0; a < STEPS; ++a) {
+    mine[a] = marks(k[a]), upto[a] = wave_scan(mine[a]);
+    const int step = bcast_i(upto[a], kWave - 1);
+    above += step & 0xFFFF, equal += step >> 16;
   }
-  above = wave_scan(above), equal = wave_scan(equal);
-  if (lane == kWave - 1) totals[0][wave] = above, totals[1][wave] = equal;
+  if (lane == 0) totals[0][wave] = above, totals[1][wave] = equal;
   __syncthreads();
-  int all_above = aboves, all_equal = equals;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < wave) aboves += totals[0][w], equals += totals[1][w];   // before this wavefront's stretch
-    all_above += totals[0][w], all_equal += totals[1][w];
-  }
-  for (int i0 = begin; i0 < end; i0 += AHEAD * STEP) {
-    u32x4 k[AHEAD], what[AHEAD];
+  for (int w = 0; w < WAVES; ++w)
+    if (w < wave) aboves += totals[0][w], equals += totals[1][w];
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int i = i0 + a * STEP + lane * 4;
-      k[a] = what[a] = u32x4{0u, 0u, 0u, 0u};
-      if (i < end) k[a] = keys(i), what[a] = payloads(i);
+  for (int a = 0; a < STEPS; ++a) {
+    const int i = begin + a * STEP + lane * 4;
+    int above_before = aboves + ((upto[a] - mine[a]) & 0xFFFF), equal_before = equals + ((upto[a] - mine[a]) >> 16);
+    if (i < used) place(i, above_before + min(equal_before, need));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool more = k[a][j] > threshold, same = k[a][j] == threshold && k[a][j] != 0;
+      const int to = above_before + min(equal_before, need);
+      if ((more || (same && equal_before < need)) && to < count) emit(to, i + j, what[a][j]);
+      above_before += more, equal_before += same;
     }
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      if (i0 + a * STEP >= end) break;
-      const int i = i0 + a * STEP + lane * 4, mine = marks(k[a]), upto = wave_scan(mine);
-      int above_before = aboves + ((upto - mine) & 0xFFFF), equal_before = equals + ((upto - mine) >> 16);
-      if (i < end) place(i, above_before + min(equal_before, need));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool more = k[a][j] > threshold, same = k[a][j] == threshold && k[a][j] != 0;
-        const int to = above_before + min(equal_before, need);
-        if ((more || (same && equal_before < need)) && to < count) emit(to, i + j, what[a][j]);
-        above_before += more, equal_before += same;
-      }
-      const int step = bcast_i(upto, kWave - 1);
-      aboves += step & 0xFFFF, equals += step >> 16;
-    }
+    const int step = bcast_i(upto[a], kWave - 1);
+    aboves += step & 0xFFFF, equals += step >> 16;
   }
-  return min(count, all_above + min(all_equal, need));
 }
 
 // Whether a row is to be cut.  One that is not gets its list here (all of a sequence that is short enough, or nothing: a sequence with pages given back has no
@@ -247,7 +232,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_slice_kernel(EvictParams 
     unsigned* to = p.histograms + (STAGE % 2 * all + (size_t)row * p.slices + slice) * 256;
     if (tid < 256) to[tid] = histogram[tid];
   } else {
-    take_largest<kEvictThreads>(
+    take_largest<kEvictThreads, kEvictSlice / (kEvictThreads * 4)>(
         first, used, p.keep, (unsigned)found.x, found.y, found.z, found.w, [&](int i) { return its.keys_at(i); }, [&](int i) { return its.weights_at(i); },
         [&](int to, int i, unsigned weight) { its.take(to, i, weight); }, [&](int i, int taken) { its.place(i, taken); });
   }
@@ -390,6 +375,9 @@ void launch_bounds(const EvictParams& p, int head_dim, unsigned grid, hipStream_
   else hipLaunchKernelGGL((evict_bounds_kernel<BF16, 256, E8>), dim3(grid), dim3(256), 0, s, p);
 }
 
+// A table that holds no more than is kept: nothing ever moves.
+bool never(const iex_paged_cache& c, int keep) { return (long long)c.table_width * c.page_size <= keep; }
+
 struct Layout {
   long long rows, chunks;
   int slices;                                                              // of a row, 0: rows are in LDS
@@ -397,6 +385,7 @@ struct Layout {
 };
 Layout layout_of(const iex_paged_cache& c, int keep) {
   Layout l;
+  if (never(c, keep)) keep = 0;
   l.rows = (long long)c.seqs * c.kv_heads, l.chunks = ceil_div(keep, chunk_of(c));
   l.tickets = (size_t)l.rows * 4;
   l.flags = l.tickets + (size_t)l.rows * 4;
@@ -412,8 +401,6 @@ Layout layout_of(const iex_paged_cache& c, int keep) {
 // Workgroups of 512 threads where there are many more rows than CUs, which then have several at a time, or rows are short (both launches, 512 rows of 1024
 // tokens 15.9 us, 2048 of 8192 88; by 1024 threads 17.5 and 99); else of 1024 (8 rows of 4096 16.9, 512 of 8192 32.5; by 512 18.4 and 34.5).
 bool few_threads(long long rows, long long room) { return room <= 1024 || (room <= 12288 && rows * 10 > room); }
-// A table that holds no more than is kept: nothing ever moves.
-bool never(const iex_paged_cache& c, int keep) { return (long long)c.table_width * c.page_size <= keep; }
 
 }  // namespace
 }  // namespace iex
@@ -437,8 +424,9 @@ extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, floa
   IEX_REQUIRE(aligned(kept, 4), IEX_ERR_UNSUPPORTED, "evict_tokens: operands must be aligned to their elements");
   IEX_REQUIRE((long long)cache->pages * cache->page_size < (1ll << 31), IEX_ERR_TOO_LARGE, "evict_tokens: up to 2^31 tokens in a cache");
   const Layout l = layout_of(*cache, keep);
-  const long long pages = ceil_div(keep, cache->page_size);
-  IEX_REQUIRE(l.rows < (1ll << 22) && l.rows * l.slices < (1ll << 22) && l.rows * l.chunks < (1ll << 24) && (!cache->bounds || l.rows * pages < (1ll << 24)), IEX_ERR_TOO_LARGE,
+  const bool moves = !never(*cache, keep) && cache->pages > 0;
+  const long long pages = moves && cache->bounds ? ceil_div(keep, cache->page_size) : 0;   // whose bounds change
+  IEX_REQUIRE(l.rows < (1ll << 22) && l.rows * l.slices < (1ll << 22) && l.rows * l.chunks < (1ll << 24) && l.rows * pages < (1ll << 24), IEX_ERR_TOO_LARGE,
               "evict_tokens: too many sequences, heads or tokens to keep");
   IEX_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= l.bytes, IEX_ERR_BAD_ARGUMENT, "evict_tokens: needs a 256-byte aligned workspace of %zu bytes", l.bytes);
   EvictParams p{};
@@ -478,12 +466,12 @@ extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, floa
     else hipLaunchKernelGGL((evict_select_kernel<kEvictThreads>), dim3((unsigned)l.rows), dim3(kEvictThreads), lds, s, p, chunk_shift);
   }
   if (int rc = check_hip(hipGetLastError(), "evict_tokens launch")) return rc;
-  if (never(*cache, keep) || cache->pages == 0) return 0;
+  if (!moves) return 0;
   const unsigned grid = (unsigned)(l.rows * l.chunks);
   if (cache->eight_bits) launch_move<true>(p, cache->head_dim, grid, s);
   else launch_move<false>(p, cache->head_dim, grid, s);
   if (int rc = check_hip(hipGetLastError(), "evict_tokens launch")) return rc;
-  if (!cache->bounds) return 0;
+  if (!pages) return 0;
   const unsigned page_grid = (unsigned)(l.rows * pages);
   if (cache->dtype == IEX_BF16) cache->eight_bits ? launch_bounds<true, true>(p, cache->head_dim, page_grid, s) : launch_bounds<true, false>(p, cache->head_dim, page_grid, s);
   else cache->eight_bits ? launch_bounds<false, true>(p, cache->head_dim, page_grid, s) : launch_bounds<false, false>(p, cache->head_dim, page_grid, s);

@@ -81,7 +81,7 @@ def check(ops, c, weights, keep, recent, first=0, bounds=None, passed_over=()):
         plain_bounds.__dict__.update(c.__dict__)
         plain_bounds.bounds = old_bounds
         for s in range(c.lengths.numel()):
-            if int(lengths[s]) > keep and s not in passed_over:
+            if min(int(lengths[s]), c.width * c.page) > keep and s not in passed_over:
                 for i in range(-(-keep // c.page)):
                     plain_bounds.set_bounds(int(c.table[s, i]), min(c.page, keep - i * c.page))
         assert torch.equal(bounds, plain_bounds.bounds)
@@ -190,6 +190,56 @@ def test_replays_follow_what_is_there(ops, dev):
         want = [evict(ops, c, weights, 200, 20, 2), c.keys, c.values, c.lengths, weights]
         for x, y in zip(got, want):
             assert torch.equal(x, y)
+
+
+def test_two_streams_and_threads(ops, dev):
+    """Passes that keep account over one cache, each with an account of its own, and evictions of different sequences of it, at once on two streams."""
+    import threading
+
+    c = Cache(dev, [3000, 900, 2500, 1400], 2, 64, 16, F16, poison=False)
+    halves = [slice(0, 2), slice(2, 4)]
+    q = torch.randn(2, 2, 4, 64, generator=torch.Generator(device=dev).manual_seed(1), device=dev).half()
+
+    def pass_over(i, cache, lengths, weights):
+        out = [ops.paged_attention_accumulate_(q[i], cache.keys, cache.values, cache.table[halves[i]], lengths, weights, 0.2) for _ in range(5)]
+        kept = ops.evict_tokens_(cache.keys, cache.values, cache.table[halves[i]], lengths, weights, 700, 100, 4)
+        return [out[-1], kept, ops.paged_attention(q[i], cache.keys, cache.values, cache.table[halves[i]], lengths, 0.2)]
+
+    def copy():
+        new = Cache.__new__(Cache)
+        new.__dict__.update(c.__dict__)
+        new.keys, new.values = c.keys.clone(), c.values.clone()
+        return new, [c.lengths[h].clone() for h in halves], [torch.zeros(2, 2, c.width * 16, device=dev) for _ in halves]
+
+    alone, lengths, weights = copy()
+    want = [pass_over(i, alone, lengths[i], weights[i]) for i in range(2)]
+    both, lengths2, weights2 = copy()
+    torch.cuda.synchronize()
+    got, streams = [None, None], [torch.cuda.Stream() for _ in range(2)]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            got[i] = pass_over(i, both, lengths2[i], weights2[i])
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])) and torch.equal(weights[i], weights2[i]) and torch.equal(lengths[i], lengths2[i])
+    assert torch.equal(both.keys, alone.keys) and torch.equal(both.values, alone.values)
+
+
+def test_a_budget_beyond_the_table(ops, dev):
+    """Nothing ever leaves: the list is the tokens, whatever the budget; a length beyond the table stays as it is."""
+    c = Cache(dev, [48, 20, 0], 2, 64, 16, F16, width=3, poison=False, bounds=True)
+    c.lengths[0] = 1 << 20
+    weights = random_weights(c)
+    for keep in (48, 49, 100000):
+        check(ops, c, weights, keep, 10, 2, c.bounds)
+    assert c.lengths.tolist() == [1 << 20, 20, 0]
 
 
 def test_offsets_beyond_32_bits(ops, dev):

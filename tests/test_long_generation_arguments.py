@@ -58,7 +58,7 @@ def test_caches_that_are_refused(call, other, code, text):
     (evict, dict(keep=0), -1, "at least one token"), (evict, dict(keep=-1), -1, "at least one token"), (evict, dict(recent=99), -1, "among them"), (evict, dict(first=-1), -1, "among them"),
     (evict, dict(recent=(1 << 31) - 1, first=1, keep=(1 << 31) - 1), -1, "among them"), (evict, dict(lengths=None), -1, "null"), (evict, dict(lengths=A + 4), -1, "null"),
     (evict, dict(weights=None), -1, "null"), (evict, dict(kept=None), -1, "null"), (evict, dict(weights=ODD), -2, "aligned"), (evict, dict(ws=None), -1, "workspace"),
-    (evict, dict(ws_bytes=64), -1, "workspace"), (evict, dict(keep=1 << 30, recent=0, first=0), -3, "too many"),
+    (evict, dict(ws_bytes=64), -1, "workspace"),
 ])
 def test_arguments_that_are_refused(call, arguments, code, text):
     assert call(cache(), **arguments) == code and text in _lib.last_error()
@@ -72,6 +72,15 @@ def test_arguments_that_are_refused(call, arguments, code, text):
     (dict(features=144, sections=[24, 24, 24]), -2, "128"), (dict(at=A + 1), -2, "aligned"), (dict(features=512, sections=[100, 100, 56]), -2, "up to 256")])
 def test_rotations_that_are_refused(call, other, code, text):
     assert call(rotation(**other)) == code and text in _lib.last_error()
+
+
+def test_evictions_that_are_too_large():
+    many = cache(seqs=100, table_width=1 << 22)
+    assert evict(many, keep=1 << 27, recent=0, first=0) == -3 and "too many" in _lib.last_error()
+    assert evict(cache(pages=(1 << 25) + 1), keep=10, recent=0, first=0) == -3 and "2^31 tokens" in _lib.last_error()
+    assert evict(cache(seqs=1 << 21), keep=10, recent=0, first=0) == -3 and "too many" in _lib.last_error()
+    # a table that holds no more than is kept: what is kept takes no room
+    assert _lib.load().iex_evict_tokens_workspace_bytes(ctypes.byref(cache()), 1 << 30) == _lib.load().iex_evict_tokens_workspace_bytes(ctypes.byref(cache()), 256) < 256
 
 
 def test_more_refusals_of_rotations():
