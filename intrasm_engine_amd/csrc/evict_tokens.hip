@@ -8,7 +8,8 @@
 // at place i or behind it, so what chunk c writes, places c * chunk and on, is only ever read by itself and by chunks before it (the list's stretch
 // with tokens there ends before its own); all of a chunk's rows are in registers before its first write, and it writes when the chunks before it that
 // read there, two at most, have said that theirs are too.  Chunks are drawn by ticket: the one that is waited for has been drawn before, by a workgroup that is
-// running and that waits for nobody before it has read, so every wait ends.
+// running and that waits for nobody before it has read, so every wait ends.  (It is bounded all the same, to about a second: calls that share a workspace at the
+// same time, which they must not, leave rows unmoved and do not hang.)
 //
 // What bounds it: memory, kept rows read and written once: 64 sequences of 1500 .. 4224 tokens to 2048, 8 key heads of 128 in 16 bits 149 us = 5.1 TB/s,
 // selection 16; 131071 tokens to 32768, every fourth row of 256 bytes, 66 us = 4.1 TB/s, selection 32 in five launches (by one workgroup a row, whose CU reads
@@ -39,6 +40,7 @@ struct EvictParams {
 
 constexpr int kEvictThreads = 1024, kEvictKept = 32768;   // ... whose weights fit in LDS
 constexpr int kEvictSlice = 8192;                         // tokens
+constexpr int kEvictTries = 1 << 20;                      // of a wait
 
 // Four words from place i on of a 16-byte aligned row of `used`, 0 behind it.
 __device__ __forceinline__ u32x4 four_of(const unsigned* row, int i, int used) {
@@ -255,6 +257,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   if (tid == 0) drawn = atomicAdd(p.tickets + row, 1);
   __syncthreads();
   const int chunk = drawn, first = chunk * T, count = min(T, p.keep - first);
+  if ((unsigned)chunk >= (unsigned)p.chunks) return;
   const int* const kept = p.kept + (size_t)row * p.keep;
   float* const weights = p.weights + (size_t)row * ((size_t)c.table_width << c.page_shift);
   // the weights, which nobody reads here: those of the chunk's tokens, and this chunk's share of the zeros behind the kept ones
@@ -303,10 +306,12 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   __syncthreads();
   int* const flags = p.flags + (size_t)row * p.chunks;
   if (tid == 0) __hip_atomic_store(flags + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  bool read = true;
   if (low < high && tid <= (high - 1) / T - low / T) {
-    while (__hip_atomic_load(flags + low / T + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(2);
+    for (int tries = 0; !(read = __hip_atomic_load(flags + low / T + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0) && tries < kEvictTries; ++tries)
+      __builtin_amdgcn_s_sleep(2);
   }
-  __syncthreads();
+  if (!__syncthreads_and(read)) return;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int at = line + i * (256 / LANES);

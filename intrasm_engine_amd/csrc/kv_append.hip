@@ -28,7 +28,7 @@ extern "C" int iex_kv_append_at(const iex_paged_cache* cache, int tokens, const 
   IEX_REQUIRE(heads == 0 || (q && q_out && q_strides && q_out_strides), IEX_ERR_BAD_ARGUMENT, "kv_append: null pointer argument");
   IEX_REQUIRE(cache->seqs == 0 || cache->lengths, IEX_ERR_BAD_ARGUMENT, "kv_append: null pointer argument");   // (without key heads too: queries turn by them)
   AppendParams p{};
-  if (int rc = check_rotation(rotation, tokens, "kv_append", p.rotation)) return rc;
+  if (int rc = check_rotation(rotation, "kv_append", p.rotation)) return rc;
   const int rotary = p.rotation.features;
   IEX_REQUIRE(rotary % 16 == 0 && rotary <= cache->head_dim, IEX_ERR_UNSUPPORTED,
               "kv_append: rotated features must be a multiple of 16 of the head's (%d of %d)", rotary, cache->head_dim);

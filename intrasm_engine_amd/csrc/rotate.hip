@@ -300,12 +300,13 @@ extern "C" int iex_rotate(int dtype, int tokens, int heads, int head_dim, const 
   trail_reset();
   IEX_REQUIRE(dtype == IEX_F32 || dtype == IEX_F16 || dtype == IEX_BF16, IEX_ERR_UNSUPPORTED, "rotate: fp32, fp16 or bf16");
   IEX_REQUIRE(tokens >= 0 && heads >= 0 && head_dim >= 0, IEX_ERR_BAD_ARGUMENT, "rotate: negative dimension");
-  IEX_REQUIRE(rotation && (rotation->at || tokens == 0), IEX_ERR_BAD_ARGUMENT, "rotate: null pointer argument");
+  if (tokens == 0) return 0;
+  IEX_REQUIRE(rotation && rotation->at, IEX_ERR_BAD_ARGUMENT, "rotate: null pointer argument");
   RotateParams p{};
-  if (int rc = check_rotation(rotation, tokens, "rotate", p.rotation)) return rc;
+  if (int rc = check_rotation(rotation, "rotate", p.rotation)) return rc;
   IEX_REQUIRE(p.rotation.features % 2 == 0 && p.rotation.features <= head_dim, IEX_ERR_UNSUPPORTED, "rotate: rotated features must be an even number of the head's (%d of %d)",
               p.rotation.features, head_dim);
-  if (tokens == 0 || heads == 0 || head_dim == 0) return 0;
+  if (heads == 0 || head_dim == 0) return 0;
   IEX_REQUIRE(x && out && x_strides && out_strides, IEX_ERR_BAD_ARGUMENT, "rotate: null pointer argument");
   IEX_REQUIRE(aligned(x, dtype == IEX_F32 ? 4 : 2) && aligned(out, dtype == IEX_F32 ? 4 : 2), IEX_ERR_UNSUPPORTED, "rotate: operands must be aligned to their elements");
   IEX_REQUIRE((long long)tokens * ((head_dim + 1) / 2) < (1ll << 31) && heads < 65536 && head_dim < 65536, IEX_ERR_TOO_LARGE, "rotate: too many tokens or heads");

@@ -6,8 +6,8 @@
 namespace iex {
 namespace {
 
-// `tokens` of the call; positions come with it (null `at`: the caller knows where tokens are, and that the table has those rows).
-int check_rotation(const iex_rotation* r, int tokens, const char* what, Rotation& out) {
+// Of a call that has tokens.  Null `at`: the caller knows where they are, and that the table has those rows.
+int check_rotation(const iex_rotation* r, const char* what, Rotation& out) {
   out = Rotation{};
   out.axes = 1;
   if (!r || r->features == 0) {
@@ -21,7 +21,7 @@ int check_rotation(const iex_rotation* r, int tokens, const char* what, Rotation
     IEX_REQUIRE(r->axes <= 1 && !r->sections, IEX_ERR_BAD_ARGUMENT, "%s: several axes without positions", what);
     return 0;
   }
-  IEX_REQUIRE(tokens == 0 || r->rows > 0, IEX_ERR_BAD_ARGUMENT, "%s: the rotation must have a row", what);
+  IEX_REQUIRE(r->rows > 0, IEX_ERR_BAD_ARGUMENT, "%s: the rotation must have a row", what);
   IEX_REQUIRE(r->axes >= 1 && r->axes <= 4, IEX_ERR_UNSUPPORTED, "%s: positions of one to four axes (%d)", what, r->axes);
   IEX_REQUIRE(aligned(r->at, 4), IEX_ERR_UNSUPPORTED, "%s: operands must be aligned to their elements", what);
   out.positions = r->at, out.axis_stride = r->axis_stride, out.axes = r->axes;

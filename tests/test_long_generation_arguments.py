@@ -104,7 +104,7 @@ def test_workspaces_and_calls_with_nothing_to_do():
     assert lib.iex_evict_tokens_workspace_bytes(ctypes.byref(c), 0) == 0 and lib.iex_evict_tokens_workspace_bytes(None, 5) == 0
     assert accumulate(cache(seqs=0)) == 0 and accumulate(c, heads=0) == 0 and evict(cache(seqs=0)) == 0 and evict(cache(kv_heads=0)) == 0
     assert append(c, None, tokens=0, heads=0) == -1 and rotate(rotation(), tokens=0) == 0 and rotate(rotation(), heads=0) == 0
-    assert rotate(rotation(rows=0, at=None, axes=1, sections=None), tokens=0) == 0
+    assert rotate(rotation(rows=0, at=None, axes=1, sections=None), tokens=0) == 0 and rotate(rotation(at=None, table=None), tokens=0, x=None, out=None) == 0
     for call in (accumulate, evict, append):
         assert call(None) == -1 and "null" in _lib.last_error()
 

@@ -231,6 +231,9 @@ def test_refusals(ops, dev):
     with pytest.raises(RuntimeError, match="up to 256"):
         ops.rotate(wide, torch.zeros(5, 320, device=dev), torch.zeros(2, 2, dtype=torch.int32, device=dev), [80, 80])
     assert ops.rotate(x[:0], table, positions[:, :0], good).shape == (0, 2, 64) and ops.rotate(x[:, :0], table, positions, good).shape == (8, 0, 64)
+    nothing = torch.zeros(0, 2, 64, dtype=F16, device=dev, requires_grad=True)      # (tensors without memory)
+    out = ops.rotate(nothing, table, torch.zeros(3, 0, dtype=torch.int32, device=dev), good)
+    assert torch.autograd.grad(out.sum(), nothing)[0].shape == (0, 2, 64)
     one = inputs(dev, 5, 1, 320, 320, 1, F16)      # (one axis: any number of features)
     want, slack = turned(*one)
     close(ops.rotate(*one), want, slack)
@@ -306,6 +309,10 @@ def test_append_refusals(ops, dev):
                        ((table[:0], False, None, None, None, positions, [16, 16]), "must have a row")]:
         with pytest.raises(RuntimeError, match=text):
             append(*more)
+    none = torch.zeros(0, 1, 64, dtype=F16, device=dev)
+    got = ops.kv_append_(none, none, c.keys, c.values, c.table, c.lengths, torch.zeros(2, dtype=torch.int32, device=dev), none, table, False, None, None, None,
+                         torch.zeros(2, 0, dtype=torch.int32, device=dev), [16, 16])
+    assert got.shape == (0, 1, 64)
     append(table[:2], False, None, None, None, positions.clamp(max=1), [16, 16])      # (a table shorter than the cache's)
     with pytest.raises(RuntimeError, match="every position"):
         append(table[:2], False)
