@@ -722,8 +722,10 @@ struct TrainableRotate : torch::autograd::Function<TrainableRotate> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& rotation, const Tensor& positions, at::OptionalIntArrayRef sections, bool in_turn, bool interleaved,
                         bool back) {
     ctx->save_for_backward({rotation, positions});
-    ctx->saved_data["sections"] = sections ? c10::IValue(sections->vec()) : c10::IValue();
-    ctx->saved_data["in_turn"] = in_turn, ctx->saved_data["interleaved"] = interleaved, ctx->saved_data["back"] = back;
+    // (flags, then the sections)
+    std::vector<int64_t> how{in_turn, interleaved, back, sections.has_value()};
+    if (sections) how.insert(how.end(), sections->begin(), sections->end());
+    ctx->saved_data["how"] = std::move(how);
     return rotated(x, rotation, positions, sections, in_turn, interleaved, back);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads);
@@ -738,10 +740,9 @@ variable_list TrainableRotate::backward(AutogradContext* ctx, variable_list grad
   const auto saved = ctx->get_saved_variables();
   variable_list out(7);
   if (!ctx->needs_input_grad(0) || !grads[0].defined()) return out;
-  const c10::IValue& sections = ctx->saved_data["sections"];
-  const std::vector<int64_t> by = sections.isNone() ? std::vector<int64_t>() : sections.toIntVector();
-  out[0] = trainable_rotate(grads[0], saved[0], saved[1], sections.isNone() ? at::OptionalIntArrayRef() : at::OptionalIntArrayRef(by), ctx->saved_data["in_turn"].toBool(),
-                            ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["back"].toBool());
+  const std::vector<int64_t> how = ctx->saved_data["how"].toIntVector();
+  const at::IntArrayRef sections = at::IntArrayRef(how).slice(4);
+  out[0] = trainable_rotate(grads[0], saved[0], saved[1], how[3] ? at::OptionalIntArrayRef(sections) : at::OptionalIntArrayRef(), how[0], how[1], !how[2]);
   return out;
 }
 
