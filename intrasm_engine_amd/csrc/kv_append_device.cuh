@@ -517,10 +517,17 @@ __global__ __launch_bounds__(256, 4) void kv_append_columns_kernel(AppendParams 
           for (int j = 0; j < 4; ++j) packed[j] = x[2 * j * D] | (unsigned)x[(2 * j + 1) * D] << 16;
           *reinterpret_cast<AnyChunk*>(out + (f + k * 32) * p.out_feature + token0 + c * 8) = packed;
         }
-      } else if (p.columns) {
+      } else if (p.columns && high - low > 32) {
         for (int i = threadIdx.x; i < T * D; i += 256) {
           const int t = i % T, f = i / T;
           if (t >= low && t < high) out[f * p.out_feature + token0 + t] = *element(t, f);
+        }
+      } else if (p.columns) {
+        // few rows: the lanes go over as many tokens, to a power of two (256 sequences of 5 tokens, 30 + 2 x 5 heads of 256 116 us over all 64, 86 so)
+        const int wide = high - low > 16 ? 5 : high - low > 8 ? 4 : 3;
+        for (int i = threadIdx.x; i < D << wide; i += 256) {
+          const int t = low + (i & ((1 << wide) - 1)), f = i >> wide;
+          if (t < high) out[f * p.out_feature + token0 + t] = *element(t, f);
         }
       } else {
         for (int i = threadIdx.x; i < T * (D / 8); i += 256) {
