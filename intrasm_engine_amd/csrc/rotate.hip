@@ -120,27 +120,40 @@ __device__ __forceinline__ void pair_of(const RotateParams& p, int plane, bool i
   f0 = plane < half && !interleaved ? plane : 2 * plane, f1 = plane < half && !interleaved ? plane + half : 2 * plane + 1;
 }
 
+// Cosines and sines of 64 tokens and up to 32 planes, by a workgroup into LDS: the table's rows are read where they are long and used where tokens are next
+// to each other.  (Each lane its own from memory: 7394 tokens of 16 heads of 256 74 us, 39 so.)
+constexpr int kTilePlanes = 32, kTilePitch = 65;   // (both sides without bank conflicts)
+struct RotationTile {
+  float c[kTilePlanes][kTilePitch], s[kTilePlanes][kTilePitch];
+  __device__ __forceinline__ void load(const RotateParams& p, int token0, int plane0, int planes) {   // a power of two
+    const int turned = p.rotation.features / 2;
+    for (int i = threadIdx.x; i < 64 * planes; i += 256) {
+      const int plane = i & (planes - 1), token = i / planes;
+      if (token0 + token >= p.tokens || plane0 + plane >= turned) continue;
+      float its, other;
+      load_plane(p.rotation, token0 + token, plane0 + plane, its, other);
+      c[plane][token] = its, s[plane][token] = p.back ? -other : other;
+    }
+    __syncthreads();
+  }
+};
+
 // Workgroups of 64 tokens x 32 planes: lanes have eight tokens each, eight of them and then the planes next to each other.
 template <int DTYPE>
 __global__ __launch_bounds__(256) void rotate_columns_kernel(RotateParams p, int interleaved) {
   typedef typename rotate_element<DTYPE>::type T;
   typedef Eight<DTYPE> Chunk;
-  const int token = blockIdx.x * 64 + threadIdx.x % 8 * 8, plane = blockIdx.y * 32 + threadIdx.x / 8;
+  __shared__ RotationTile tile;
+  tile.load(p, blockIdx.x * 64, blockIdx.y * kTilePlanes, kTilePlanes);
+  const int token = blockIdx.x * 64 + threadIdx.x % 8 * 8, plane = blockIdx.y * kTilePlanes + threadIdx.x / 8;
   if (token >= p.tokens || plane >= p.dim / 2) return;
   const bool turned = plane < p.rotation.features / 2;
   const int count = min(8, p.tokens - token);
   int f0, f1;
   pair_of(p, plane, interleaved, f0, f1);
   float c[8], s[8];
-  if (turned) {
-    const int axis = axis_of(p.rotation, plane);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int t = token + min(i, count - 1);
-      load_plane(p.rotation, RotationPlace(p.rotation, t), axis, plane, c[i], s[i]);
-      if (p.back) s[i] = -s[i];
-    }
-  }
+  for (int i = 0; i < 8; ++i) c[i] = tile.c[threadIdx.x / 8][threadIdx.x % 8 * 8 + i], s[i] = tile.s[threadIdx.x / 8][threadIdx.x % 8 * 8 + i];
   const T* x = static_cast<const T*>(p.x) + token;
   T* out = static_cast<T*>(p.out) + token;
   const int first = blockIdx.z * p.per_thread, end = min(p.heads, first + p.per_thread);
@@ -183,24 +196,23 @@ __global__ __launch_bounds__(256) void rotate_columns_kernel(RotateParams p, int
   }
 }
 
-// Workgroups of 64 tokens, a lane each, x up to 32 planes, in turn: the table's rows come once from memory for all of them.  (16 bytes a lane at any alignment:
+// Workgroups of 64 tokens, a lane each, x up to 32 planes, in turn.  (16 bytes a lane at any alignment:
 // 8191 tokens of 32 heads of 128 in fp16 66 us, 44 so.)
 template <int DTYPE>
 __global__ __launch_bounds__(256) void rotate_tokens_kernel(RotateParams p, int interleaved) {
   typedef typename rotate_element<DTYPE>::type T;
-  const int token = blockIdx.x * 64 + lane_id(), wave = uniform(threadIdx.x >> 6);
+  __shared__ RotationTile tile;
+  const int plane0 = blockIdx.y * p.planes, token = blockIdx.x * 64 + lane_id(), wave = uniform(threadIdx.x >> 6);
+  tile.load(p, blockIdx.x * 64, plane0, p.planes);
   if (token >= p.tokens) return;
-  const RotationPlace place(p.rotation, token);
-  const int first = blockIdx.z * p.per_thread, end = min(p.heads, first + p.per_thread), planes = min(p.dim / 2, (int)(blockIdx.y + 1) * p.planes);
+  const int first = blockIdx.z * p.per_thread, end = min(p.heads, first + p.per_thread), planes = min(p.dim / 2 - plane0, p.planes);
   const T* x = static_cast<const T*>(p.x) + token;
   T* out = static_cast<T*>(p.out) + token;
-  for (int plane = blockIdx.y * p.planes + wave; plane < planes; plane += 4) {
-    const bool turned = plane < p.rotation.features / 2;   // (uniform)
+  for (int i = wave; i < planes; i += 4) {
+    const bool turned = plane0 + i < p.rotation.features / 2;   // (uniform)
     int f0, f1;
-    pair_of(p, plane, interleaved, f0, f1);
-    float c = 1.f, s = 0.f;
-    if (turned) load_plane(p.rotation, place, axis_of(p.rotation, plane), plane, c, s);
-    if (p.back) s = -s;
+    pair_of(p, plane0 + i, interleaved, f0, f1);
+    const float c = tile.c[i][lane_id()], s = tile.s[i][lane_id()];
     for (int head = first; head < end; head += kColumnsAhead) {
       T a[kColumnsAhead], b[kColumnsAhead];
 #pragma unroll
@@ -236,7 +248,7 @@ __global__ __launch_bounds__(256) void rotate_single_kernel(RotateParams p, int 
   int f0, f1;
   pair_of(p, plane, interleaved, f0, f1);
   float c = 1.f, s = 0.f;
-  if (turned) load_plane(p.rotation, RotationPlace(p.rotation, token), axis_of(p.rotation, plane), plane, c, s);
+  if (turned) load_plane(p.rotation, token, plane, c, s);
   if (p.back) s = -s;
   const T* x = static_cast<const T*>(p.x) + token * p.x_strides[0];
   T* out = static_cast<T*>(p.out) + token * p.out_strides[0];
@@ -275,7 +287,7 @@ int launch(RotateParams p, bool interleaved, hipStream_t s) {
   } else if (p.dim % 2 == 0 && p.x_strides[0] == 1 && p.out_strides[0] == 1 && p.tokens >= 8) {
     const bool whole = columns_aligned(p.x, p.x_strides) && columns_aligned(p.out, p.out_strides);
     auto grid = [&] { return (long long)ceil_div(p.tokens, 64) * ceil_div(p.dim, 2 * p.planes); };
-    p.planes = 32;
+    p.planes = kTilePlanes;
     // (a wavefront's planes come one after the other: fewer of them where there are too few workgroups; 2001 tokens of 8 heads 17.3 us by 32)
     while (!whole && p.planes > 4 && grid() * ceil_div(p.heads, kColumnsAhead) < 1024) p.planes /= 2;
     p.per_thread = heads_of_a_thread(p, grid(), kColumnsAhead);

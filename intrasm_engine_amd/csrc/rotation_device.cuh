@@ -51,11 +51,14 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 
 // Cosine and sine of one plane.
 __device__ __forceinline__ int axis_of(const Rotation& r, int plane) { return r.axes > 1 ? (int)(axis_word(r, plane / 32) >> (plane % 32 * 2)) & 3 : 0; }
-__device__ __forceinline__ void load_plane(const Rotation& r, const RotationPlace& place, int axis, int plane, float& c, float& s) {
-  const RotationRow row(r, place.on(axis));
+__device__ __forceinline__ void load_plane_at(const Rotation& r, int position, int plane, float& c, float& s) {
+  const RotationRow row(r, position);
   const float* t = r.table + (size_t)row.row * r.features + plane;
   c = t[0], s = t[r.features / 2];
   if (!row.known) c = s = NAN;
+}
+__device__ __forceinline__ void load_plane(const Rotation& r, int token, int plane, float& c, float& s) {
+  load_plane_at(r, r.positions[axis_of(r, plane) * r.axis_stride + token], plane, c, s);
 }
 
 // ... of planes 8 u .. 8 u + 7, 16 bytes at a time where they are of one axis.
@@ -80,7 +83,7 @@ struct Planes {
       const unsigned axes = r.axes > 1 ? (unsigned)(axis_word(r, u / 4) >> (u % 4 * 16)) & 0xFFFFu : 0u;
       if (__ballot(axes != (axes & 3u) * 0x5555u)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_plane(r, place, axes >> (2 * i) & 3u, 8 * u + i, c[i], s[i]);
+        for (int i = 0; i < 8; ++i) load_plane_at(r, place.on(axes >> (2 * i) & 3u), 8 * u + i, c[i], s[i]);
         return;
       }
       const RotationRow row(r, place.on(axes & 3u));
