@@ -7,7 +7,7 @@
 //             are not 16-byte aligned, planes of a token
 //   single    everything else: a thread has a plane of a token
 // Measured: 30001 tokens of 32 heads of 128 in bf16, 64 features by three axes in turn, rows 114 us = 4.4 TB/s read and written (with streaming loads 123, with
-// streaming stores 133); 8192 tokens in fp16, columns 31 us = 4.4; 300 tokens of 16 heads of 64 4.1.
+// streaming stores 133); 8192 tokens in fp16, columns 30 us = 4.6; 300 tokens of 16 heads of 64 4.1.
 #include "rotation_host.h"
 
 namespace iex {
