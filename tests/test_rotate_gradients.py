@@ -1,0 +1,26 @@
+"""Which gradients a rotation has, without a GPU: tensors of a device that nothing stands behind (a call that passes the checks ends at their memory)."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import intrasm_engine_amd  # noqa: F401
+
+PASSED = "data is not allocated"
+
+
+@pytest.fixture
+def operands():
+    with FakeTensorMode():
+        yield torch.empty(4, 2, 64, device="cuda"), torch.empty(9, 64, device="cuda"), torch.empty(4, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("learned", [False, True])
+@pytest.mark.parametrize("trained", [False, True])
+def test_a_table_that_requires_a_gradient(operands, trained, learned):
+    """It gets none, so the call is refused, whether x requires one or not; without gradients it is a table like any other."""
+    x, table, positions = operands
+    x.requires_grad_(trained), table.requires_grad_(learned)
+    with pytest.raises(RuntimeError, match="the table has no gradient" if learned else PASSED):
+        torch.ops.iex_ops.rotate(x, table, positions)
+    with torch.no_grad(), pytest.raises(RuntimeError, match=PASSED):
+        torch.ops.iex_ops.rotate(x, table, positions)
