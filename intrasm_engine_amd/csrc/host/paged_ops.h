@@ -20,8 +20,14 @@ void check_ints(const Tensor& t, const Tensor& with, int64_t dim, const char* op
   TORCH_CHECK(dim == 1 ? t.is_contiguous() : t.size(-1) <= 1 || t.stride(-1) == 1, name, " must have contiguous rows");
 }
 
+// A tangent (forward mode) would be lost: nothing below the operators looks for one.
+void check_no_tangent(const Tensor& t, const char* op) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), op, " has no forward-mode derivative: unpack the dual tensor");
+}
+
 // Nothing here has a gradient: tokens are generated with it.
 void check_no_gradient(const Tensor& t, const char* op) {
+  check_no_tangent(t, op);
   TORCH_CHECK(!at::GradMode::is_enabled() || !t.requires_grad(), op, " has no gradient: call it under torch.no_grad()");
 }
 

@@ -732,6 +732,7 @@ struct TrainableRotate : torch::autograd::Function<TrainableRotate> {
 };
 
 Tensor trainable_rotate(const Tensor& x, const Tensor& rotation, const Tensor& positions, at::OptionalIntArrayRef sections, bool in_turn, bool interleaved, bool back) {
+  for (const Tensor* t : {&x, &rotation}) check_no_tangent(*t, "rotate");
   // (here: below apply() nothing requires a gradient any more)
   TORCH_CHECK(!at::GradMode::is_enabled() || !rotation.requires_grad(), "rotate: the table has no gradient, only x has: pass rotation.detach()");
   if (!at::GradMode::is_enabled() || !x.requires_grad()) return rotated(x, rotation, positions, sections, in_turn, interleaved, back);

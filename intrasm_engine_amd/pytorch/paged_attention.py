@@ -2,7 +2,7 @@
 dropped that got least attention.
 
 Operators under ``torch.ops.iex_ops`` (``csrc/host/paged_ops.h``), on the current stream, capturable, without a gradient but for
-``rotate``'s of x (its table has none: a table that requires one is refused):
+``rotate``'s of x (its table has none: a table that requires one is refused), none with forward mode (dual tensors are refused):
 
     kv_append_(k, v, keys, values, page_table, lengths, offsets=None, q=None, rotation=None, interleaved=False, bounds=None,
                key_exponents=None, value_exponents=None, positions=None, sections=None, in_turn=False) -> q, rotated (None without q)

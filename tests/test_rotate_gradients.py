@@ -1,6 +1,7 @@
 """Which gradients a rotation has, without a GPU: tensors of a device that nothing stands behind (a call that passes the checks ends at their memory)."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 import intrasm_engine_amd  # noqa: F401
@@ -24,3 +25,19 @@ def test_a_table_that_requires_a_gradient(operands, trained, learned):
         torch.ops.iex_ops.rotate(x, table, positions)
     with torch.no_grad(), pytest.raises(RuntimeError, match=PASSED):
         torch.ops.iex_ops.rotate(x, table, positions)
+
+
+@pytest.mark.parametrize("dual", ["x", "table"])
+@pytest.mark.parametrize("trained", [False, True])
+def test_forward_mode(operands, trained, dual):
+    """No result without the tangent that it should have: a dual operand is refused, gradients or not; what is not differentiated passes."""
+    x, table, positions = operands
+    x.requires_grad_(trained)
+    rotate = torch.ops.iex_ops.rotate
+    with forward.dual_level():
+        given = [forward.make_dual(t, t.detach()) if name == dual else t for name, t in (("x", x), ("table", table))]
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                rotate(*given, positions)
+        with pytest.raises(RuntimeError, match=PASSED):
+            rotate(*(forward.unpack_dual(t).primal for t in given), positions)
