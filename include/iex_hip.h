@@ -550,10 +550,15 @@ int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, con
  * Other sequences stay as they are, kept has their tokens 0 .. lengths[s] - 1 and -1 behind them.  A sequence of more than `keep` tokens with pages
  * given back among those it uses is passed over: nothing changes, kept is -1.  Rows move in place: a sequence that loses tokens must have its
  * pages for itself (no other one reads right what it shares with it, and a page that two such sequences, or one twice, have holds what either wrote).
- * workspace: iex_evict_tokens_workspace_bytes, 256-byte aligned. */
+ * workspace: iex_evict_tokens_workspace_bytes, 256-byte aligned, for one call at a time: rows wait in the kernel for rows that are to be read before.  Waits
+ * are bounded; where one gives up, as calls that share a workspace at the same time can make it, the places that its rows should have come to hold NaN, keys and
+ * values (rows that others were yet to read from there can be NaN too), and kept has -2 there; weights and lengths are as if they had moved.
+ * iex_evict_tokens_within: `tries` (0 .. 2^20; iex_evict_tokens: 2^20, about a second) is how often a wait looks before it gives up. */
 size_t iex_evict_tokens_workspace_bytes(const iex_paged_cache* cache, int keep);
 int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, float* weights, int keep, int recent, int first, int* kept,
                      void* workspace, size_t workspace_bytes, void* stream);
+int iex_evict_tokens_within(const iex_paged_cache* cache, int* lengths, float* weights, int keep, int recent, int first, int* kept,
+                            int tries, void* workspace, size_t workspace_bytes, void* stream);
 
 /* In-place row-wise softmax over the stored entries of a CSR matrix:
  * values[z, j] = exp(scale*values[z, j] - max_row) / sum_row.  values is (batch, nnz).

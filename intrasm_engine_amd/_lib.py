@@ -105,6 +105,7 @@ SIGNATURES = {
     "iex_select_pages": (_i, [_cache, _i, _vp, _strides, _i, _i, _i, _vp, _vp, _c.c_size_t, _vp]),
     "iex_evict_tokens_workspace_bytes": (_c.c_size_t, [_cache, _i]),
     "iex_evict_tokens": (_i, [_cache, _vp, _vp, _i, _i, _i, _vp, _vp, _c.c_size_t, _vp]),
+    "iex_evict_tokens_within": (_i, [_cache, _vp, _vp, _i, _i, _i, _vp, _i, _vp, _c.c_size_t, _vp]),
     "iex_csr_softmax": (_i, [_i, _i, _i, _vp, _vp, _vp, _f, _vp, _i]),
     "iex_gemm": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _ll, _ll, _ll, _vp]),
     "iex_gemm_ws": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _ll, _ll, _ll, _vp, _vp, _c.c_size_t]),

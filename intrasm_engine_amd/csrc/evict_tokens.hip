@@ -8,8 +8,8 @@
 // at place i or behind it, so what chunk c writes, places c * chunk and on, is only ever read by itself and by chunks before it (the list's stretch
 // with tokens there ends before its own); all of a chunk's rows are in registers before its first write, and it writes when the chunks before it that
 // read there, two at most, have said that theirs are too.  Chunks are drawn by ticket: the one that is waited for has been drawn before, by a workgroup that is
-// running and that waits for nobody before it has read, so every wait ends.  (It is bounded all the same, to about a second: calls that share a workspace at the
-// same time, which they must not, leave rows unmoved and do not hang.)
+// running and that waits for nobody before it has read, so every wait ends.  It is bounded all the same, to about a second, for calls that share a workspace at
+// the same time, which they must not: a chunk that gives up leaves NaN in the places that it should have written, and -2 in the list.
 //
 // What bounds it: memory, kept rows read and written once: 64 sequences of 1500 .. 4224 tokens to 2048, 8 key heads of 128 in 16 bits 149 us = 5.1 TB/s,
 // selection 16; 131071 tokens to 32768, every fourth row of 256 bytes, 66 us = 4.1 TB/s, selection 32 in five launches (by one workgroup a row, whose CU reads
@@ -36,11 +36,12 @@ struct EvictParams {
   unsigned* histograms;   // slices: two of (rows, slices, 256)
   int4* found;            // ... (rows, slices) what of the threshold is known, how many that agree with it are wanted, how many before the slice are above it
   int slices;
+  int tries;              // of a wait
 };
 
 constexpr int kEvictThreads = 1024, kEvictKept = 32768;   // ... whose weights fit in LDS
 constexpr int kEvictSlice = 8192;                         // tokens
-constexpr int kEvictTries = 1 << 20;                      // of a wait
+constexpr int kEvictTries = 1 << 20;                      // of a wait: about a second
 
 // Four words from place i on of a 16-byte aligned row of `used`, 0 behind it.
 __device__ __forceinline__ u32x4 four_of(const unsigned* row, int i, int used) {
@@ -299,19 +300,24 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
     static_assert(T <= 256, "a thread has a token's exponents");
     if (tid < T) ke = key_exponents[exponent_at(from[tid])], ve = value_exponents[exponent_at(from[tid])];
   }
-  // who reads what this chunk writes: tokens before it that are kept from places low .. high of the list
-  const int* const before = p.before + (size_t)row * (p.chunks + 1);
-  const int low = before[chunk], high = first + T >= length ? first : min(before[chunk + 1], first);
+  const EvictReaders readers = evict_readers(chunk, T, length, p.before + (size_t)row * (p.chunks + 1));
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   int* const flags = p.flags + (size_t)row * p.chunks;
   if (tid == 0) __hip_atomic_store(flags + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   bool read = true;
-  if (low < high && tid <= (high - 1) / T - low / T) {
-    for (int tries = 0; !(read = __hip_atomic_load(flags + low / T + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0) && tries < kEvictTries; ++tries)
-      __builtin_amdgcn_s_sleep(2);
+  if (tid < readers.count) {
+    read = false;
+    for (int tries = 0; tries < p.tries && !read; ++tries) {
+      if (tries) __builtin_amdgcn_s_sleep(2);
+      read = __hip_atomic_load(flags + readers.first + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+    }
   }
-  if (!__syncthreads_and(read)) return;
+  if (!__syncthreads_and(read)) {   // given up: NaN in the chunk's places, of every type, and the list says so (nobody else reads its entries)
+    for (int i = tid; i < count; i += 256) p.kept[(size_t)row * p.keep + first + i] = kEvictAbandoned;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) k[i] = v[i] = u32x4{~0u, ~0u, ~0u, ~0u};
+  }
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int at = line + i * (256 / LANES);
@@ -418,11 +424,17 @@ extern "C" size_t iex_evict_tokens_workspace_bytes(const iex_paged_cache* cache,
 
 extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, float* weights, int keep, int recent, int first, int* kept, void* workspace,
                                 size_t workspace_bytes, void* stream) {
+  return iex_evict_tokens_within(cache, lengths, weights, keep, recent, first, kept, iex::kEvictTries, workspace, workspace_bytes, stream);
+}
+
+extern "C" int iex_evict_tokens_within(const iex_paged_cache* cache, int* lengths, float* weights, int keep, int recent, int first, int* kept, int tries, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
   using namespace iex;
   trail_reset();
   if (int rc = check_paged_cache(cache, "evict_tokens", true)) return rc;
   IEX_REQUIRE(keep > 0 && first >= 0 && recent >= 0 && (long long)first + recent <= keep, IEX_ERR_BAD_ARGUMENT,
               "evict_tokens: at least one token, the first and recent ones that are always kept among them (keep=%d first=%d recent=%d)", keep, first, recent);
+  IEX_REQUIRE(tries >= 0 && tries <= kEvictTries, IEX_ERR_BAD_ARGUMENT, "evict_tokens: a wait of 0 to %d looks (%d)", kEvictTries, tries);
   if (cache->seqs == 0 || cache->kv_heads == 0) return 0;
   IEX_REQUIRE(lengths == cache->lengths && kept && (weights || cache->table_width == 0), IEX_ERR_BAD_ARGUMENT, "evict_tokens: null pointer argument");
   IEX_REQUIRE(aligned(weights, 16), IEX_ERR_UNSUPPORTED, "evict_tokens: the weights must be 16-byte aligned");
@@ -436,7 +448,7 @@ extern "C" int iex_evict_tokens(const iex_paged_cache* cache, int* lengths, floa
   IEX_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= l.bytes, IEX_ERR_BAD_ARGUMENT, "evict_tokens: needs a 256-byte aligned workspace of %zu bytes", l.bytes);
   EvictParams p{};
   p.cache = paged_params(*cache);
-  p.keep = keep, p.first = first, p.recent = recent, p.chunks = (int)l.chunks;
+  p.keep = keep, p.first = first, p.recent = recent, p.chunks = (int)l.chunks, p.tries = tries;
   p.lengths = lengths, p.weights = weights, p.kept = kept, p.bounds = static_cast<unsigned short*>(cache->bounds);
   char* const ws = static_cast<char*>(workspace);
   p.tokens = reinterpret_cast<int*>(ws), p.tickets = reinterpret_cast<int*>(ws + l.tickets), p.flags = reinterpret_cast<int*>(ws + l.flags);

@@ -106,4 +106,17 @@ IEX_HD unsigned select_key(unsigned score_bits) {
   return score_bits & 0x80000000u ? ~score_bits : score_bits | 0x80000000u;
 }
 
+// ---- eviction ---------------------------------------------------------------------------------------------------------
+// A list of kept tokens, ascending, moves to places 0, 1 .. of its sequence in chunks of `size`.  Who reads what a chunk writes: itself and the chunks before
+// it, of which those have to have read that hold the tokens before the chunk's own that are kept from the places it writes.  before[i]: how many of the kept
+// tokens are before place i * size (of places within the sequence).  At most two chunks: as many tokens, one behind the other in the list, as a chunk has.
+struct EvictReaders {
+  int first, count;   // chunks
+};
+IEX_HD EvictReaders evict_readers(int chunk, int size, int length, const int* before) {
+  const int first = chunk * size, low = before[chunk], upto = length - first <= size ? first : before[chunk + 1], high = upto < first ? upto : first;
+  return low < high ? EvictReaders{low / size, (high - 1) / size - low / size + 1} : EvictReaders{0, 0};
+}
+constexpr int kEvictAbandoned = -2;   // in the list, at the places of a chunk that gave up waiting
+
 }  // namespace iex

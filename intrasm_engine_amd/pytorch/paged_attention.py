@@ -106,5 +106,6 @@ class KVCache:
         largest ``weights`` stay (of two that are equal the earlier) and move up, in order, within the sequence's own pages, which it must share
         with nobody; ``lengths``, ``weights`` and bounds follow.  Returns where they were, (sequences, kv_heads, keep), -1 behind shorter sequences.  New
         tokens then need ``positions`` of their own.  A sequence with pages given back is passed over (all -1).  Pages that no sequence needs any
-        more are the caller's to give to others."""
+        more are the caller's to give to others.  (-2, and NaN in the cache: rows whose move was given up, as graphs that share memory can make it if they
+        are replayed at the same time.)"""
         return ops.evict_tokens_(self.keys, self.values, page_table, lengths, weights, keep, recent, first, self.bounds, self.key_exponents, self.value_exponents)
