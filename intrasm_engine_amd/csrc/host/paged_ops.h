@@ -4,6 +4,7 @@
 
 int as_int(int64_t x, const char* op) {
   TORCH_CHECK(x <= std::numeric_limits<int>::max(), op, ": a dimension of ", x, " is too large");
+  TORCH_CHECK(x >= std::numeric_limits<int>::min(), op, ": a dimension of ", x, " is too small");
   return (int)x;
 }
 
