@@ -547,6 +547,7 @@ int iex_select_pages(const iex_paged_cache* cache, int heads, const void* q, con
  * with the largest weights[s, g, t] (seqs, kv_heads, table_width * page_size; 16-byte aligned; ties: the earlier token; a NaN is larger than all).  Their rows move, in order,
  * to the sequence's first `keep` places, their weights with them; the weights of places behind are 0 then, lengths[s] is `keep`, bounds (if the
  * cache has them) are those of the tokens that the pages then hold.  kept: (seqs, kv_heads, keep), where the tokens were, ascending.
+ * (Caches of several layers that go by the same lengths: a copy of them for each call but the last, else the first leaves nothing to do to the others.)
  * Other sequences stay as they are, kept has their tokens 0 .. lengths[s] - 1 and -1 behind them.  A sequence of more than `keep` tokens with pages
  * given back among those it uses is passed over: nothing changes, kept is -1.  Rows move in place: a sequence that loses tokens must have its
  * pages for itself (no other one reads right what it shares with it, and a page that two such sequences, or one twice, have holds what either wrote).

@@ -191,8 +191,8 @@ class SparseDecoderLayer:
         """One new token of every sequence: x (hidden, sequences) fp16 -> same shape.  Its key and value go into the cache (``lengths``
         counts it) and it attends to all of its sequence, or to the ``pages`` pages that its query can score highest with (a cache
         with bounds; the page with the new token is always among them, and the first one if there are more).  ``weights`` (:meth:`KVCache.new_weights`): what
-        tokens get of attention is added to them, for :meth:`KVCache.evict_` between steps, behind which new tokens need ``positions``.  Capturable: a graph
-        follows ``page_table``, ``lengths`` and ``positions``."""
+        tokens get of attention is added to them, for :meth:`KVCache.evict_` between steps (of several layers: by a copy of ``lengths`` each but the last, which it
+        cuts), behind which new tokens need ``positions``.  Capturable: a graph follows ``page_table``, ``lengths`` and ``positions``."""
         if pages < 0:
             raise ValueError("decode: pages must not be negative")
         if pages and weights is not None:

@@ -104,7 +104,8 @@ class KVCache:
     def evict_(self, page_table, lengths, weights, keep: int, recent: int, first: int = 0):
         """Sequences of more than ``keep`` tokens lose those that got least: of every key head's the ``first``, the ``recent`` and the ones with the
         largest ``weights`` stay (of two that are equal the earlier) and move up, in order, within the sequence's own pages, which it must share
-        with nobody; ``lengths``, ``weights`` and bounds follow.  Returns where they were, (sequences, kv_heads, keep), -1 behind shorter sequences.  New
+        with nobody; ``lengths``, ``weights`` and bounds follow.  ``lengths`` are cut in place: the caches of several layers, which go by one ``lengths``, are
+        cut by a copy each (``lengths.clone()``) but the last, else the first leaves nothing to do to the others.  Returns where they were, (sequences, kv_heads, keep), -1 behind shorter sequences.  New
         tokens then need ``positions`` of their own.  A sequence with pages given back is passed over (all -1).  Pages that no sequence needs any
         more are the caller's to give to others.  (-2, and NaN in the cache: rows whose move was given up, as graphs that share memory can make it if they
         are replayed at the same time.)"""
