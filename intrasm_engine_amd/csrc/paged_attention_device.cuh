@@ -57,15 +57,22 @@ __device__ __forceinline__ size_t account_place(const PagedAttentionParams& p, i
 // scores are NaN or infinite leaves no trace in what it does not attend to.
 constexpr unsigned kNoScore = 0xFFFFFFFFu;
 
+// exp2((score - maximum) * scale) is taken as exp2(score * scale - maximum * scale) in one fused step, whose second product is rounded: to 2^-8 at 2^16, by
+// more where it is larger, up to what leaves 16 bits, or 32 (fp16 heads of 128 of values around 10^4: infinite results).  Beyond, the difference comes first.
+constexpr float kFarShift = 65536.f;
+
 // Four tokens' scores of one query as weights: exp2((score - maximum) * scale) / sum.
 struct QueryWeights {
-  float shift, share;
-  __device__ __forceinline__ QueryWeights(float top, float sum, float scale_log2) : shift(sum == -1.f ? 0.f : -top * scale_log2), share(sum == -1.f ? 0.f : 1.f / sum) {}
-  __device__ __forceinline__ QueryWeights(float2 both) : shift(both.x), share(both.y) {}
+  float top, share;
+  __device__ __forceinline__ QueryWeights(float maximum, float sum) : top(sum == -1.f ? 0.f : maximum), share(sum == -1.f ? 0.f : 1.f / sum) {}
+  __device__ __forceinline__ QueryWeights(float2 both) : top(both.x), share(both.y) {}
   __device__ __forceinline__ void add(f32x4& to, const f32x4& score, float scale_log2) const {
+    const float product = -top * scale_log2;
+    const bool far = fabsf(product) > kFarShift;
+    const float first = far ? top : 0.f, shift = far ? 0.f : product;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float more = fmaf(__builtin_amdgcn_exp2f(fmaf(score[r], scale_log2, shift)), share, to[r]);
+      const float more = fmaf(__builtin_amdgcn_exp2f(fmaf(score[r] - first, scale_log2, shift)), share, to[r]);
       to[r] = __float_as_uint(score[r]) == kNoScore ? to[r] : more;
     }
   }
@@ -427,7 +434,15 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
           for (int r = 0; r < 4; ++r) o[j][r] *= keep;
       }
     }
-    const float shift = top == -INFINITY ? 0.f : -top * p.scale_log2;
+    float shift = top == -INFINITY ? 0.f : -top * p.scale_log2;
+    if (__ballot(fabsf(shift) > kFarShift)) {   // (of some query)
+      const bool far = fabsf(shift) > kFarShift;
+#pragma unroll
+      for (int a = 0; a < SUB; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[a][r] -= far ? top : 0.f;
+      shift = far ? 0.f : shift;
+    }
 #pragma unroll
     for (int a = 0; a < SUB; ++a) {
 #pragma unroll
@@ -532,8 +547,8 @@ __global__ __launch_bounds__(WAVES * 64, paged_simd_waves(D)) void paged_attenti
       p.out[seq * p.out_strides[0] + head * p.out_strides[1] + d * p.out_strides[2]] = f32_to_16(any ? acc / (all * up) : 0.f, BF16);
       if (WEIGH && d == 0 && !p.at_once) *reinterpret_cast<float2*>(p.row_stats + ((size_t)seq * p.heads + head) * 2) = float2{m, any ? all : -1.f};
       if (WEIGH && d == 0 && p.at_once) {
-        const QueryWeights mine(m, any ? all : -1.f, p.scale_log2);
-        shares[row] = float2{mine.shift, mine.share};
+        const QueryWeights mine(m, any ? all : -1.f);
+        shares[row] = float2{mine.top, mine.share};
       }
     } else {
       const size_t to = (size_t)blockIdx.x * p.pitch + row;
@@ -668,8 +683,8 @@ __global__ __launch_bounds__(256) void paged_account_kernel(PagedAttentionParams
       sum = wave_sum(mine);
       if (!__ballot(counts)) sum = -1.f;
     }
-    const QueryWeights its(top, sum, p.scale_log2);
-    if (lane == 0) shares[i] = float2{its.shift, its.share};
+    const QueryWeights its(top, sum);
+    if (lane == 0) shares[i] = float2{its.top, its.share};
   }
   __syncthreads();
   const float* from = account_scores(p, seq, kv_head);
