@@ -315,8 +315,13 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   }
   if (!__syncthreads_and(read)) {   // given up: NaN in the chunk's places, of every type, and the list says so (nobody else reads its entries)
     for (int i = tid; i < count; i += 256) p.kept[(size_t)row * p.keep + first + i] = kEvictAbandoned;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) k[i] = v[i] = u32x4{~0u, ~0u, ~0u, ~0u};
+#pragma unroll 1
+    for (int at = line; at < count; at += 256 / LANES) {
+      const u32x4 nan = {~0u, ~0u, ~0u, ~0u};
+      *reinterpret_cast<u32x4*>(keys + row_at(to[at], c.key_page) + piece) = nan;
+      *reinterpret_cast<u32x4*>(values + row_at(to[at], c.value_page) + piece) = nan;
+    }
+    return;
   }
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
