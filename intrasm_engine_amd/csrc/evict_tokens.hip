@@ -11,9 +11,10 @@
 // running and that waits for nobody before it has read, so every wait ends.  It is bounded all the same, to about a second, for calls that share a workspace at
 // the same time, which they must not: a chunk that gives up leaves NaN in the places that it should have written, and -2 in the list.
 //
-// What bounds it: memory, kept rows read and written once: 64 sequences of 1500 .. 4224 tokens to 2048, 8 key heads of 128 in 16 bits 149 us = 5.1 TB/s,
-// selection 16; 131071 tokens to 32768, every fourth row of 256 bytes, 66 us = 4.1 TB/s, selection 32 in five launches (by one workgroup a row, whose CU reads
-// the weights again in every round, 143); 700 tokens to 512, 32 key heads 6.7 and 7.1.
+// What bounds it: memory, kept rows read and written once: 64 sequences of 1500 .. 4224 tokens to 2048, 8 key heads of 128 in 16 bits 150 us = 5.0 TB/s,
+// selection 17; 131071 tokens to 32768, every fourth row of 256 bytes, 67 us = 4.1 TB/s, selection 32 in five launches (by one workgroup a row, whose CU reads
+// the weights again in every round, 143); 700 tokens to 512, 32 key heads 6.4, selection 6.9.  The 64 sequences with weights spread evenly 134 us, in e4m3
+// 66; bounds of their pages another 126, e4m3 86 (evict_bounds_kernel).
 #include "paged_cache_host.h"
 #include "select_device.cuh"
 
@@ -336,7 +337,8 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   }
 }
 
-// Bounds of the pages that a cut row's tokens are in now, a workgroup each: a thread has a feature and tokens SIDE apart; they meet in LDS.
+// Bounds of the pages that a cut row's tokens are in now, a workgroup each: a thread has a feature and tokens SIDE apart; they meet in LDS.  Bound by its loads,
+// of an element a lane each (64 sequences to 2048 tokens, 8 key heads of 128: 126 us for 189 MB, 1.5 TB/s; e4m3 86).
 template <bool BF16, int D, bool E8>
 __global__ __launch_bounds__(256) void evict_bounds_kernel(EvictParams p) {
   constexpr int SIDE = 256 / D;

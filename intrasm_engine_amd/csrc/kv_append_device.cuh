@@ -12,7 +12,8 @@
 // -> store is the longest chain of loads.  Measured: 16 prompts of 512 tokens, 3 x 32 heads of 128, feature-major 79 us = 5.1 TB/s read
 // and written; 23 of 3 .. 5001 tokens, 32 + 2 x 8 heads, into e4m3 with bounds 96 us = 4.2 (waiting for a row's maximum, vector
 // units 36 %); a step of one sequence of 3 x 32 heads 3.0 us, of 64 of 32 + 2 x 8 heads with bounds 4.2.  Positions given on
-// three axes: 4 prompts of 2200 .. 5001 tokens of 32 + 2 x 8 heads 65 us = 5.3, a step of 64 sequences 3.9.
+// three axes: 4 prompts of 2200 .. 5001 tokens of 32 + 2 x 8 heads 65 us = 5.3, a step of 64 sequences 3.9; the prompts with planes dealt to the axes
+// in turn, each plane's cosine and sine a load of its own, 75; feature-major, where sequences begin off a chunk, 130, in turn 175.
 #pragma once
 #include "rotation_device.cuh"
 

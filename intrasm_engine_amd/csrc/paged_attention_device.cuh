@@ -645,7 +645,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttentionParams p)
 
 // The second launch of attention that keeps account: the first workgroups add the weights of 1024 tokens at a time of a sequence and key head, `side` of
 // them taking turns; the last `joins` join parts (of rows that were cut: in one launch with the weights, since neither waits for the other; each works out the
-// rows' maxima and sums from the parts').  64 x 2049 .. 4224 tokens, 32 heads over 8 14.9 us (the joins first: 17.4).
+// rows' maxima and sums from the parts').  64 x 2049 .. 4224 tokens, 32 heads over 8 15.2 us (with the joins first 17.4, when this order took 14.9).
 constexpr int kAccountTokens = 1024;
 template <bool BF16, int D, bool E8>
 __global__ __launch_bounds__(256) void paged_account_kernel(PagedAttentionParams p, int joins, int side) {

@@ -7,7 +7,8 @@
 //             are not 16-byte aligned, planes of a token
 //   single    everything else: a thread has a plane of a token
 // Measured: 30001 tokens of 32 heads of 128 in bf16, 64 features by three axes in turn, rows 114 us = 4.4 TB/s read and written (with streaming loads 123, with
-// streaming stores 133); 8192 tokens in fp16, columns 30 us = 4.6; 300 tokens of 16 heads of 64 4.1.
+// streaming stores 133); 8192 tokens in fp16, columns 30 us = 4.6; 300 tokens of 16 heads of 64 4.1.  In fp32, 30001 tokens of 32 heads of 128, forward or back:
+// rows 215 us = 4.6 TB/s, columns (30000 tokens) 229 = 4.3, tokens at other alignments 312 = 3.2.
 #include "rotation_host.h"
 
 namespace iex {
@@ -122,7 +123,7 @@ __device__ __forceinline__ void pair_of(const RotateParams& p, int plane, bool i
 
 // Cosines and sines of 64 tokens and up to 32 planes, by a workgroup into LDS: the table's rows are read where they are long and used where tokens are next
 // to each other.  (Each lane its own from memory: 7394 tokens of 16 heads of 256 74 us, 39 so.)
-constexpr int kTilePlanes = 32, kTilePitch = 65;   // (both sides without bank conflicts)
+constexpr int kTilePlanes = 32, kTilePitch = 65;   // (without bank conflicts where it is read; writes are two lanes a bank, by fewer planes up to eight)
 struct RotationTile {
   float c[kTilePlanes][kTilePitch], s[kTilePlanes][kTilePitch];
   __device__ __forceinline__ void load(const RotateParams& p, int token0, int plane0, int planes) {   // a power of two
